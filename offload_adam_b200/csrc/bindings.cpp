@@ -460,6 +460,7 @@ struct PyEngine {
 }  // namespace
 
 void bind_loss(py::module_& m);
+void bind_linear_ce(py::module_& m);
 void bind_model(py::module_& m);
 void bind_quant(py::module_& m);
 void bind_symm(py::module_& m);
@@ -563,6 +564,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
       .def("reset_counters", &PyEngine::reset_counters);
 
   bind_loss(m);
+  bind_linear_ce(m);
   bind_model(m);
   bind_quant(m);
   bind_symm(m);

@@ -1,0 +1,720 @@
+// Softmax cross entropy of h W^T against labels, in pieces of the vocabulary, without the logits.
+//
+//   z_ij = sum_k h_ik W_jk        lse_i = log sum_j exp z_ij        loss_i = lse_i - z_i,label
+//   d_ij = (exp(z_ij - lse_i) - [j = label_i]) g_i      dh = d W      dW = d^T h
+//
+// Rows whose label is ignored take no part: the others are packed first, so their work is saved
+// and nothing that stands in them (a padded batch's NaN) reaches a sum.
+//
+// Forward: one product whose epilogue keeps, per row and 128 words, the maximum and the sum of
+// exponentials (8 bytes for 256 bytes of bf16 logits), and a small kernel that joins them.
+// Backward, for each piece of the vocabulary: the product again, whose epilogue writes the
+// gradient of the piece's logits in bf16, and one launch for both products that read it; dh is
+// summed over the pieces in fp32 and rounded once.  Where the scale of the incoming gradient is one
+// number it is applied to the fp32 sums, so d holds p - [j = label] as it is: its largest
+// entries, near -1, lose least.
+//
+// All three products are one pipeline: a CTA pair computes a 256 x 256 tile with tcgen05 (each CTA
+// 128 rows, half of B each), TMA fills six stages of 64 inner values, two accumulators in tensor
+// memory let the epilogue of a tile overlap the products of the next, one pair per two SMs
+// takes tiles in turn.
+#include <cudaTypedefs.h>
+
+#include "common.cuh"
+#include "linear_ce.h"
+#include "umma.cuh"
+
+namespace oab {
+namespace {
+
+using namespace umma;
+
+constexpr int kTile = kLceTile;
+constexpr int kInner = 64;                              // inner values of a stage: 128 bytes
+constexpr int kStages = 6;
+constexpr int kHalfBytes = 128 * kInner * 2;            // one CTA's part of an operand's stage
+constexpr int kStageBytes = 2 * kHalfBytes;
+constexpr int kSmemBytes = kStages * kStageBytes + 1024;  // stages start on 1024 bytes
+constexpr int kEpilogueWarps = 8;
+constexpr int kGemmThreads = 64 + 32 * kEpilogueWarps;
+constexpr int kGroup = 16;  // row tiles that share a column tile in turn: 4096 rows of h stay in L2
+
+enum Pass { kStats = 0, kLogitGrad = 1, kGrads = 2 };
+
+struct GemmParams {
+  CUtensorMap a, b;    // kStats, kLogitGrad: packed rows and W.  kGrads: d and W, for dh
+  CUtensorMap a2, b2;  // kGrads: d and packed rows, for dW
+  const int* count;
+  int64_t rows;        // capacity of the per-row arrays
+  int64_t padded;
+  int hidden;
+  int64_t vocab;
+  int64_t word0;       // first word of the piece
+  int words;           // and how many
+  int64_t* report;
+  const int* label;
+  // kStats
+  float2* part;
+  float* picked;
+  // kLogitGrad
+  const float* lse;
+  const float* row_g;  // by row, or null
+  uint16_t* d;
+  int64_t pitch;
+  // kGrads
+  const int* index;
+  const float *inv, *g;  // each may be null (1)
+  float* acc;
+  uint16_t *gh, *gw;
+  int splits;
+  int first, last;
+};
+
+__device__ __forceinline__ float exp_of(float x) {  // relative error below 2^-21 for |x| < 20
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(__fmul_rn(x, 1.4426950408889634f)));
+  return r;
+}
+__device__ __forceinline__ float finite_shift(float m) { return m == -INFINITY ? 0.f : m; }
+
+struct Tile {
+  int kind;       // kGrads: 0 dh, 1 dW
+  int m, n;       // first row and column
+  int k0, steps;  // first inner value, stages
+  int split;
+};
+
+// Tiles of a pass and the t-th of them.  Column tiles turn slower than up to kGroup row tiles.
+struct Plan {
+  int mt, nt, per_split, dh_tiles, wt, ht, total, k_steps, row_steps;
+  template <int PASS>
+  __device__ __forceinline__ void make(const GemmParams& p, int n_rows) {
+    mt = (n_rows + kTile - 1) / kTile;
+    if (PASS == kGrads) {
+      ht = (p.hidden + kTile - 1) / kTile;
+      nt = ht;
+      wt = p.gw != nullptr ? (p.words + kTile - 1) / kTile : 0;
+      per_split = mt * nt;
+      dh_tiles = p.gh != nullptr ? per_split * p.splits : 0;
+      total = dh_tiles + wt * ht;
+      k_steps = (p.words + kInner - 1) / kInner;
+      row_steps = (n_rows + kInner - 1) / kInner;
+    } else {
+      nt = (p.words + kTile - 1) / kTile;
+      total = mt * nt;
+      k_steps = (p.hidden + kInner - 1) / kInner;
+    }
+  }
+  __device__ __forceinline__ static void place(int t, int mt, int nt, int& m, int& n) {
+    const int g = t / (kGroup * nt), first = g * kGroup, r = t - g * kGroup * nt;
+    const int gm = mt - first < kGroup ? mt - first : kGroup;
+    m = first + r % gm;
+    n = r / gm;
+  }
+  template <int PASS>
+  __device__ __forceinline__ Tile at(const GemmParams& p, int t) const {
+    Tile x;
+    x.kind = 0;
+    x.split = 0;
+    x.k0 = 0;
+    int m, n;
+    if (PASS == kGrads) {
+      if (t < dh_tiles) {
+        x.split = t / per_split;
+        place(t - x.split * per_split, mt, nt, m, n);
+        const int lo = (int)((int64_t)k_steps * x.split / p.splits), hi = (int)((int64_t)k_steps * (x.split + 1) / p.splits);
+        x.k0 = lo * kInner;
+        x.steps = hi - lo;
+      } else {
+        x.kind = 1;
+        place(t - dh_tiles, wt, ht, m, n);
+        x.steps = row_steps;
+      }
+    } else {
+      place(t, mt, nt, m, n);
+      x.steps = k_steps;
+    }
+    x.m = m * kTile;
+    x.n = n * kTile;
+    return x;
+  }
+};
+
+// ------------------------------------------------------------------- epilogues
+// Every epilogue warp handles 32 rows (lanes) and 128 columns of the CTA's 128 x 256 tile.
+
+__device__ __forceinline__ void stats_tile(const GemmParams& p, const Tile& x, uint32_t tmem, int row, int n_rows, int half) {
+  const int lab = row < n_rows ? p.label[row] : -1;
+  float m = -INFINITY, s = 0.f;
+#pragma unroll 1
+  for (int c = 0; c < 4; ++c) {
+    float v[32];
+    tmem_load32(tmem + c * 32, v);
+    const int col = x.n + half * 128 + c * 32, left = p.words - col;
+    if (left < 32) {
+#pragma unroll
+      for (int i = 0; i < 32; ++i)
+        if (i >= left) v[i] = -INFINITY;
+    }
+    const int hit = lab - col;
+    if (hit >= 0 && hit < 32) {
+      float z = v[0];
+#pragma unroll
+      for (int i = 1; i < 32; ++i)
+        if (i == hit) z = v[i];
+      p.picked[row] = z;
+    }
+    float mn = m;
+#pragma unroll
+    for (int i = 0; i < 32; ++i) mn = fmaxf(mn, v[i]);
+    const float sh = finite_shift(mn);
+    float t0 = 0.f, t1 = 0.f;
+#pragma unroll
+    for (int i = 0; i < 32; i += 2) {
+      t0 = __fadd_rn(t0, exp_of(__fsub_rn(v[i], sh)));
+      t1 = __fadd_rn(t1, exp_of(__fsub_rn(v[i + 1], sh)));
+    }
+    s = __fadd_rn(__fmul_rn(s, exp_of(__fsub_rn(m, sh))), __fadd_rn(t0, t1));
+    m = mn;
+  }
+  if (row < n_rows) p.part[(int64_t)(x.n / 128 + half) * p.rows + row] = make_float2(m, s);
+}
+
+__device__ __forceinline__ void logit_grad_tile(const GemmParams& p, const Tile& x, uint32_t tmem, int row, int n_rows, int half) {
+  const bool in = row < n_rows;
+  const int lab = in && p.label[row] >= 0 ? (int)(p.label[row] - p.word0) : -1;
+  const float lse = in ? p.lse[row] : 0.f;
+  const float g = !in ? 0.f : p.row_g != nullptr ? p.row_g[p.index[row]] : 1.f;
+  // rows that pad the inner dimension of dW are zero
+  const bool store = row < (n_rows + kLceRowPad - 1) / kLceRowPad * kLceRowPad;
+#pragma unroll 1
+  for (int c = 0; c < 4; ++c) {
+    float v[32];
+    tmem_load32(tmem + c * 32, v);
+    const int col = x.n + half * 128 + c * 32;
+#pragma unroll
+    for (int i = 0; i < 32; ++i) v[i] = exp_of(__fsub_rn(v[i], lse));
+    const int hit = lab - col;
+    if (lab >= 0 && hit >= 0 && hit < 32) {
+#pragma unroll
+      for (int i = 0; i < 32; ++i)
+        if (i == hit) v[i] = __fsub_rn(v[i], 1.f);
+    }
+    V8 o[2];
+#pragma unroll
+    for (int i = 0; i < 16; ++i)
+      o[i >> 3].w[i & 7] = in ? f32x2_to_bf16x2_rne(__fmul_rn(v[2 * i], g), __fmul_rn(v[2 * i + 1], g)) : 0u;
+    if (store) {
+      uint16_t* at = p.d + (int64_t)row * p.pitch + col;
+      if (col < p.pitch) st32(at, o[0]);
+      if (col + 16 < p.pitch) st32(at + 16, o[1]);
+    }
+  }
+}
+
+__device__ __forceinline__ void store_bf16x8(uint16_t* at, const float* v, float scale) {
+  uint4 o;
+  o.x = f32x2_to_bf16x2_rne(__fmul_rn(v[0], scale), __fmul_rn(v[1], scale));
+  o.y = f32x2_to_bf16x2_rne(__fmul_rn(v[2], scale), __fmul_rn(v[3], scale));
+  o.z = f32x2_to_bf16x2_rne(__fmul_rn(v[4], scale), __fmul_rn(v[5], scale));
+  o.w = f32x2_to_bf16x2_rne(__fmul_rn(v[6], scale), __fmul_rn(v[7], scale));
+  *reinterpret_cast<uint4*>(at) = o;
+}
+
+__device__ __forceinline__ void grads_tile(const GemmParams& p, const Tile& x, uint32_t tmem, int row, int n_rows, int half, float scale) {
+  // x.steps == 0 happens only for dW without a row that counts
+  const bool direct = x.kind == 1 || (p.last && p.splits == 1);  // the rounded result goes out
+  const bool add = x.kind == 0 && !p.first;
+  const bool in = x.kind == 1 ? row < p.words : row < n_rows;
+  float* acc = nullptr;
+  uint16_t* out = nullptr;
+  if (in) {
+    if (x.kind == 1) out = p.gw + (p.word0 + row) * p.hidden;
+    else if (direct) out = p.gh + (int64_t)p.index[row] * p.hidden;
+    if (x.kind == 0 && p.acc != nullptr) acc = p.acc + ((int64_t)x.split * p.padded + row) * p.hidden;
+  }
+#pragma unroll 1
+  for (int c = 0; c < 4; ++c) {
+    float v[32];
+    tmem_load32(tmem + c * 32, v);
+    if (x.steps == 0) {
+#pragma unroll
+      for (int i = 0; i < 32; ++i) v[i] = 0.f;
+    }
+    const int col = x.n + half * 128 + c * 32;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const int at = col + q * 8;
+      if (!in || at >= p.hidden) continue;
+      float* w = v + q * 8;
+      if (add) {
+        const V8 old = ld32(acc + at);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) w[i] = __fadd_rn(__uint_as_float(old.w[i]), w[i]);
+      }
+      if (direct) {
+        store_bf16x8(out + at, w, scale);
+      } else {
+        V8 o;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) o.w[i] = __float_as_uint(w[i]);
+        st32(acc + at, o);
+      }
+    }
+  }
+}
+
+// --------------------------------------------------------------------- product
+template <int PASS>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmThreads, 1)
+lce_product_kernel(const __grid_constant__ GemmParams p) {
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ uint64_t full[kStages], empty[kStages], done[2], drained[2];
+  __shared__ uint32_t tmem_at;
+  __shared__ int gave_up;
+  const uint32_t stages = (smem_addr(smem_raw) + 1023u) & ~1023u;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = cluster_rank();
+  const uint32_t full0 = smem_addr(full), empty0 = smem_addr(empty), done0 = smem_addr(done), drained0 = smem_addr(drained);
+
+  if (threadIdx.x == 0) {
+    gave_up = 0;
+    for (int i = 0; i < kStages; ++i) {
+      mbar_init(full0 + 8 * i, 1);
+      mbar_init(empty0 + 8 * i, 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(done0 + 8 * i, 1);
+      mbar_init(drained0 + 8 * i, 2 * kEpilogueWarps);
+    }
+    mbar_init_fence();
+    prefetch_map(&p.a);
+    prefetch_map(&p.b);
+  }
+  if (warp == 1) tmem_alloc_pair(smem_addr(&tmem_at), 512);
+  fence_before();
+  __syncthreads();
+  cluster_sync();
+  fence_after();
+  const uint32_t tmem = tmem_at;
+
+  const int n_rows = *p.count;
+  Plan plan{};
+  plan.make<PASS>(p, n_rows);
+  const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
+  bool ok = true;
+
+  if (warp == 0) {
+    if (elect_one()) {
+      const uint32_t lead_full0 = map_to_rank(full0, 0);
+      int it = 0;
+      for (int t = pair; t < plan.total && ok; t += pairs) {
+        const Tile x = plan.at<PASS>(p, t);
+        const bool outer_a = PASS == kGrads && x.kind == 1, outer_b = PASS == kGrads;
+        const CUtensorMap* ma = outer_a ? &p.a2 : &p.a;
+        const CUtensorMap* mb = outer_a ? &p.b2 : &p.b;
+        const int am = x.m + rank * 128, bn = x.n + rank * 128;
+        // kLogitGrad: W's rows start at the piece; dh: so do the inner values of W
+        const int b_row0 = PASS == kLogitGrad ? (int)p.word0 : 0, b_k0 = PASS == kGrads && x.kind == 0 ? (int)p.word0 : 0;
+        for (int k = 0; k < x.steps; ++k, ++it) {
+          const int s = it % kStages;
+          if (!mbar_wait(empty0 + 8 * s, ((it / kStages) & 1) ^ 1)) { ok = false; break; }
+          if (rank == 0) mbar_expect_tx(full0 + 8 * s, 2 * kStageBytes);
+          const uint32_t at = stages + s * kStageBytes, bt = at + kHalfBytes, bar = lead_full0 + 8 * s;
+          const int kk = x.k0 + k * kInner;
+          if (outer_a) {
+            tma_load_pair(at, ma, am, kk, bar);
+            tma_load_pair(at + kHalfBytes / 2, ma, am + 64, kk, bar);
+          } else {
+            tma_load_pair(at, ma, kk, am, bar);
+          }
+          if (outer_b) {
+            tma_load_pair(bt, mb, bn, b_k0 + kk, bar);
+            tma_load_pair(bt + kHalfBytes / 2, mb, bn + 64, b_k0 + kk, bar);
+          } else {
+            tma_load_pair(bt, mb, kk, b_row0 + bn, bar);
+          }
+        }
+      }
+      // every stage is released before this CTA may go: the last arrivals come from the partner
+      for (int i = 0; i < kStages && ok; ++i, ++it) ok = mbar_wait(empty0 + 8 * (it % kStages), ((it / kStages) & 1) ^ 1);
+      if (!ok) {  // copies that are still under way end within microseconds
+        for (int i = 0; i < 100; ++i) __nanosleep(10000);
+      }
+    }
+    __syncwarp();
+  } else if (warp == 1) {
+    if (rank == 0 && elect_one()) {
+      int it = 0, mine = 0;
+      for (int t = pair; t < plan.total && ok; t += pairs, ++mine) {
+        const Tile x = plan.at<PASS>(p, t);
+        const bool outer_a = PASS == kGrads && x.kind == 1;
+        constexpr bool outer_b = PASS == kGrads;
+        const uint32_t idesc = instruction(kTile, kTile, outer_a, outer_b);
+        const uint32_t acc = mine & 1, d = tmem + acc * kTile;
+        if (!mbar_wait(drained0 + 8 * acc, ((mine >> 1) & 1) ^ 1)) { ok = false; break; }
+        fence_after();
+        for (int k = 0; k < x.steps; ++k, ++it) {
+          const int s = it % kStages;
+          if (!mbar_wait(full0 + 8 * s, (it / kStages) & 1)) { ok = false; break; }
+          fence_after();
+          const uint32_t at = stages + s * kStageBytes, bt = at + kHalfBytes;
+          const uint64_t da = outer_a ? operand(at, kHalfBytes / 2, 1024) : operand(at, 16, 1024);
+          const uint64_t db = outer_b ? operand(bt, kHalfBytes / 2, 1024) : operand(bt, 16, 1024);
+          // 16 inner values further: 32 bytes along a row, or 16 lines of 128 bytes
+          const uint64_t step_a = outer_a ? 2048 >> 4 : 32 >> 4, step_b = outer_b ? 2048 >> 4 : 32 >> 4;
+#pragma unroll
+          for (int q = 0; q < kInner / 16; ++q) mma_pair(d, da + q * step_a, db + q * step_b, idesc, k > 0 || q > 0);
+          commit_pair(empty0 + 8 * s);
+        }
+        commit_pair(done0 + 8 * acc);
+      }
+    }
+    __syncwarp();
+  } else {
+    const int quarter = warp & 3, half = (warp - 2) >> 2;
+    const uint32_t lead_drained0 = map_to_rank(drained0, 0);
+    float scale = 1.f;
+    if (PASS == kGrads) {
+      if (p.inv != nullptr) scale = *p.inv;
+      if (p.g != nullptr) scale = __fmul_rn(scale, *p.g);
+    }
+    int mine = 0;
+    for (int t = pair; t < plan.total; t += pairs, ++mine) {
+      const Tile x = plan.at<PASS>(p, t);
+      const uint32_t acc = mine & 1;
+      ok = mbar_wait(done0 + 8 * acc, (mine >> 1) & 1);
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) break;
+      fence_after();
+      const uint32_t at = tmem + acc * kTile + half * 128 + ((uint32_t)(quarter * 32) << 16);
+      const int row = x.m + (int)rank * 128 + quarter * 32 + lane;
+      if (PASS == kStats) stats_tile(p, x, at, row, n_rows, half);
+      if (PASS == kLogitGrad) logit_grad_tile(p, x, at, row, n_rows, half);
+      if (PASS == kGrads) grads_tile(p, x, at, row, n_rows, half, scale);
+      fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive_cluster(lead_drained0 + 8 * acc);
+    }
+  }
+  if (!ok) gave_up = 1;
+  fence_before();
+  __syncthreads();
+  if (gave_up && threadIdx.x == 0) *reinterpret_cast<volatile int64_t*>(p.report + 1) = 1;
+  cluster_sync();
+  fence_after();
+  if (warp == 1) tmem_free_pair(tmem, 512);
+}
+
+// ------------------------------------------------------------- packing of rows
+constexpr int kScanThreads = 1024;
+
+// index[k] = row of the k-th label that counts, label[k] = that label (-1: outside the vocabulary),
+// count[0] = how many, count[1] = 0, inv; row_loss of ignored rows = 0.
+__global__ void __launch_bounds__(kScanThreads)
+lce_scan_kernel(const int64_t* __restrict__ labels, int64_t rows, int64_t vocab, int64_t ignore, int* index, int* label,
+                int* count, float* inv, float* row_loss, volatile int64_t* bad) {
+  __shared__ int warps[kScanThreads / 32 + 1];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int base = 0;
+  for (int64_t r0 = 0; r0 < rows; r0 += kScanThreads) {
+    const int64_t r = r0 + threadIdx.x;
+    const int64_t lab = r < rows ? labels[r] : ignore;
+    const bool in = lab != ignore;
+    const unsigned mask = __ballot_sync(0xffffffffu, in);
+    if (lane == 0) warps[warp] = __popc(mask);
+    __syncthreads();
+    if (warp == 0) {
+      const int c = warps[lane];
+      int x = c;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int y = __shfl_up_sync(0xffffffffu, x, o);
+        if (lane >= o) x += y;
+      }
+      warps[lane] = x - c;
+      if (lane == 31) warps[32] = x;
+    }
+    __syncthreads();
+    if (in) {
+      const int k = base + warps[warp] + __popc(mask & ((1u << lane) - 1u));
+      const bool known = lab >= 0 && lab < vocab;
+      if (!known) *bad = lab;
+      index[k] = (int)r;
+      label[k] = known ? (int)lab : -1;
+    } else if (row_loss != nullptr && r < rows) {
+      row_loss[r] = 0.f;
+    }
+    base += warps[32];
+    __syncthreads();
+  }
+  if (threadIdx.x == 0) {
+    count[0] = base;
+    count[1] = 0;
+    *inv = __fdiv_rn(1.f, (float)(base < 1 ? 1 : base));
+  }
+}
+
+// packed[k] = h[index[k]], zero rows up to the next multiple of kLceRowPad; rows of `gh` whose
+// label is ignored become zero.
+__global__ void __launch_bounds__(128)
+lce_pack_kernel(const uint16_t* __restrict__ h, int64_t stride, const int64_t* __restrict__ labels, int64_t ignore,
+                const int* __restrict__ index, const int* __restrict__ count, int64_t rows, int hidden, uint16_t* packed,
+                uint16_t* gh) {
+  const int64_t k = blockIdx.x;
+  const int n = *count, vecs = hidden >> 3;
+  const uint4 zero = make_uint4(0, 0, 0, 0);
+  uint4* to = reinterpret_cast<uint4*>(packed + k * hidden);
+  if (k < n) {
+    const uint4* from = reinterpret_cast<const uint4*>(h + index[k] * stride);
+    for (int v = threadIdx.x; v < vecs; v += 128) to[v] = from[v];
+  } else if (k < (n + kLceRowPad - 1) / kLceRowPad * kLceRowPad) {
+    for (int v = threadIdx.x; v < vecs; v += 128) to[v] = zero;
+  }
+  if (gh != nullptr && k < rows && labels[k] == ignore) {
+    uint4* g = reinterpret_cast<uint4*>(gh + k * hidden);
+    for (int v = threadIdx.x; v < vecs; v += 128) g[v] = zero;
+  }
+}
+
+// ------------------------------------------------------------ joining the sums
+// 32 rows and 32 slices of the words a block.
+constexpr int kJoinThreads = 1024;
+__device__ __forceinline__ void join(float& m, float& s, float m2, float s2) {
+  const float mn = fmaxf(m, m2), sh = finite_shift(mn);
+  s = __fadd_rn(__fmul_rn(s, expf(__fsub_rn(m, sh))), __fmul_rn(s2, expf(__fsub_rn(m2, sh))));
+  m = mn;
+}
+__global__ void __launch_bounds__(kJoinThreads)
+lce_join_kernel(const float2* __restrict__ part, int parts, int64_t rows, const int* __restrict__ index,
+                const int* __restrict__ label, int* count, const float* __restrict__ picked, const float* __restrict__ inv,
+                float* lse, int reduction, double* sums, float* loss) {
+  __shared__ float sm[32][33], ss[32][33];
+  __shared__ int is_last;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int n = *count;
+  const int64_t row = (int64_t)blockIdx.x * 32 + lane;
+  float m = -INFINITY, s = 0.f;
+  if (row < n) {
+#pragma unroll 4
+    for (int i = warp; i < parts; i += 32) {
+      const float2 x = part[(int64_t)i * rows + row];
+      join(m, s, x.x, x.y);
+    }
+  }
+  sm[warp][lane] = m;
+  ss[warp][lane] = s;
+  __syncthreads();
+  // warp w finishes the block's row w: lane i has slice i
+  m = sm[lane][warp];
+  s = ss[lane][warp];
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    const float m2 = __shfl_xor_sync(0xffffffffu, m, o), s2 = __shfl_xor_sync(0xffffffffu, s, o);
+    join(m, s, m2, s2);
+  }
+  const int64_t at = (int64_t)blockIdx.x * 32 + warp;
+  float one = 0.f;
+  if (at < n) {
+    const bool known = label[at] >= 0;
+    const float l = !known ? NAN : isinf(m) ? m : __fadd_rn(m, logf(s));
+    one = known ? __fsub_rn(l, picked[at]) : NAN;
+    if (lane == 0) {
+      lse[at] = l;
+      if (reduction == kLceNone) loss[index[at]] = one;
+    }
+  }
+  if (reduction == kLceNone) return;
+  __syncthreads();
+  if (lane == 0) sm[0][warp] = one;
+  __syncthreads();
+  if (warp == 0) {  // the same order whatever the blocks' order
+    double t = sm[0][lane];
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
+    if (lane == 0) {
+      sums[blockIdx.x] = t;
+      __threadfence();
+      is_last = atomicAdd(count + 1, 1) == (int)gridDim.x - 1;
+    }
+  }
+  __syncthreads();
+  if (is_last && warp == 0) {
+    __threadfence();
+    double t = 0.0;
+    for (int i = lane; i < (int)gridDim.x; i += 32) t += __ldcg(sums + i);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
+    if (lane == 0) *loss = (float)(reduction == kLceMean ? t * (double)*inv : t);
+  }
+}
+
+// ------------------------------------------------------- splits of dh, joined
+__global__ void __launch_bounds__(128)
+lce_join_grad_kernel(const float* __restrict__ acc, int splits, int64_t padded, const int* __restrict__ index,
+                     const int* __restrict__ count, int hidden, const float* inv, const float* g, uint16_t* gh) {
+  const int64_t k = blockIdx.x;
+  if (k >= *count) return;
+  float scale = inv != nullptr ? *inv : 1.f;
+  if (g != nullptr) scale = __fmul_rn(scale, *g);
+  const int col = (blockIdx.y * 128 + threadIdx.x) * 8;
+  if (col >= hidden) return;
+  float v[8] = {};
+  for (int s = 0; s < splits; ++s) {
+    const V8 x = ld32(acc + ((int64_t)s * padded + k) * hidden + col);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = __fadd_rn(v[i], __uint_as_float(x.w[i]));
+  }
+  store_bf16x8(gh + (int64_t)index[k] * hidden + col, v, scale);
+}
+
+// ------------------------------------------------------------------- launching
+PFN_cuTensorMapEncodeTiled_v12000 encoder() {
+  static const PFN_cuTensorMapEncodeTiled_v12000 fn = [] {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult found;
+    if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &p, 12000, cudaEnableDefault, &found) != cudaSuccess ||
+        found != cudaDriverEntryPointSuccess)
+      p = nullptr;
+    return reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(p);
+  }();
+  return fn;
+}
+
+// Boxes of 64 contiguous values and `lines` lines of a bf16 matrix; what lies outside reads as zero.
+bool encode(CUtensorMap* map, const void* base, int64_t inner, int64_t lines_all, int64_t stride, int lines) {
+  const auto fn = encoder();
+  if (fn == nullptr) return false;
+  const cuuint64_t dims[2] = {(cuuint64_t)inner, (cuuint64_t)lines_all}, strides[1] = {(cuuint64_t)stride * 2};
+  const cuuint32_t box[2] = {64, (cuuint32_t)lines}, steps[2] = {1, 1};
+  return fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(base), dims, strides, box, steps,
+            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <int PASS>
+cudaError_t launch_product(const GemmParams& p, int64_t tiles, cudaStream_t st) {
+  if (tiles <= 0) return cudaSuccess;
+  if (tiles > (int64_t(1) << 30)) return cudaErrorInvalidValue;
+  const cudaError_t e = cudaFuncSetAttribute(lce_product_kernel<PASS>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes);
+  if (e != cudaSuccess) return e;
+  const int pairs = (int)(tiles < kNumSMs / 2 ? tiles : kNumSMs / 2);
+  count_launch();
+  lce_product_kernel<PASS><<<2 * pairs, kGemmThreads, kSmemBytes, st>>>(p);
+  return cudaGetLastError();
+}
+
+bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+int64_t tiles_of(int64_t n) { return (n + kTile - 1) / kTile; }
+
+bool args_ok(const LceArgs& a) {
+  constexpr int64_t most = int64_t(1) << 31;
+  return a.rows > 0 && a.rows < most - kTile && a.hidden > 0 && a.hidden < most - kTile && a.hidden % 8 == 0 && a.vocab > 0 &&
+         a.vocab < most - kTile && a.h_stride % 8 == 0 && a.w_stride % 8 == 0 && aligned16(a.h) && aligned16(a.w) &&
+         aligned16(a.packed) && a.report != nullptr && a.h_stride < (int64_t(1) << 36) && a.w_stride < (int64_t(1) << 36);
+}
+
+void common_params(GemmParams& p, const LceArgs& a) {
+  p.count = a.count;
+  p.rows = a.rows;
+  p.padded = lce_padded(a.rows);
+  p.hidden = (int)a.hidden;
+  p.vocab = a.vocab;
+  p.report = a.report;
+  p.label = a.label;
+  p.index = a.index;
+}
+
+cudaError_t pack_rows(const LceArgs& a, void* gh, cudaStream_t st) {
+  count_launch();
+  lce_pack_kernel<<<(unsigned)lce_padded(a.rows), 128, 0, st>>>((const uint16_t*)a.h, a.h_stride, a.labels, a.ignore, a.index,
+                                                               a.count, a.rows, (int)a.hidden, (uint16_t*)a.packed, (uint16_t*)gh);
+  return cudaGetLastError();
+}
+
+}  // namespace
+
+int64_t lce_part_floats(int64_t rows, int64_t vocab) { return 4 * tiles_of(vocab) * rows; }
+int64_t lce_sum_doubles(int64_t rows) { return (rows + 31) / 32; }
+
+cudaError_t launch_lce_forward(const LceArgs& a, int reduction, float* part, float* picked, double* sums, float* loss,
+                               cudaStream_t st) {
+  if (!args_ok(a)) return cudaErrorInvalidValue;
+  count_launch();
+  lce_scan_kernel<<<1, kScanThreads, 0, st>>>(a.labels, a.rows, a.vocab, a.ignore, a.index, a.label, a.count, a.inv,
+                                              reduction == kLceNone ? loss : nullptr, a.report);
+  cudaError_t e = cudaGetLastError();
+  if (e != cudaSuccess || (e = pack_rows(a, nullptr, st)) != cudaSuccess) return e;
+  GemmParams p{};
+  common_params(p, a);
+  if (!encode(&p.a, a.packed, a.hidden, p.padded, a.hidden, 128) || !encode(&p.b, a.w, a.hidden, a.vocab, a.w_stride, 128))
+    return cudaErrorInvalidValue;
+  p.words = (int)a.vocab;
+  p.part = reinterpret_cast<float2*>(part);
+  p.picked = picked;
+  if ((e = launch_product<kStats>(p, tiles_of(a.rows) * tiles_of(a.vocab), st)) != cudaSuccess) return e;
+  count_launch();
+  lce_join_kernel<<<(unsigned)lce_sum_doubles(a.rows), kJoinThreads, 0, st>>>(
+      p.part, (int)(2 * tiles_of(a.vocab)), a.rows, a.index, a.label, a.count, picked, a.inv, a.lse, reduction, sums, loss);
+  return cudaGetLastError();
+}
+
+int64_t lce_default_piece(int64_t rows, int64_t hidden, int64_t vocab) {
+  const int64_t words = (int64_t(256) << 20) / (2 * lce_padded(rows)) / kTile * kTile;
+  const int64_t all = tiles_of(vocab) * kTile;
+  return words < kTile ? kTile : words < all ? words : all;
+}
+
+int lce_splits(int64_t rows, int64_t hidden, int64_t vocab, int64_t piece) {
+  const int64_t tiles = tiles_of(rows) * tiles_of(hidden), steps = (piece < vocab ? piece : vocab) / kInner;
+  int64_t s = kNumSMs / 2 / tiles;
+  if (s > steps / 8) s = steps / 8;
+  return s < 1 ? 1 : (int)s;
+}
+
+cudaError_t launch_lce_backward(const LceArgs& a, const LceGrad& g, cudaStream_t st) {
+  if (!args_ok(a) || g.piece <= 0 || g.piece % kTile != 0 || g.splits < 1 || g.g == nullptr) return cudaErrorInvalidValue;
+  if (g.gh == nullptr && g.gw == nullptr) return cudaSuccess;
+  cudaError_t e = pack_rows(a, g.gh, st);
+  if (e != cudaSuccess) return e;
+  const int64_t pieces = lce_pieces(a.vocab, g.piece), pitch = lce_piece_pitch(a.vocab, g.piece);
+  if (g.gh != nullptr && (pieces > 1 || g.splits > 1) && g.acc == nullptr) return cudaErrorInvalidValue;
+  GemmParams p{};
+  common_params(p, a);
+  p.lse = a.lse;
+  p.row_g = g.reduction == kLceNone ? g.g : nullptr;
+  p.d = (uint16_t*)g.d;
+  p.pitch = pitch;
+  GemmParams q{};
+  common_params(q, a);
+  q.inv = g.reduction == kLceMean ? a.inv : nullptr;
+  q.g = g.reduction == kLceNone ? nullptr : g.g;
+  q.acc = g.acc;
+  q.gh = (uint16_t*)g.gh;
+  q.gw = (uint16_t*)g.gw;
+  q.splits = g.splits;
+  if (!encode(&p.a, a.packed, a.hidden, p.padded, a.hidden, 128) || !encode(&p.b, a.w, a.hidden, a.vocab, a.w_stride, 128) ||
+      !encode(&q.b, a.w, a.hidden, a.vocab, a.w_stride, 64) || !encode(&q.b2, a.packed, a.hidden, p.padded, a.hidden, 64))
+    return cudaErrorInvalidValue;
+  for (int64_t i = 0; i < pieces; ++i) {
+    p.word0 = q.word0 = i * g.piece;
+    p.words = q.words = (int)(a.vocab - p.word0 < g.piece ? a.vocab - p.word0 : g.piece);
+    q.first = i == 0;
+    q.last = i == pieces - 1;
+    if ((e = launch_product<kLogitGrad>(p, tiles_of(a.rows) * tiles_of(p.words), st)) != cudaSuccess) return e;
+    if (!encode(&q.a, g.d, q.words, p.padded, pitch, 128) || !encode(&q.a2, g.d, q.words, p.padded, pitch, 64))
+      return cudaErrorInvalidValue;
+    const int64_t dh = g.gh != nullptr ? tiles_of(a.rows) * tiles_of(a.hidden) * g.splits : 0;
+    const int64_t dw = g.gw != nullptr ? tiles_of(q.words) * tiles_of(a.hidden) : 0;
+    if ((e = launch_product<kGrads>(q, dh + dw, st)) != cudaSuccess) return e;
+  }
+  if (g.gh != nullptr && g.splits > 1) {
+    count_launch();
+    lce_join_grad_kernel<<<dim3((unsigned)a.rows, (unsigned)((a.hidden + 1023) / 1024)), 128, 0, st>>>(
+        g.acc, g.splits, p.padded, a.index, a.count, (int)a.hidden, q.inv, q.g, (uint16_t*)g.gh);
+    e = cudaGetLastError();
+  }
+  return e;
+}
+
+}  // namespace oab

@@ -1,0 +1,128 @@
+// Autograd function of the cross entropy that keeps no logits, and its Python binding.
+#include <ATen/cuda/CUDAContext.h>
+#include <c10/cuda/CUDAGuard.h>
+#include <torch/extension.h>
+
+#include "linear_ce.h"
+#include "loss_ops.h"
+
+namespace py = pybind11;
+using at::Tensor;
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
+namespace {
+
+cudaStream_t cur() { return at::cuda::getCurrentCUDAStream().stream(); }
+void ok(cudaError_t e, const char* what) { TORCH_CHECK(e == cudaSuccess, what, ": ", cudaGetErrorString(e)); }
+
+// Rows that the kernels can read in place: 16-byte aligned, none overlapping.
+Tensor rows_layout(const Tensor& t) {
+  const bool fits = t.stride(1) == 1 && (t.size(0) == 1 || (t.stride(0) % 8 == 0 && t.stride(0) >= t.size(1))) &&
+                    (reinterpret_cast<uintptr_t>(t.data_ptr()) & 15u) == 0;
+  return fits ? t : t.clone(at::MemoryFormat::Contiguous);
+}
+int64_t row_stride(const Tensor& t) { return t.size(0) == 1 ? t.size(1) : t.stride(0); }
+
+// What backward needs of forward, in one int32 tensor: index, label and lse of the packed rows,
+// their number with the ticket, 1 / number.
+int64_t kept_words(int64_t rows) { return 3 * rows + 4; }
+oab::LceArgs make_args(const Tensor& h, const Tensor& w, const Tensor& labels, const Tensor& kept, int64_t ignore, const Tensor& packed) {
+  oab::LceArgs a;
+  a.h = h.data_ptr();
+  a.h_stride = row_stride(h);
+  a.w = w.data_ptr();
+  a.w_stride = row_stride(w);
+  a.labels = labels.data_ptr<int64_t>();
+  a.rows = h.size(0);
+  a.hidden = h.size(1);
+  a.vocab = w.size(0);
+  a.ignore = ignore;
+  int* k = kept.data_ptr<int>();
+  a.index = k;
+  a.label = k + a.rows;
+  a.lse = reinterpret_cast<float*>(k + 2 * a.rows);
+  a.count = k + 3 * a.rows;
+  a.inv = reinterpret_cast<float*>(k + 3 * a.rows + 2);
+  a.packed = packed.data_ptr();
+  a.report = oab::loss_report();
+  return a;
+}
+
+struct LinearCE : torch::autograd::Function<LinearCE> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& h, const Tensor& w, const Tensor& labels, int64_t reduction,
+                        int64_t ignore, int64_t piece) {
+    TORCH_CHECK(h.is_cuda() && h.scalar_type() == at::kBFloat16 && h.dim() == 2 && w.scalar_type() == at::kBFloat16 && w.dim() == 2 &&
+                    w.size(1) == h.size(1) && h.size(1) % 8 == 0 && h.numel() > 0 && w.numel() > 0 && w.device() == h.device(),
+                "linear_cross_entropy: bf16 CUDA matrices of one device, rows of a multiple of 8");
+    TORCH_CHECK(labels.scalar_type() == at::kLong && labels.dim() == 1 && labels.size(0) == h.size(0) && labels.device() == h.device() &&
+                    labels.is_contiguous(), "linear_cross_entropy: one contiguous int64 label per row");
+    TORCH_CHECK(reduction >= 0 && reduction <= 2 && piece >= 0, "linear_cross_entropy: reduction or piece");
+    c10::cuda::CUDAGuard guard(h.device());
+    oab::raise_loss_report();
+    const Tensor hc = rows_layout(h), wc = rows_layout(w);
+    const int64_t rows = h.size(0);
+    const auto f32 = h.options().dtype(at::kFloat);
+    Tensor kept = at::empty({kept_words(rows)}, h.options().dtype(at::kInt));
+    Tensor loss = reduction == oab::kLceNone ? at::empty({rows}, f32) : at::empty({}, f32);
+    const Tensor packed = at::empty({oab::lce_padded(rows), h.size(1)}, h.options());
+    const Tensor part = at::empty({oab::lce_part_floats(rows, w.size(0)) + rows}, f32);
+    const Tensor sums = at::empty({oab::lce_sum_doubles(rows)}, h.options().dtype(at::kDouble));
+    ok(oab::launch_lce_forward(make_args(hc, wc, labels, kept, ignore, packed), (int)reduction, part.data_ptr<float>(),
+                               part.data_ptr<float>() + part.numel() - rows, sums.data_ptr<double>(), loss.data_ptr<float>(), cur()),
+       "linear_cross_entropy");
+    ctx->save_for_backward({h, w, labels, kept});
+    ctx->saved_data["reduction"] = reduction;
+    ctx->saved_data["ignore"] = ignore;
+    ctx->saved_data["piece"] = piece;
+    return loss;
+  }
+
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const Tensor& g = grads[0];
+    const bool want_h = ctx->needs_input_grad(0), want_w = ctx->needs_input_grad(1);
+    if (!g.defined() || !(want_h || want_w)) return {Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
+    TORCH_CHECK(!at::GradMode::is_enabled(), "linear_cross_entropy has no second derivative (create_graph)");
+    const auto saved = ctx->get_saved_variables();
+    const Tensor &h = saved[0], &w = saved[1], &labels = saved[2], kept = saved[3].contiguous();
+    const int64_t reduction = ctx->saved_data["reduction"].toInt(), ignore = ctx->saved_data["ignore"].toInt();
+    c10::cuda::CUDAGuard guard(h.device());
+    oab::raise_loss_report();
+    const Tensor hc = rows_layout(h), wc = rows_layout(w), lc = labels.contiguous(), gc = g.to(at::kFloat).contiguous();
+    const int64_t rows = h.size(0), hidden = h.size(1), vocab = w.size(0);
+    int64_t piece = ctx->saved_data["piece"].toInt();
+    piece = piece > 0 ? (piece + oab::kLceTile - 1) / oab::kLceTile * oab::kLceTile : oab::lce_default_piece(rows, hidden, vocab);
+    oab::LceGrad x;
+    x.reduction = (int)reduction;
+    x.g = gc.data_ptr<float>();
+    x.piece = piece;
+    x.splits = want_h ? oab::lce_splits(rows, hidden, vocab, piece) : 1;
+    Tensor gh, gw, acc;
+    if (want_h) {
+      gh = at::empty({rows, hidden}, h.options());
+      x.gh = gh.data_ptr();
+      if (x.splits > 1 || oab::lce_pieces(vocab, piece) > 1) {
+        acc = at::empty({x.splits, oab::lce_padded(rows), hidden}, h.options().dtype(at::kFloat));
+        x.acc = acc.data_ptr<float>();
+      }
+    }
+    if (want_w) {
+      gw = at::empty({vocab, hidden}, w.options());
+      x.gw = gw.data_ptr();
+    }
+    const Tensor packed = at::empty({oab::lce_padded(rows), hidden}, h.options());
+    const Tensor d = at::empty({oab::lce_padded(rows), oab::lce_piece_pitch(vocab, piece)}, h.options());
+    x.d = d.data_ptr();
+    ok(oab::launch_lce_backward(make_args(hc, wc, lc, kept, ignore, packed), x, cur()), "linear_cross_entropy backward");
+    return {gh, gw, Tensor(), Tensor(), Tensor(), Tensor()};
+  }
+};
+
+}  // namespace
+
+void bind_linear_ce(py::module_& m) {
+  m.def("linear_ce", [](const Tensor& h, const Tensor& w, const Tensor& labels, int64_t reduction, int64_t ignore, int64_t piece) {
+    return LinearCE::apply(h, w, labels, reduction, ignore, piece);
+  });
+  m.def("linear_ce_piece", &oab::lce_default_piece, py::arg("rows"), py::arg("hidden"), py::arg("vocab"));
+}
