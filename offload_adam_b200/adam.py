@@ -17,6 +17,7 @@ from torch.optim.optimizer import Optimizer
 
 from ._master import MasterLoadingMixin, is_quant
 from .ops.adam_step import MANY_TENSORS, STEP_FNS, adam_step_many
+from .ops.clip_grad import check_max_norm, clip_coefficient
 
 STATE_DTYPES = {
     "stochastic_rounding": {"exp_avg": torch.bfloat16, "exp_avg_sq": torch.bfloat16},
@@ -48,12 +49,16 @@ class Adam(MasterLoadingMixin, Optimizer):
             ``'fp31_master'`` or ``'fp32_master_custom_rounding'``.
         decoupled_weight_decay: AdamW-style decay when True.
         seed: seeds the stochastic-rounding stream (default: Python's ``random``).
+        max_grad_norm: L2 global-norm clipping threshold over all parameters, or None.  The
+            gradients stay as they are: the coefficient is applied in fp32 inside the step.
+            ``grad_norm`` holds the norm of the last step's gradients (a device scalar).
     """
 
     configs = {k: {"step": STEP_FNS[k], "states": v} for k, v in STATE_DTYPES.items()}
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.01,
-                 mode="stochastic_rounding", decoupled_weight_decay=False, seed=None):
+                 mode="stochastic_rounding", decoupled_weight_decay=False, seed=None,
+                 max_grad_norm=None):
         super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay))
         assert mode in self.configs, f"Invalid mode: {mode}"
         self.mode = mode
@@ -61,6 +66,10 @@ class Adam(MasterLoadingMixin, Optimizer):
         self.step_fn = self.config["step"]
         self.decoupled_weight_decay = decoupled_weight_decay
         self._has_master = "master_params" in self.config["states"]
+        if max_grad_norm is not None:
+            check_max_norm(max_grad_norm)
+        self.max_grad_norm = max_grad_norm
+        self.grad_norm = None
         self._rng = random.Random(seed)
         n_quant = sum(1 for g in self.param_groups for p in g["params"] if is_quant(p))
         if n_quant and mode != "fp32_master":
@@ -95,6 +104,10 @@ class Adam(MasterLoadingMixin, Optimizer):
             with torch.enable_grad():
                 loss = closure()
         states, with_seed = self.config["states"], self.mode == "stochastic_rounding"
+        clip = None
+        if self.max_grad_norm is not None:
+            clip, self.grad_norm = clip_coefficient(
+                (p for g in self.param_groups for p in g["params"]), self.max_grad_norm)
         for group in self.param_groups:
             due = []  # CUDA parameters of one step count, which the next launch takes
             fresh = 0  # elements of new state among them
@@ -110,7 +123,7 @@ class Adam(MasterLoadingMixin, Optimizer):
                     # a gradient in another dtype: one bf16 copy at a time
                     alone = not bf16 or not grad.is_cuda
                     if due and (alone or len(due) == MANY_TENSORS or state.get("step", 0) + 1 != due[0][2]["step"]):
-                        self._step_due(group, due)
+                        self._step_due(group, due, clip)
                         fresh = 0
                         if p.grad is None:  # a packed weight that the group lists twice
                             continue
@@ -130,13 +143,13 @@ class Adam(MasterLoadingMixin, Optimizer):
                     # a first step's allocations and launches alternate: the GPU works while the
                     # host allocates (4 M elements are 10 us of work, about a launch's host time)
                     if alone or fresh >= 1 << 22:
-                        self._step_due(group, due)
+                        self._step_due(group, due, clip)
                         fresh = 0
             finally:  # an error stops at its parameter: those before it are stepped
-                self._step_due(group, due)
+                self._step_due(group, due, clip)
         return loss
 
-    def _step_due(self, group, due):
+    def _step_due(self, group, due, clip):
         items = due[:]
         due.clear()
         if not items:
@@ -147,11 +160,11 @@ class Adam(MasterLoadingMixin, Optimizer):
             params, tensors, seed = items[0][3]
             if not tensors["grad"].is_cuda:  # one at a time
                 self.step_fn(params, tensors, group["lr"], group["weight_decay"], beta1, beta2, group["eps"], step,
-                             decoupled_weight_decay=self.decoupled_weight_decay,
+                             decoupled_weight_decay=self.decoupled_weight_decay, clip_coef=clip,
                              **({"seed": seed} if self.mode == "stochastic_rounding" else {}))
             else:
                 adam_step_many(self.mode, [it[3] for it in items], group["lr"], group["weight_decay"], beta1, beta2,
-                               group["eps"], step, self.decoupled_weight_decay)
+                               group["eps"], step, self.decoupled_weight_decay, clip)
             stepped = len(items)
         except Exception as e:
             stepped = getattr(e, "stepped", 0)

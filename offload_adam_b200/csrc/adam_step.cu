@@ -153,7 +153,8 @@ struct ManyTable {
 
 template <int MODE, bool DECOUPLED>
 __global__ void __launch_bounds__(kThreads, 3)
-adam_step_many_kernel(const __grid_constant__ ManyTable table, AdamScalars s) {
+adam_step_many_kernel(const __grid_constant__ ManyTable table, AdamScalars s, const float* __restrict__ clip_ptr) {
+  const float clip = clip_ptr != nullptr ? *clip_ptr : 1.0f;
   int lo = 0, hi = table.count - 1;  // the last tensor whose first CTA is not after this one
   while (lo < hi) {
     const int mid = (lo + hi + 1) >> 1;
@@ -172,12 +173,12 @@ adam_step_many_kernel(const __grid_constant__ ManyTable table, AdamScalars s) {
     for (int64_t vec = begin / kVec + threadIdx.x; vec < vec_end; vec += kThreads) {
       VecRegs<MODE> r;
       load_vec<MODE, false, false>(r, t, none, vec);
-      compute_vec<MODE, DECOUPLED, false, false>(r, vec, 1.0f, s, seed, 0);
+      compute_vec<MODE, DECOUPLED, false, false>(r, vec, clip, s, seed, 0);
       store_vec<MODE, false>(r, t, none, vec);
     }
   }
   for (int64_t i = scalar_begin + threadIdx.x; i < end; i += kThreads)
-    scalar_element<MODE, DECOUPLED>(t, i, false, 1.0f, s, seed, 0);
+    scalar_element<MODE, DECOUPLED>(t, i, false, clip, s, seed, 0);
 }
 
 // True when a tensor of the table writes what another one reads or writes: parameters that
@@ -210,14 +211,15 @@ bool share_memory(const ManyTable& t, int mode) {
 }
 
 template <int MODE>
-void launch_many(const ManyTable& t, unsigned grid, bool decoupled, const AdamScalars& s, cudaStream_t st) {
-  if (decoupled) adam_step_many_kernel<MODE, true><<<grid, kThreads, 0, st>>>(t, s);
-  else adam_step_many_kernel<MODE, false><<<grid, kThreads, 0, st>>>(t, s);
+void launch_many(const ManyTable& t, unsigned grid, bool decoupled, const AdamScalars& s, const float* clip, cudaStream_t st) {
+  if (decoupled) adam_step_many_kernel<MODE, true><<<grid, kThreads, 0, st>>>(t, s, clip);
+  else adam_step_many_kernel<MODE, false><<<grid, kThreads, 0, st>>>(t, s, clip);
 }
 }  // namespace
 
 cudaError_t launch_adam_step_many(ManyEntry* entries, int count, int mode, bool decoupled, float lr, float wd,
-                                  float beta1_hat, float beta2_hat, float eps, cudaStream_t stream) {
+                                  float beta1_hat, float beta2_hat, float eps, const float* clip_coef,
+                                  cudaStream_t stream) {
   AdamScalars s;
   s.lr = lr; s.wd = wd; s.lr_wd = lr * wd;
   s.one_m_b1h = 1.0f - beta1_hat; s.one_m_b2h = 1.0f - beta2_hat; s.eps = eps;
@@ -240,7 +242,8 @@ cudaError_t launch_adam_step_many(ManyEntry* entries, int count, int mode, bool 
     if (t.count == 0) continue;
     if (t.count > 1 && share_memory(t, mode)) {  // one after the other, as adam_step would
       for (int i = 0; i < t.count; ++i) {
-        const cudaError_t err = launch_adam_step_many(&t.e[i], 1, mode, decoupled, lr, wd, beta1_hat, beta2_hat, eps, stream);
+        const cudaError_t err = launch_adam_step_many(&t.e[i], 1, mode, decoupled, lr, wd, beta1_hat, beta2_hat, eps, clip_coef,
+                                                      stream);
         if (err != cudaSuccess) return err;
       }
       continue;
@@ -257,10 +260,10 @@ cudaError_t launch_adam_step_many(ManyEntry* entries, int count, int mode, bool 
     if (blocks >= (int64_t(1) << 31)) return cudaErrorInvalidValue;
     count_launch();
     switch (mode) {
-      case kModeSR: launch_many<kModeSR>(t, (unsigned)blocks, decoupled, s, stream); break;
-      case kModeFP32Master: launch_many<kModeFP32Master>(t, (unsigned)blocks, decoupled, s, stream); break;
-      case kModeFP31: launch_many<kModeFP31>(t, (unsigned)blocks, decoupled, s, stream); break;
-      case kModeCustom: launch_many<kModeCustom>(t, (unsigned)blocks, decoupled, s, stream); break;
+      case kModeSR: launch_many<kModeSR>(t, (unsigned)blocks, decoupled, s, clip_coef, stream); break;
+      case kModeFP32Master: launch_many<kModeFP32Master>(t, (unsigned)blocks, decoupled, s, clip_coef, stream); break;
+      case kModeFP31: launch_many<kModeFP31>(t, (unsigned)blocks, decoupled, s, clip_coef, stream); break;
+      case kModeCustom: launch_many<kModeCustom>(t, (unsigned)blocks, decoupled, s, clip_coef, stream); break;
       default: return cudaErrorInvalidValue;
     }
     const cudaError_t err = cudaGetLastError();

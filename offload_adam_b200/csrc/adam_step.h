@@ -75,10 +75,11 @@ struct ManyEntry {
 };
 // Steps `count` tensors that share mode and hyper-parameters, kManyTensors per launch; the
 // table travels as a kernel argument.  Each tensor gets the bits of its own
-// launch_adam_step (elem_offset 0, no clip, no peers).
+// launch_adam_step (elem_offset 0, no peers); `clip_coef` as there, one for all.
 constexpr int kManyTensors = 120;
 cudaError_t launch_adam_step_many(ManyEntry* entries, int count, int mode, bool decoupled, float lr, float wd,
-                                  float beta1_hat, float beta2_hat, float eps, cudaStream_t stream);
+                                  float beta1_hat, float beta2_hat, float eps, const float* clip_coef,
+                                  cudaStream_t stream);
 
 // Table-driven step over many small tensors in one launch.
 struct MultiTensorEntry {

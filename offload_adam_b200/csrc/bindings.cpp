@@ -135,12 +135,15 @@ void adam_step(int64_t mode, const OptT& p, const OptT& g, const OptT& g2, const
 // that adam_step refuses.
 int64_t adam_step_many(int64_t mode, const std::vector<OptT>& p, const std::vector<Tensor>& g, const std::vector<Tensor>& m,
                        const std::vector<Tensor>& v, const std::vector<OptT>& extra, const std::vector<int64_t>& seeds,
-                       double lr, double wd, double b1h, double b2h, double eps, bool decoupled) {
+                       double lr, double wd, double b1h, double b2h, double eps, bool decoupled, const OptT& clip) {
   const size_t k = g.size();
   TORCH_CHECK(p.size() == k && m.size() == k && v.size() == k && extra.size() == k && seeds.size() == k,
               "adam_step_many: lists of one length");
   std::vector<oab::ManyEntry> e;
   e.reserve(k);
+  const bool clipped = clip.has_value() && clip->defined();
+  TORCH_CHECK(!clipped || (clip->is_cuda() && clip->scalar_type() == at::kFloat && clip->numel() >= 1),
+              "clip_coef must be a CUDA fp32 scalar");
   try {
     for (size_t i = 0; i < k; ++i) {
       const auto a = make_args(mode, p[i], OptT(g[i]), OptT(), m[i], v[i], extra[i], lr, wd, b1h, b2h, eps, decoupled,
@@ -151,7 +154,7 @@ int64_t adam_step_many(int64_t mode, const std::vector<OptT>& p, const std::vect
   } catch (const c10::Error&) {  // tensor e.size() is refused
   }
   cu_check(oab::launch_adam_step_many(e.data(), (int)e.size(), (int)mode, decoupled, (float)lr, (float)wd, (float)b1h,
-                                      (float)b2h, (float)eps, pick_stream(0)),
+                                      (float)b2h, (float)eps, clipped ? clip->data_ptr<float>() : nullptr, pick_stream(0)),
            "adam_step_many launch");
   return (int64_t)e.size();
 }
@@ -461,6 +464,7 @@ struct PyEngine {
 
 void bind_loss(py::module_& m);
 void bind_linear_ce(py::module_& m);
+void bind_clip(py::module_& m);
 void bind_model(py::module_& m);
 void bind_quant(py::module_& m);
 void bind_symm(py::module_& m);
@@ -480,7 +484,9 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         py::arg("scratch") = py::none(), py::arg("max_ctas") = 0, py::arg("stream") = 0);
   m.def("clip_finalize", &clip_finalize, py::arg("slots"), py::arg("index"), py::arg("extra_sq"),
         py::arg("max_norm"), py::arg("coef_norm"), py::arg("total_sq"), py::arg("stream") = 0);
-  m.def("adam_step_many", &adam_step_many);
+  m.def("adam_step_many", &adam_step_many, py::arg("mode"), py::arg("p"), py::arg("g"), py::arg("m"), py::arg("v"), py::arg("extra"),
+        py::arg("seeds"), py::arg("lr"), py::arg("wd"), py::arg("b1h"), py::arg("b2h"), py::arg("eps"), py::arg("decoupled"),
+        py::arg("clip") = py::none());
   m.def("multi_tensor_adam", &multi_tensor_adam);
   m.def("multi_tensor_chunk", &oab::multi_tensor_chunk);
   m.def("sumsq_scratch_bytes", []() { return (int64_t)oab::kSumsqScratchBytes; });
@@ -565,6 +571,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
 
   bind_loss(m);
   bind_linear_ce(m);
+  bind_clip(m);
   bind_model(m);
   bind_quant(m);
   bind_symm(m);
