@@ -97,6 +97,24 @@ Tensor grad_norm(const std::vector<Tensor>& grads, int64_t norm, double max_norm
   return out;
 }
 
+// The same for the gradients of `params`; nothing (and nothing done) when one of them is not a
+// plain gradient of one CUDA device that the kernels take, or when there is none.
+std::optional<Tensor> param_grad_norm(const std::vector<Tensor>& params, int64_t norm, double max_norm, bool scale) {
+  std::vector<Tensor> grads;
+  grads.reserve(params.size());
+  for (const Tensor& p : params) {
+    const Tensor& g = p.grad();
+    if (!g.defined()) continue;
+    const auto t = g.scalar_type();
+    if (!g.is_cuda() || g.layout() != at::kStrided || g.key_set().has(c10::DispatchKey::Python) ||
+        (t != at::kBFloat16 && t != at::kHalf && t != at::kFloat) || g.get_device() != (grads.empty() ? g : grads[0]).get_device())
+      return std::nullopt;
+    grads.push_back(g);
+  }
+  if (grads.empty()) return std::nullopt;
+  return grad_norm(grads, norm, max_norm, scale);
+}
+
 // The gradients times `coef`, one fp32 value on their device.
 void grad_scale(const std::vector<Tensor>& grads, const Tensor& coef) {
   if (grads.empty()) return;
@@ -112,5 +130,6 @@ void grad_scale(const std::vector<Tensor>& grads, const Tensor& coef) {
 
 void bind_clip(py::module_& m) {
   m.def("grad_norm", &grad_norm, py::arg("grads"), py::arg("norm"), py::arg("max_norm"), py::arg("scale"));
+  m.def("param_grad_norm", &param_grad_norm, py::arg("params"), py::arg("norm"), py::arg("max_norm"), py::arg("scale"));
   m.def("grad_scale", &grad_scale, py::arg("grads"), py::arg("coef"));
 }

@@ -34,8 +34,9 @@ constexpr int kInner = 64;                              // inner values of a sta
 constexpr int kStages = 6;
 constexpr int kHalfBytes = 128 * kInner * 2;            // one CTA's part of an operand's stage
 constexpr int kStageBytes = 2 * kHalfBytes;
-constexpr int kSmemBytes = kStages * kStageBytes + 1024;  // stages start on 1024 bytes
 constexpr int kEpilogueWarps = 8;
+constexpr int kStagingBytes = 32 * 128;  // of an epilogue warp: 32 lines of 128 bytes on their way out
+constexpr int kSmemBytes = kStages * kStageBytes + kEpilogueWarps * kStagingBytes + 1024;  // starts on 1024 bytes
 constexpr int kGemmThreads = 64 + 32 * kEpilogueWarps;
 constexpr int kGroup = 16;  // row tiles that share a column tile in turn: 4096 rows of h stay in L2
 
@@ -44,6 +45,8 @@ enum Pass { kStats = 0, kLogitGrad = 1, kGrads = 2 };
 struct GemmParams {
   CUtensorMap a, b;    // kStats, kLogitGrad: packed rows and W.  kGrads: d and W, for dh
   CUtensorMap a2, b2;  // kGrads: d and packed rows, for dW
+  CUtensorMap out;     // kLogitGrad: d.  kGrads: dW
+  CUtensorMap out_acc; // kGrads: the fp32 sums of dh, by split
   const int* count;
   int64_t rows;        // capacity of the per-row arrays
   int64_t padded;
@@ -59,15 +62,12 @@ struct GemmParams {
   // kLogitGrad
   const float* lse;
   const float* row_g;  // by row, or null
-  uint16_t* d;
-  int64_t pitch;
-  // kGrads
   const int* index;
+  // kGrads
   const float *inv, *g;  // each may be null (1)
-  float* acc;
-  uint16_t *gh, *gw;
+  int want_dh, want_dw;
   int splits;
-  int first, last;
+  int first;             // piece: its dh starts the sums
 };
 
 __device__ __forceinline__ float exp_of(float x) {  // relative error below 2^-21 for |x| < 20
@@ -84,26 +84,58 @@ struct Tile {
   int split;
 };
 
-// Tiles of a pass and the t-th of them.  Column tiles turn slower than up to kGroup row tiles.
+// Tiles of a pass, and which of them a CTA pair takes.  Column tiles turn slower than up to kGroup
+// row tiles.
 struct Plan {
   int mt, nt, per_split, dh_tiles, wt, ht, total, k_steps, row_steps;
+  int pairs, alone, first_dw;  // see pick
   template <int PASS>
-  __device__ __forceinline__ void make(const GemmParams& p, int n_rows) {
+  __device__ __forceinline__ void make(const GemmParams& p, int n_rows, int n_pairs) {
     mt = (n_rows + kTile - 1) / kTile;
+    pairs = n_pairs;
     if (PASS == kGrads) {
       ht = (p.hidden + kTile - 1) / kTile;
       nt = ht;
-      wt = p.gw != nullptr ? (p.words + kTile - 1) / kTile : 0;
+      wt = p.want_dw ? (p.words + kTile - 1) / kTile : 0;
       per_split = mt * nt;
-      dh_tiles = p.gh != nullptr ? per_split * p.splits : 0;
+      dh_tiles = p.want_dh ? per_split * p.splits : 0;
       total = dh_tiles + wt * ht;
       k_steps = (p.words + kInner - 1) / kInner;
       row_steps = (n_rows + kInner - 1) / kInner;
+      // The tiles of dh are long (a sum over the words) and come first, those of dW (a sum over the
+      // rows) fill up.  Pairs that a last, partial round of dh leaves idle take as many tiles
+      // of dW as such a tile is long before the others join in.  4096 rows, hidden 4096, 32768
+      // words: 256 tiles of dh for 74 pairs; shared out in turn the launch took 1500 us.
+      alone = dh_tiles % pairs;
+      first_dw = 0;
+      if (alone != 0 && wt > 0) {
+        const int length = (k_steps + p.splits - 1) / p.splits + 2, one = row_steps + 2;
+        const int64_t fill = (int64_t)(length / one) * (pairs - alone);
+        first_dw = (int)(fill < (int64_t)wt * ht ? fill : (int64_t)wt * ht);
+      }
     } else {
       nt = (p.words + kTile - 1) / kTile;
       total = mt * nt;
       k_steps = (p.hidden + kInner - 1) / kInner;
     }
+  }
+  // The `turn`-th tile of `pair`, or -1.
+  template <int PASS>
+  __device__ __forceinline__ int pick(int pair, int turn) const {
+    if (PASS != kGrads) {
+      const int t = pair + turn * pairs;
+      return t < total ? t : -1;
+    }
+    const int rounds = dh_tiles / pairs + (pair < alone ? 1 : 0);
+    if (turn < rounds) return pair + turn * pairs;
+    turn -= rounds;
+    if (pair >= alone && first_dw > 0) {
+      const int idle = pairs - alone, own = first_dw / idle + (pair - alone < first_dw % idle ? 1 : 0);
+      if (turn < own) return dh_tiles + (pair - alone) + turn * idle;
+      turn -= own;
+    }
+    const int64_t t = (int64_t)dh_tiles + first_dw + pair + (int64_t)turn * pairs;
+    return t < total ? (int)t : -1;
   }
   __device__ __forceinline__ static void place(int t, int mt, int nt, int& m, int& n) {
     const int g = t / (kGroup * nt), first = g * kGroup, r = t - g * kGroup * nt;
@@ -180,13 +212,31 @@ __device__ __forceinline__ void stats_tile(const GemmParams& p, const Tile& x, u
   if (row < n_rows) p.part[(int64_t)(x.n / 128 + half) * p.rows + row] = make_float2(m, s);
 }
 
-__device__ __forceinline__ void logit_grad_tile(const GemmParams& p, const Tile& x, uint32_t tmem, int row, int n_rows, int half) {
+// A warp's 32 lines of 128 bytes leave through its staging buffer, 16-byte parts swizzled as TMA
+// expects them (part c of line r at c ^ (r % 8), which also keeps the stores free of bank
+// conflicts).  A store a thread, straight from its row, touched 32 lines an instruction: a tile of
+// dW took longer to write than 10 stages to compute.
+__device__ __forceinline__ void stage_begin(int lane) {
+  if (lane == 0) store_wait_read();
+  __syncwarp();
+}
+__device__ __forceinline__ void stage_part(uint32_t staging, int lane, int c, uint32_t w0, uint32_t w1, uint32_t w2, uint32_t w3) {
+  st_shared16(staging + lane * 128 + ((c ^ (lane & 7)) << 4), w0, w1, w2, w3);
+}
+// 64 columns as bf16
+__device__ __forceinline__ void stage_bf16(uint32_t staging, int lane, int half32, const float (&v)[32]) {
+#pragma unroll
+  for (int c = 0; c < 4; ++c)
+    stage_part(staging, lane, half32 * 4 + c, f32x2_to_bf16x2_rne(v[8 * c], v[8 * c + 1]), f32x2_to_bf16x2_rne(v[8 * c + 2], v[8 * c + 3]),
+               f32x2_to_bf16x2_rne(v[8 * c + 4], v[8 * c + 5]), f32x2_to_bf16x2_rne(v[8 * c + 6], v[8 * c + 7]));
+}
+
+__device__ __forceinline__ void logit_grad_tile(const GemmParams& p, const Tile& x, uint32_t tmem, int row, int n_rows, int half,
+                                                uint32_t staging, int lane) {
   const bool in = row < n_rows;
   const int lab = in && p.label[row] >= 0 ? (int)(p.label[row] - p.word0) : -1;
   const float lse = in ? p.lse[row] : 0.f;
   const float g = !in ? 0.f : p.row_g != nullptr ? p.row_g[p.index[row]] : 1.f;
-  // rows that pad the inner dimension of dW are zero
-  const bool store = row < (n_rows + kLceRowPad - 1) / kLceRowPad * kLceRowPad;
 #pragma unroll 1
   for (int c = 0; c < 4; ++c) {
     float v[32];
@@ -200,65 +250,65 @@ __device__ __forceinline__ void logit_grad_tile(const GemmParams& p, const Tile&
       for (int i = 0; i < 32; ++i)
         if (i == hit) v[i] = __fsub_rn(v[i], 1.f);
     }
-    V8 o[2];
+    // rows that pad the inner dimension of dW are zero, whatever stands in them
 #pragma unroll
-    for (int i = 0; i < 16; ++i)
-      o[i >> 3].w[i & 7] = in ? f32x2_to_bf16x2_rne(__fmul_rn(v[2 * i], g), __fmul_rn(v[2 * i + 1], g)) : 0u;
-    if (store) {
-      uint16_t* at = p.d + (int64_t)row * p.pitch + col;
-      if (col < p.pitch) st32(at, o[0]);
-      if (col + 16 < p.pitch) st32(at + 16, o[1]);
+    for (int i = 0; i < 32; ++i) v[i] = in ? __fmul_rn(v[i], g) : 0.f;
+    if ((c & 1) == 0) stage_begin(lane);
+    stage_bf16(staging, lane, c & 1, v);
+    if ((c & 1) == 1) {
+      store_fence();
+      __syncwarp();
+      if (lane == 0 && col - 32 < p.words && row < p.padded) {
+        tma_store(&p.out, staging, col - 32, row);
+        store_commit();
+      }
     }
   }
 }
 
-__device__ __forceinline__ void store_bf16x8(uint16_t* at, const float* v, float scale) {
-  uint4 o;
-  o.x = f32x2_to_bf16x2_rne(__fmul_rn(v[0], scale), __fmul_rn(v[1], scale));
-  o.y = f32x2_to_bf16x2_rne(__fmul_rn(v[2], scale), __fmul_rn(v[3], scale));
-  o.z = f32x2_to_bf16x2_rne(__fmul_rn(v[4], scale), __fmul_rn(v[5], scale));
-  o.w = f32x2_to_bf16x2_rne(__fmul_rn(v[6], scale), __fmul_rn(v[7], scale));
-  *reinterpret_cast<uint4*>(at) = o;
-}
-
-__device__ __forceinline__ void grads_tile(const GemmParams& p, const Tile& x, uint32_t tmem, int row, int n_rows, int half, float scale) {
-  // x.steps == 0 happens only for dW without a row that counts
-  const bool direct = x.kind == 1 || (p.last && p.splits == 1);  // the rounded result goes out
-  const bool add = x.kind == 0 && !p.first;
-  const bool in = x.kind == 1 ? row < p.words : row < n_rows;
-  float* acc = nullptr;
-  uint16_t* out = nullptr;
-  if (in) {
-    if (x.kind == 1) out = p.gw + (p.word0 + row) * p.hidden;
-    else if (direct) out = p.gh + (int64_t)p.index[row] * p.hidden;
-    if (x.kind == 0 && p.acc != nullptr) acc = p.acc + ((int64_t)x.split * p.padded + row) * p.hidden;
-  }
+__device__ __forceinline__ void dh_tile(const GemmParams& p, const Tile& x, uint32_t tmem, int row, int n_rows, int half,
+                                        uint32_t staging, int lane) {
 #pragma unroll 1
   for (int c = 0; c < 4; ++c) {
     float v[32];
     tmem_load32(tmem + c * 32, v);
-    if (x.steps == 0) {
+    const int col = x.n + half * 128 + c * 32;
+    if (x.steps == 0) {  // a last piece of fewer stages than splits: nothing was summed
 #pragma unroll
       for (int i = 0; i < 32; ++i) v[i] = 0.f;
     }
+    stage_begin(lane);
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      stage_part(staging, lane, i, __float_as_uint(v[4 * i]), __float_as_uint(v[4 * i + 1]), __float_as_uint(v[4 * i + 2]),
+                 __float_as_uint(v[4 * i + 3]));
+    store_fence();
+    __syncwarp();
+    if (lane == 0 && col < p.hidden && row < n_rows) {
+      tma_store3(&p.out_acc, staging, col, row, x.split, !p.first);
+      store_commit();
+    }
+  }
+}
+
+__device__ __forceinline__ void dw_tile(const GemmParams& p, const Tile& x, uint32_t tmem, int row, int half, float scale,
+                                        uint32_t staging, int lane) {
+#pragma unroll 1
+  for (int c = 0; c < 4; ++c) {
+    float v[32];
+    tmem_load32(tmem + c * 32, v);
     const int col = x.n + half * 128 + c * 32;
+    // no row that counts: nothing was summed
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      const int at = col + q * 8;
-      if (!in || at >= p.hidden) continue;
-      float* w = v + q * 8;
-      if (add) {
-        const V8 old = ld32(acc + at);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) w[i] = __fadd_rn(__uint_as_float(old.w[i]), w[i]);
-      }
-      if (direct) {
-        store_bf16x8(out + at, w, scale);
-      } else {
-        V8 o;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) o.w[i] = __float_as_uint(w[i]);
-        st32(acc + at, o);
+    for (int i = 0; i < 32; ++i) v[i] = x.steps != 0 ? __fmul_rn(v[i], scale) : 0.f;
+    if ((c & 1) == 0) stage_begin(lane);
+    stage_bf16(staging, lane, c & 1, v);
+    if ((c & 1) == 1) {
+      store_fence();
+      __syncwarp();
+      if (lane == 0 && col - 32 < p.hidden && row < p.words) {
+        tma_store(&p.out, staging, col - 32, (int)p.word0 + row);
+        store_commit();
       }
     }
   }
@@ -300,15 +350,15 @@ lce_product_kernel(const __grid_constant__ GemmParams p) {
 
   const int n_rows = *p.count;
   Plan plan{};
-  plan.make<PASS>(p, n_rows);
-  const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
+  plan.make<PASS>(p, n_rows, gridDim.x >> 1);
+  const int pair = blockIdx.x >> 1;
   bool ok = true;
 
   if (warp == 0) {
     if (elect_one()) {
       const uint32_t lead_full0 = map_to_rank(full0, 0);
       int it = 0;
-      for (int t = pair; t < plan.total && ok; t += pairs) {
+      for (int turn = 0, t; ok && (t = plan.pick<PASS>(pair, turn)) >= 0; ++turn) {
         const Tile x = plan.at<PASS>(p, t);
         const bool outer_a = PASS == kGrads && x.kind == 1, outer_b = PASS == kGrads;
         const CUtensorMap* ma = outer_a ? &p.a2 : &p.a;
@@ -345,8 +395,8 @@ lce_product_kernel(const __grid_constant__ GemmParams p) {
     __syncwarp();
   } else if (warp == 1) {
     if (rank == 0 && elect_one()) {
-      int it = 0, mine = 0;
-      for (int t = pair; t < plan.total && ok; t += pairs, ++mine) {
+      int it = 0;
+      for (int mine = 0, t; ok && (t = plan.pick<PASS>(pair, mine)) >= 0; ++mine) {
         const Tile x = plan.at<PASS>(p, t);
         const bool outer_a = PASS == kGrads && x.kind == 1;
         constexpr bool outer_b = PASS == kGrads;
@@ -379,8 +429,8 @@ lce_product_kernel(const __grid_constant__ GemmParams p) {
       if (p.inv != nullptr) scale = *p.inv;
       if (p.g != nullptr) scale = __fmul_rn(scale, *p.g);
     }
-    int mine = 0;
-    for (int t = pair; t < plan.total; t += pairs, ++mine) {
+    const uint32_t staging = stages + kStages * kStageBytes + (warp - 2) * kStagingBytes;
+    for (int mine = 0, t; (t = plan.pick<PASS>(pair, mine)) >= 0; ++mine) {
       const Tile x = plan.at<PASS>(p, t);
       const uint32_t acc = mine & 1;
       ok = mbar_wait(done0 + 8 * acc, (mine >> 1) & 1);
@@ -390,12 +440,15 @@ lce_product_kernel(const __grid_constant__ GemmParams p) {
       const uint32_t at = tmem + acc * kTile + half * 128 + ((uint32_t)(quarter * 32) << 16);
       const int row = x.m + (int)rank * 128 + quarter * 32 + lane;
       if (PASS == kStats) stats_tile(p, x, at, row, n_rows, half);
-      if (PASS == kLogitGrad) logit_grad_tile(p, x, at, row, n_rows, half);
-      if (PASS == kGrads) grads_tile(p, x, at, row, n_rows, half, scale);
+      if (PASS == kLogitGrad) logit_grad_tile(p, x, at, row, n_rows, half, staging, lane);
+      if (PASS == kGrads && x.kind == 0) dh_tile(p, x, at, row, n_rows, half, staging, lane);
+      if (PASS == kGrads && x.kind == 1) dw_tile(p, x, at, row, half, scale, staging, lane);
       fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive_cluster(lead_drained0 + 8 * acc);
     }
+    if (PASS != kStats && lane == 0) store_wait();
+    __syncwarp();
   }
   if (!ok) gave_up = 1;
   fence_before();
@@ -478,8 +531,10 @@ lce_pack_kernel(const uint16_t* __restrict__ h, int64_t stride, const int64_t* _
 }
 
 // ------------------------------------------------------------ joining the sums
-// 32 rows and 32 slices of the words a block.
-constexpr int kJoinThreads = 1024;
+// A block has 8 rows (the partials of 4 are one 32-byte sector) and 64 slices of the words; a thread
+// loads eight partials at a time.  One row of 128256 words: 1002 partials, 20 us with one load at a
+// time in 32 slices.
+constexpr int kJoinRows = 8, kJoinSlices = 64, kJoinThreads = kJoinRows * kJoinSlices, kJoinLoads = 8;
 __device__ __forceinline__ void join(float& m, float& s, float m2, float s2) {
   const float mn = fmaxf(m, m2), sh = finite_shift(mn);
   s = __fadd_rn(__fmul_rn(s, expf(__fsub_rn(m, sh))), __fmul_rn(s2, expf(__fsub_rn(m2, sh))));
@@ -489,54 +544,63 @@ __global__ void __launch_bounds__(kJoinThreads)
 lce_join_kernel(const float2* __restrict__ part, int parts, int64_t rows, const int* __restrict__ index,
                 const int* __restrict__ label, int* count, const float* __restrict__ picked, const float* __restrict__ inv,
                 float* lse, int reduction, double* sums, float* loss) {
-  __shared__ float sm[32][33], ss[32][33];
+  __shared__ float sm[kJoinSlices][kJoinRows], ss[kJoinSlices][kJoinRows], one[kJoinRows];
   __shared__ int is_last;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int n = *count;
-  const int64_t row = (int64_t)blockIdx.x * 32 + lane;
+  const int n = *count, of = threadIdx.x % kJoinRows, slice = threadIdx.x / kJoinRows;
+  const int64_t row = (int64_t)blockIdx.x * kJoinRows + of;
   float m = -INFINITY, s = 0.f;
   if (row < n) {
-#pragma unroll 4
-    for (int i = warp; i < parts; i += 32) {
-      const float2 x = part[(int64_t)i * rows + row];
-      join(m, s, x.x, x.y);
+    for (int i = slice; i < parts; i += kJoinSlices * kJoinLoads) {
+      float2 x[kJoinLoads];
+      float mn = m;
+#pragma unroll
+      for (int u = 0; u < kJoinLoads; ++u) {
+        const int at = i + u * kJoinSlices;
+        x[u] = at < parts ? part[(int64_t)at * rows + row] : make_float2(-INFINITY, 0.f);
+      }
+#pragma unroll
+      for (int u = 0; u < kJoinLoads; ++u) mn = fmaxf(mn, x[u].x);
+      const float sh = finite_shift(mn);
+      s = __fmul_rn(s, expf(__fsub_rn(m, sh)));
+#pragma unroll
+      for (int u = 0; u < kJoinLoads; ++u) s = __fadd_rn(s, __fmul_rn(x[u].y, expf(__fsub_rn(x[u].x, sh))));
+      m = mn;
     }
   }
-  sm[warp][lane] = m;
-  ss[warp][lane] = s;
+  sm[slice][of] = m;
+  ss[slice][of] = s;
   __syncthreads();
-  // warp w finishes the block's row w: lane i has slice i
-  m = sm[lane][warp];
-  s = ss[lane][warp];
+  if (warp < kJoinRows) {  // warp w finishes the block's row w
+    m = sm[lane][warp];
+    s = ss[lane][warp];
+    join(m, s, sm[lane + 32][warp], ss[lane + 32][warp]);
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    const float m2 = __shfl_xor_sync(0xffffffffu, m, o), s2 = __shfl_xor_sync(0xffffffffu, s, o);
-    join(m, s, m2, s2);
-  }
-  const int64_t at = (int64_t)blockIdx.x * 32 + warp;
-  float one = 0.f;
-  if (at < n) {
-    const bool known = label[at] >= 0;
-    const float l = !known ? NAN : isinf(m) ? m : __fadd_rn(m, logf(s));
-    one = known ? __fsub_rn(l, picked[at]) : NAN;
+    for (int o = 16; o > 0; o >>= 1) {
+      const float m2 = __shfl_xor_sync(0xffffffffu, m, o), s2 = __shfl_xor_sync(0xffffffffu, s, o);
+      join(m, s, m2, s2);
+    }
+    const int64_t at = (int64_t)blockIdx.x * kJoinRows + warp;
     if (lane == 0) {
-      lse[at] = l;
-      if (reduction == kLceNone) loss[index[at]] = one;
+      float loss_of = 0.f;
+      if (at < n) {
+        const bool known = label[at] >= 0;
+        const float l = !known ? NAN : isinf(m) ? m : __fadd_rn(m, logf(s));
+        loss_of = known ? __fsub_rn(l, picked[at]) : NAN;
+        lse[at] = l;
+        if (reduction == kLceNone) loss[index[at]] = loss_of;
+      }
+      one[warp] = loss_of;
     }
   }
   if (reduction == kLceNone) return;
   __syncthreads();
-  if (lane == 0) sm[0][warp] = one;
-  __syncthreads();
-  if (warp == 0) {  // the same order whatever the blocks' order
-    double t = sm[0][lane];
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
-    if (lane == 0) {
-      sums[blockIdx.x] = t;
-      __threadfence();
-      is_last = atomicAdd(count + 1, 1) == (int)gridDim.x - 1;
-    }
+  if (threadIdx.x == 0) {  // the same order whatever the blocks' order
+    double t = 0.0;
+    for (int i = 0; i < kJoinRows; ++i) t += one[i];
+    sums[blockIdx.x] = t;
+    __threadfence();
+    is_last = atomicAdd(count + 1, 1) == (int)gridDim.x - 1;
   }
   __syncthreads();
   if (is_last && warp == 0) {
@@ -549,7 +613,15 @@ lce_join_kernel(const float2* __restrict__ part, int parts, int64_t rows, const 
   }
 }
 
-// ------------------------------------------------------- splits of dh, joined
+// -------------------------------------------------- dh: splits joined, rounded
+__device__ __forceinline__ void store_bf16x8(uint16_t* at, const float* v, float scale) {
+  uint4 o;
+  o.x = f32x2_to_bf16x2_rne(__fmul_rn(v[0], scale), __fmul_rn(v[1], scale));
+  o.y = f32x2_to_bf16x2_rne(__fmul_rn(v[2], scale), __fmul_rn(v[3], scale));
+  o.z = f32x2_to_bf16x2_rne(__fmul_rn(v[4], scale), __fmul_rn(v[5], scale));
+  o.w = f32x2_to_bf16x2_rne(__fmul_rn(v[6], scale), __fmul_rn(v[7], scale));
+  *reinterpret_cast<uint4*>(at) = o;
+}
 __global__ void __launch_bounds__(128)
 lce_join_grad_kernel(const float* __restrict__ acc, int splits, int64_t padded, const int* __restrict__ index,
                      const int* __restrict__ count, int hidden, const float* inv, const float* g, uint16_t* gh) {
@@ -581,7 +653,18 @@ PFN_cuTensorMapEncodeTiled_v12000 encoder() {
   return fn;
 }
 
-// Boxes of 64 contiguous values and `lines` lines of a bf16 matrix; what lies outside reads as zero.
+// The fp32 sums of dh as (hidden, rows, splits) in boxes of 32 columns and 32 rows.
+bool encode_acc(CUtensorMap* map, float* base, int64_t hidden, int64_t padded, int splits) {
+  const auto fn = encoder();
+  if (fn == nullptr) return false;
+  const cuuint64_t dims[3] = {(cuuint64_t)hidden, (cuuint64_t)padded, (cuuint64_t)splits};
+  const cuuint64_t strides[2] = {(cuuint64_t)hidden * 4, (cuuint64_t)hidden * 4 * (cuuint64_t)padded};
+  const cuuint32_t box[3] = {32, 32, 1}, steps[3] = {1, 1, 1};
+  return fn(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 3, base, dims, strides, box, steps, CU_TENSOR_MAP_INTERLEAVE_NONE,
+            CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+// Boxes of 64 contiguous values and `lines` lines of a bf16 matrix; what lies outside reads as zero
+// and is not written.
 bool encode(CUtensorMap* map, const void* base, int64_t inner, int64_t lines_all, int64_t stride, int lines) {
   const auto fn = encoder();
   if (fn == nullptr) return false;
@@ -635,7 +718,7 @@ cudaError_t pack_rows(const LceArgs& a, void* gh, cudaStream_t st) {
 }  // namespace
 
 int64_t lce_part_floats(int64_t rows, int64_t vocab) { return 4 * tiles_of(vocab) * rows; }
-int64_t lce_sum_doubles(int64_t rows) { return (rows + 31) / 32; }
+int64_t lce_sum_doubles(int64_t rows) { return (rows + kJoinRows - 1) / kJoinRows; }
 
 cudaError_t launch_lce_forward(const LceArgs& a, int reduction, float* part, float* picked, double* sums, float* loss,
                                cudaStream_t st) {
@@ -675,40 +758,39 @@ int lce_splits(int64_t rows, int64_t hidden, int64_t vocab, int64_t piece) {
 cudaError_t launch_lce_backward(const LceArgs& a, const LceGrad& g, cudaStream_t st) {
   if (!args_ok(a) || g.piece <= 0 || g.piece % kTile != 0 || g.splits < 1 || g.g == nullptr) return cudaErrorInvalidValue;
   if (g.gh == nullptr && g.gw == nullptr) return cudaSuccess;
+  if (g.d == nullptr || (g.gh != nullptr && g.acc == nullptr)) return cudaErrorInvalidValue;
   cudaError_t e = pack_rows(a, g.gh, st);
   if (e != cudaSuccess) return e;
   const int64_t pieces = lce_pieces(a.vocab, g.piece), pitch = lce_piece_pitch(a.vocab, g.piece);
-  if (g.gh != nullptr && (pieces > 1 || g.splits > 1) && g.acc == nullptr) return cudaErrorInvalidValue;
   GemmParams p{};
   common_params(p, a);
   p.lse = a.lse;
   p.row_g = g.reduction == kLceNone ? g.g : nullptr;
-  p.d = (uint16_t*)g.d;
-  p.pitch = pitch;
   GemmParams q{};
   common_params(q, a);
   q.inv = g.reduction == kLceMean ? a.inv : nullptr;
   q.g = g.reduction == kLceNone ? nullptr : g.g;
-  q.acc = g.acc;
-  q.gh = (uint16_t*)g.gh;
-  q.gw = (uint16_t*)g.gw;
+  q.want_dh = g.gh != nullptr;
+  q.want_dw = g.gw != nullptr;
   q.splits = g.splits;
   if (!encode(&p.a, a.packed, a.hidden, p.padded, a.hidden, 128) || !encode(&p.b, a.w, a.hidden, a.vocab, a.w_stride, 128) ||
-      !encode(&q.b, a.w, a.hidden, a.vocab, a.w_stride, 64) || !encode(&q.b2, a.packed, a.hidden, p.padded, a.hidden, 64))
+      !encode(&q.b, a.w, a.hidden, a.vocab, a.w_stride, 64) || !encode(&q.b2, a.packed, a.hidden, p.padded, a.hidden, 64) ||
+      (q.want_dw && !encode(&q.out, g.gw, a.hidden, a.vocab, a.hidden, 32)) ||
+      (q.want_dh && !encode_acc(&q.out_acc, g.acc, a.hidden, p.padded, g.splits)))
     return cudaErrorInvalidValue;
   for (int64_t i = 0; i < pieces; ++i) {
     p.word0 = q.word0 = i * g.piece;
     p.words = q.words = (int)(a.vocab - p.word0 < g.piece ? a.vocab - p.word0 : g.piece);
     q.first = i == 0;
-    q.last = i == pieces - 1;
-    if ((e = launch_product<kLogitGrad>(p, tiles_of(a.rows) * tiles_of(p.words), st)) != cudaSuccess) return e;
-    if (!encode(&q.a, g.d, q.words, p.padded, pitch, 128) || !encode(&q.a2, g.d, q.words, p.padded, pitch, 64))
+    if (!encode(&p.out, g.d, q.words, p.padded, pitch, 32) || !encode(&q.a, g.d, q.words, p.padded, pitch, 128) ||
+        !encode(&q.a2, g.d, q.words, p.padded, pitch, 64))
       return cudaErrorInvalidValue;
-    const int64_t dh = g.gh != nullptr ? tiles_of(a.rows) * tiles_of(a.hidden) * g.splits : 0;
-    const int64_t dw = g.gw != nullptr ? tiles_of(q.words) * tiles_of(a.hidden) : 0;
+    if ((e = launch_product<kLogitGrad>(p, tiles_of(a.rows) * tiles_of(p.words), st)) != cudaSuccess) return e;
+    const int64_t dh = q.want_dh ? tiles_of(a.rows) * tiles_of(a.hidden) * g.splits : 0;
+    const int64_t dw = q.want_dw ? tiles_of(q.words) * tiles_of(a.hidden) : 0;
     if ((e = launch_product<kGrads>(q, dh + dw, st)) != cudaSuccess) return e;
   }
-  if (g.gh != nullptr && g.splits > 1) {
+  if (g.gh != nullptr) {
     count_launch();
     lce_join_grad_kernel<<<dim3((unsigned)a.rows, (unsigned)((a.hidden + 1023) / 1024)), 128, 0, st>>>(
         g.acc, g.splits, p.padded, a.index, a.count, (int)a.hidden, q.inv, q.g, (uint16_t*)g.gh);

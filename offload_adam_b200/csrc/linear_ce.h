@@ -48,7 +48,7 @@ struct LceGrad {
   int64_t piece = 0;          // words at a time, a multiple of kLceTile
   void* d = nullptr;          // bf16 (padded rows, lce_piece_pitch)
   int splits = 1;             // of the sum over the words in gh
-  float* acc = nullptr;       // fp32 (splits, padded rows, hidden), unless one piece and one split
+  float* acc = nullptr;       // fp32 (splits, padded rows, hidden), for gh
 };
 inline int64_t lce_pieces(int64_t vocab, int64_t piece) { return (vocab + piece - 1) / piece; }
 inline int64_t lce_piece_pitch(int64_t vocab, int64_t piece) { return ((vocab < piece ? vocab : piece) + 15) / 16 * 16; }

@@ -101,10 +101,8 @@ struct LinearCE : torch::autograd::Function<LinearCE> {
     if (want_h) {
       gh = at::empty({rows, hidden}, h.options());
       x.gh = gh.data_ptr();
-      if (x.splits > 1 || oab::lce_pieces(vocab, piece) > 1) {
-        acc = at::empty({x.splits, oab::lce_padded(rows), hidden}, h.options().dtype(at::kFloat));
-        x.acc = acc.data_ptr<float>();
-      }
+      acc = at::empty({x.splits, oab::lce_padded(rows), hidden}, h.options().dtype(at::kFloat));
+      x.acc = acc.data_ptr<float>();
     }
     if (want_w) {
       gw = at::empty({vocab, hidden}, w.options());

@@ -9,6 +9,16 @@ from offload_adam_b200 import Adam, _ext, clip_grad_norm_, grad_norm
 from offload_adam_b200.adam import STATE_DTYPES
 
 gpu = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module", autouse=True)
+def _leave_no_cached_blocks():
+    """Tests that measure peak memory count whole cached blocks, whoever left them."""
+    yield
+    if torch.cuda.is_available():
+        torch.cuda.empty_cache()
+
+
 DEVICES = ["cpu", pytest.param("cuda", marks=gpu)]
 NORMS = [2.0, 1.0, math.inf]
 BF16, F16, F32 = torch.bfloat16, torch.float16, torch.float32
