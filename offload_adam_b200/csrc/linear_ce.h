@@ -11,7 +11,7 @@ constexpr int kLceRowPad = 64;    // the packed rows are padded with zeros to a 
 // Operands and workspaces of one loss.  `rows` are the rows of h; the kernels work on those whose
 // label counts, packed in order: how many there are is known on the device only.
 struct LceArgs {
-  const void* h = nullptr;           // bf16 (rows, hidden), unit column stride
+  const void* h = nullptr;           // bf16 (rows, hidden), unit column stride; forward only
   int64_t h_stride = 0;              // elements, a multiple of 8; h is 16-byte aligned
   const void* w = nullptr;           // bf16 (vocab, hidden), likewise
   int64_t w_stride = 0;
@@ -23,7 +23,6 @@ struct LceArgs {
   int* count = nullptr;              // [0] packed rows, [1] ticket
   float* inv = nullptr;              // 1 / max(1, packed rows)
   float* lse = nullptr;              // (rows,) of the packed row
-  // scratch of one direction
   void* packed = nullptr;            // bf16 (rows padded, hidden)
   int64_t* report = nullptr;         // host memory: [0] a label outside the vocabulary, [1] a wait that gave up
 };

@@ -3,6 +3,8 @@
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/extension.h>
 
+#include <algorithm>
+
 #include "linear_ce.h"
 #include "loss_ops.h"
 
@@ -27,15 +29,13 @@ int64_t row_stride(const Tensor& t) { return t.size(0) == 1 ? t.size(1) : t.stri
 // What backward needs of forward, in one int32 tensor: index, label and lse of the packed rows,
 // their number with the ticket, 1 / number.
 int64_t kept_words(int64_t rows) { return 3 * rows + 4; }
-oab::LceArgs make_args(const Tensor& h, const Tensor& w, const Tensor& labels, const Tensor& kept, int64_t ignore, const Tensor& packed) {
+oab::LceArgs make_args(const Tensor& w, const Tensor& labels, const Tensor& kept, int64_t ignore, const Tensor& packed) {
   oab::LceArgs a;
-  a.h = h.data_ptr();
-  a.h_stride = row_stride(h);
   a.w = w.data_ptr();
   a.w_stride = row_stride(w);
   a.labels = labels.data_ptr<int64_t>();
-  a.rows = h.size(0);
-  a.hidden = h.size(1);
+  a.rows = labels.size(0);
+  a.hidden = w.size(1);
   a.vocab = w.size(0);
   a.ignore = ignore;
   int* k = kept.data_ptr<int>();
@@ -48,6 +48,19 @@ oab::LceArgs make_args(const Tensor& h, const Tensor& w, const Tensor& labels, c
   a.report = oab::loss_report();
   return a;
 }
+// Fresh memory for the values of one call, cut into parts that start on 256 bytes.
+struct Scratch {
+  int64_t bytes = 0;
+  Tensor memory;
+  int64_t add(int64_t n) {
+    const int64_t at = bytes;
+    bytes += (n + 255) / 256 * 256;
+    return at;
+  }
+  void take(const Tensor& like) { memory = at::empty({bytes}, like.options().dtype(at::kByte)); }
+  template <class T>
+  T* at_byte(int64_t at) const { return reinterpret_cast<T*>(static_cast<char*>(memory.data_ptr()) + at); }
+};
 
 struct LinearCE : torch::autograd::Function<LinearCE> {
   static Tensor forward(AutogradContext* ctx, const Tensor& h, const Tensor& w, const Tensor& labels, int64_t reduction,
@@ -66,12 +79,17 @@ struct LinearCE : torch::autograd::Function<LinearCE> {
     Tensor kept = at::empty({kept_words(rows)}, h.options().dtype(at::kInt));
     Tensor loss = reduction == oab::kLceNone ? at::empty({rows}, f32) : at::empty({}, f32);
     const Tensor packed = at::empty({oab::lce_padded(rows), h.size(1)}, h.options());
-    const Tensor part = at::empty({oab::lce_part_floats(rows, w.size(0)) + rows}, f32);
-    const Tensor sums = at::empty({oab::lce_sum_doubles(rows)}, h.options().dtype(at::kDouble));
-    ok(oab::launch_lce_forward(make_args(hc, wc, labels, kept, ignore, packed), (int)reduction, part.data_ptr<float>(),
-                               part.data_ptr<float>() + part.numel() - rows, sums.data_ptr<double>(), loss.data_ptr<float>(), cur()),
+    Scratch x;
+    const int64_t part = x.add(4 * oab::lce_part_floats(rows, w.size(0))), picked = x.add(4 * rows), sums = x.add(8 * oab::lce_sum_doubles(rows));
+    x.take(h);
+    auto a = make_args(wc, labels, kept, ignore, packed);
+    a.h = hc.data_ptr();
+    a.h_stride = row_stride(hc);
+    ok(oab::launch_lce_forward(a, (int)reduction, x.at_byte<float>(part), x.at_byte<float>(picked), x.at_byte<double>(sums),
+                               loss.data_ptr<float>(), cur()),
        "linear_cross_entropy");
-    ctx->save_for_backward({h, w, labels, kept});
+    // the packed rows, not h: backward needs them in any case, so its peak is the same
+    ctx->save_for_backward({packed, w, labels, kept});
     ctx->saved_data["reduction"] = reduction;
     ctx->saved_data["ignore"] = ignore;
     ctx->saved_data["piece"] = piece;
@@ -84,34 +102,38 @@ struct LinearCE : torch::autograd::Function<LinearCE> {
     if (!g.defined() || !(want_h || want_w)) return {Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
     TORCH_CHECK(!at::GradMode::is_enabled(), "linear_cross_entropy has no second derivative (create_graph)");
     const auto saved = ctx->get_saved_variables();
-    const Tensor &h = saved[0], &w = saved[1], &labels = saved[2], kept = saved[3].contiguous();
+    const Tensor &w = saved[1], &labels = saved[2], kept = saved[3].contiguous();
     const int64_t reduction = ctx->saved_data["reduction"].toInt(), ignore = ctx->saved_data["ignore"].toInt();
-    c10::cuda::CUDAGuard guard(h.device());
+    c10::cuda::CUDAGuard guard(w.device());
     oab::raise_loss_report();
-    const Tensor hc = rows_layout(h), wc = rows_layout(w), lc = labels.contiguous(), gc = g.to(at::kFloat).contiguous();
-    const int64_t rows = h.size(0), hidden = h.size(1), vocab = w.size(0);
+    // hooks on saved tensors may have returned copies of another layout
+    const Tensor packed = rows_layout(saved[0].contiguous()), wc = rows_layout(w), lc = labels.contiguous();
+    const Tensor gc = g.to(at::kFloat).contiguous();
+    const int64_t rows = labels.size(0), hidden = w.size(1), vocab = w.size(0);
     int64_t piece = ctx->saved_data["piece"].toInt();
+    piece = std::min(piece, vocab);
     piece = piece > 0 ? (piece + oab::kLceTile - 1) / oab::kLceTile * oab::kLceTile : oab::lce_default_piece(rows, hidden, vocab);
     oab::LceGrad x;
     x.reduction = (int)reduction;
     x.g = gc.data_ptr<float>();
     x.piece = piece;
     x.splits = want_h ? oab::lce_splits(rows, hidden, vocab, piece) : 1;
-    Tensor gh, gw, acc;
+    Tensor gh, gw;
+    Scratch t;
+    const int64_t d = t.add(2 * oab::lce_padded(rows) * oab::lce_piece_pitch(vocab, piece));
+    const int64_t acc = t.add(want_h ? 4 * x.splits * oab::lce_padded(rows) * hidden : 0);
+    t.take(w);
+    x.d = t.at_byte<void>(d);
     if (want_h) {
-      gh = at::empty({rows, hidden}, h.options());
+      gh = at::empty({rows, hidden}, w.options());
       x.gh = gh.data_ptr();
-      acc = at::empty({x.splits, oab::lce_padded(rows), hidden}, h.options().dtype(at::kFloat));
-      x.acc = acc.data_ptr<float>();
+      x.acc = t.at_byte<float>(acc);
     }
     if (want_w) {
       gw = at::empty({vocab, hidden}, w.options());
       x.gw = gw.data_ptr();
     }
-    const Tensor packed = at::empty({oab::lce_padded(rows), hidden}, h.options());
-    const Tensor d = at::empty({oab::lce_padded(rows), oab::lce_piece_pitch(vocab, piece)}, h.options());
-    x.d = d.data_ptr();
-    ok(oab::launch_lce_backward(make_args(hc, wc, lc, kept, ignore, packed), x, cur()), "linear_cross_entropy backward");
+    ok(oab::launch_lce_backward(make_args(wc, lc, kept, ignore, packed), x, cur()), "linear_cross_entropy backward");
     return {gh, gw, Tensor(), Tensor(), Tensor(), Tensor()};
   }
 };

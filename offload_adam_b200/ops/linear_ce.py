@@ -120,10 +120,11 @@ def linear_cross_entropy(h, weight, labels, reduction="mean", ignore_index=-100,
     if not (h.device == weight.device == labels.device):
         raise ValueError("linear_cross_entropy: hidden states, head and labels must be on one device")
     shape = labels.shape
-    h, labels = h.reshape(-1, h.shape[-1]), labels.reshape(-1)
+    if len(shape) != 1:
+        h, labels = h.reshape(-1, h.shape[-1]), labels.reshape(-1)
     if use_kernels(h, weight) and type(labels) is torch.Tensor and h.shape[1] % 8 == 0 and h.numel() > 0:
         out = _ext.load(required=True).linear_ce(h, weight, labels.contiguous(), _REDUCTIONS[reduction], ignore_index,
                                                  piece or 0)
     else:
         out = _PlainLinearCE.apply(h, weight, labels, reduction, ignore_index, piece or _PIECE)
-    return out.view(shape) if reduction == "none" else out
+    return out.view(shape) if reduction == "none" and len(shape) != 1 else out
