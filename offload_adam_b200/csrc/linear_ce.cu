@@ -63,6 +63,8 @@ struct GemmParams {
   const float* lse;
   const float* row_g;  // by row, or null
   const int* index;
+  uint16_t* d;           // few rows
+  int64_t pitch;
   // kGrads
   const float *inv, *g;  // each may be null (1)
   int want_dh, want_dw;
@@ -109,7 +111,8 @@ struct Plan {
       alone = dh_tiles % pairs;
       first_dw = 0;
       if (alone != 0 && wt > 0) {
-        const int length = (k_steps + p.splits - 1) / p.splits + 2, one = row_steps + 2;
+        // in stages; a tile of dW takes as long as its way out, about 7 stages, at least
+        const int length = (k_steps + p.splits - 1) / p.splits, one = row_steps < 7 ? 7 : row_steps;
         const int64_t fill = (int64_t)(length / one) * (pairs - alone);
         first_dw = (int)(fill < (int64_t)wt * ht ? fill : (int64_t)wt * ht);
       }
@@ -459,6 +462,221 @@ lce_product_kernel(const __grid_constant__ GemmParams p) {
   if (warp == 1) tmem_free_pair(tmem, 512);
 }
 
+// ---------------------------------------------------------- product, few rows
+// Up to kLceFewRows rows the products read W once and little else.  A pair's tile of 256 rows would
+// spend most of its products on rows that are not there: one row of 128256 words took 166 us of
+// them at 1.9 GHz and more where the clock is lower, against 163 us of reading.  Here the words
+// (for dh: the hidden columns) are the 128 rows of a tile, one CTA's, and the packed rows its N
+// columns: lanes of tensor memory are words, columns are rows.  A stage is 18 or 24 KB, 16 of
+// them W, so that 12 or 9 stages keep more of W on its way.
+constexpr int kFewThreads = 64 + 128;
+template <int N>
+struct FewShape {
+  static constexpr int kStage = kHalfBytes + N * 128, kCount = (220 * 1024) / kStage, kSmem = kCount * kStage + 1024;
+  static constexpr int kColumns = 2 * N < 32 ? 32 : 2 * N;  // of tensor memory: two accumulators
+};
+template <int N>
+__device__ __forceinline__ void tmem_load_rows(uint32_t at, float (&v)[N]) {
+  if constexpr (N == 16) {
+    tmem_load16(at, v);
+  } else {
+#pragma unroll
+    for (int c = 0; c < N; c += 32) tmem_load32(at + c, reinterpret_cast<float(&)[32]>(v[c]));
+  }
+}
+
+template <int PASS, int N>
+__global__ void __launch_bounds__(kFewThreads, 1)
+lce_few_kernel(const __grid_constant__ GemmParams p, float* acc) {
+  using S = FewShape<N>;
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ uint64_t full[S::kCount], empty[S::kCount], done[2], drained[2];
+  __shared__ uint32_t tmem_at;
+  __shared__ int gave_up;
+  __shared__ volatile int stop;  // of the epilogue warps
+  __shared__ int label_of[N];
+  __shared__ float lse_of[N], g_of[N];
+  __shared__ float2 warp_part[4][N];
+  const uint32_t stages = (smem_addr(smem_raw) + 1023u) & ~1023u;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t full0 = smem_addr(full), empty0 = smem_addr(empty), done0 = smem_addr(done), drained0 = smem_addr(drained);
+  const int n_rows = *p.count;
+  if (threadIdx.x == 0) {
+    gave_up = 0;
+    stop = 0;
+    for (int i = 0; i < S::kCount; ++i) {
+      mbar_init(full0 + 8 * i, 1);
+      mbar_init(empty0 + 8 * i, 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(done0 + 8 * i, 1);
+      mbar_init(drained0 + 8 * i, 4);
+    }
+    mbar_init_fence();
+    prefetch_map(&p.a);
+    prefetch_map(&p.b);
+  }
+  if (PASS != kGrads && threadIdx.x < N) {
+    const int r = threadIdx.x;
+    label_of[r] = r < n_rows ? p.label[r] : -1;
+    if (PASS == kLogitGrad) {
+      lse_of[r] = r < n_rows ? p.lse[r] : 0.f;
+      g_of[r] = r < n_rows && p.row_g != nullptr ? p.row_g[p.index[r]] : 1.f;
+    }
+  }
+  if (warp == 1) tmem_alloc(smem_addr(&tmem_at), S::kColumns);
+  fence_before();
+  __syncthreads();
+  fence_after();
+  const uint32_t tmem = tmem_at;
+
+  // tiles of 128 words, or of 128 hidden columns and a share of the words
+  const int across = ((PASS == kGrads ? p.hidden : p.words) + 127) / 128, total = PASS == kGrads ? across * p.splits : across;
+  const int all_steps = ((PASS == kGrads ? p.words : p.hidden) + kInner - 1) / kInner;
+  auto share = [&](int t, int& first) {  // the inner steps of tile t
+    if (PASS != kGrads) {
+      first = 0;
+      return all_steps;
+    }
+    const int split = t / across;
+    first = (int)((int64_t)all_steps * split / p.splits);
+    return (int)((int64_t)all_steps * (split + 1) / p.splits) - first;
+  };
+  bool ok = true;
+  if (warp == 0) {
+    if (elect_one()) {
+      int it = 0;
+      for (int t = blockIdx.x; t < total && ok; t += gridDim.x) {
+        int first;
+        const int steps = share(t, first), m = t % across * 128;
+        for (int k = 0; k < steps; ++k, ++it) {
+          const int s = it % S::kCount, kk = (first + k) * kInner;
+          if (!mbar_wait(empty0 + 8 * s, ((it / S::kCount) & 1) ^ 1)) { ok = false; break; }
+          const uint32_t at = stages + s * S::kStage, bar = full0 + 8 * s;
+          mbar_expect_tx(bar, S::kStage);
+          if (PASS == kGrads) {
+            tma_load(at, &p.a, m, (int)p.word0 + kk, bar);
+            tma_load(at + kHalfBytes / 2, &p.a, m + 64, (int)p.word0 + kk, bar);
+          } else {
+            tma_load(at, &p.a, kk, (int)p.word0 + m, bar);
+          }
+          tma_load(at + kHalfBytes, &p.b, kk, 0, bar);
+        }
+      }
+      if (!ok) {  // copies that are still under way end within microseconds
+        for (int i = 0; i < 100; ++i) __nanosleep(10000);
+      }
+    }
+    __syncwarp();
+  } else if (warp == 1) {
+    if (elect_one()) {
+      constexpr uint32_t idesc = instruction(128, N, PASS == kGrads, false);
+      int it = 0, mine = 0;
+      for (int t = blockIdx.x; t < total && ok; t += gridDim.x, ++mine) {
+        int first;
+        const int steps = share(t, first);
+        const uint32_t buf = mine & 1, d = tmem + buf * N;
+        if (!mbar_wait(drained0 + 8 * buf, ((mine >> 1) & 1) ^ 1)) { ok = false; break; }
+        fence_after();
+        for (int k = 0; k < steps; ++k, ++it) {
+          const int s = it % S::kCount;
+          if (!mbar_wait(full0 + 8 * s, (it / S::kCount) & 1)) { ok = false; break; }
+          fence_after();
+          const uint32_t at = stages + s * S::kStage;
+          const uint64_t da = PASS == kGrads ? operand(at, kHalfBytes / 2, 1024) : operand(at, 16, 1024);
+          const uint64_t db = operand(at + kHalfBytes, 16, 1024);
+          constexpr uint64_t step_a = PASS == kGrads ? 2048 >> 4 : 32 >> 4;
+#pragma unroll
+          for (int q = 0; q < kInner / 16; ++q) mma(d, da + q * step_a, db + q * (32 >> 4), idesc, k > 0 || q > 0);
+          commit(empty0 + 8 * s);
+        }
+        commit(done0 + 8 * buf);
+      }
+    }
+    __syncwarp();
+  } else {
+    const int quarter = warp & 3;
+    int mine = 0;
+    for (int t = blockIdx.x; t < total; t += gridDim.x, ++mine) {
+      int first;
+      const int steps = share(t, first), m = t % across * 128;
+      const uint32_t buf = mine & 1;
+      ok = mbar_wait(done0 + 8 * buf, (mine >> 1) & 1);
+      ok = __all_sync(0xffffffffu, ok);
+      if (PASS != kStats && !ok) break;
+      fence_after();
+      float v[N];
+      tmem_load_rows<N>(tmem + buf * N + ((uint32_t)(quarter * 32) << 16), v);
+      fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(drained0 + 8 * buf);
+      const int at = m + quarter * 32 + lane;  // this lane's word of the piece, or hidden column
+      if (PASS == kStats) {
+        if (!ok) stop = 1;
+        const bool in = at < p.words;
+        float2 own = make_float2(-INFINITY, 0.f);
+#pragma unroll
+        for (int r = 0; r < N; ++r) {
+          if (r >= n_rows) break;
+          const float z = in ? v[r] : -INFINITY;
+          if (in && label_of[r] == at) p.picked[r] = z;
+          float top = z;
+#pragma unroll
+          for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+          float sum = exp_of(__fsub_rn(z, finite_shift(top)));
+#pragma unroll
+          for (int o = 16; o > 0; o >>= 1) sum = __fadd_rn(sum, __shfl_xor_sync(0xffffffffu, sum, o));
+          if (lane == (r & 31)) own = make_float2(top, sum);
+          if ((r & 31) == 31 || r == n_rows - 1) {
+            if (lane <= (r & 31)) warp_part[quarter][r - (r & 31) + lane] = own;
+          }
+        }
+        asm volatile("bar.sync 1, 128;" ::: "memory");  // the four epilogue warps; one that gave up, too, comes here
+        ok = stop == 0;
+        if (!ok) break;
+        const int r = threadIdx.x - 64;
+        if (r < n_rows) {
+          float top = -INFINITY, sum = 0.f;
+#pragma unroll
+          for (int w = 0; w < 4; ++w) top = fmaxf(top, warp_part[w][r].x);
+#pragma unroll
+          for (int w = 0; w < 4; ++w)
+            sum = __fadd_rn(sum, __fmul_rn(warp_part[w][r].y, exp_of(__fsub_rn(warp_part[w][r].x, finite_shift(top)))));
+          p.part[(int64_t)(m / 128) * p.rows + r] = make_float2(top, sum);
+        }
+        asm volatile("bar.sync 1, 128;" ::: "memory");  // before warp_part is written again
+      } else if (PASS == kLogitGrad) {
+        const int word = (int)p.word0 + at;
+        if (at < p.words) {
+#pragma unroll
+          for (int r = 0; r < N; ++r) {
+            float d = exp_of(__fsub_rn(v[r], lse_of[r]));
+            if (label_of[r] == word) d = __fsub_rn(d, 1.f);
+            // the rows that pad the inner dimension of dW are zero
+            d = r < n_rows ? __fmul_rn(d, g_of[r]) : 0.f;
+            p.d[(int64_t)r * p.pitch + at] = (uint16_t)f32_to_bf16_rne_bits(d);
+          }
+          for (int r = N; r < kLceRowPad; ++r) p.d[(int64_t)r * p.pitch + at] = 0;
+        }
+      } else if (at < p.hidden) {
+        float* to = acc + (int64_t)(t / across) * p.padded * p.hidden + at;
+#pragma unroll
+        for (int r = 0; r < N; ++r) {
+          if (r >= n_rows) break;
+          const float x = steps != 0 ? v[r] : 0.f;
+          to[(int64_t)r * p.hidden] = p.first ? x : __fadd_rn(to[(int64_t)r * p.hidden], x);
+        }
+      }
+    }
+  }
+  if (!ok) gave_up = 1;
+  fence_before();
+  __syncthreads();
+  if (gave_up && threadIdx.x == 0) *reinterpret_cast<volatile int64_t*>(p.report + 1) = 1;
+  fence_after();
+  if (warp == 1) tmem_free(tmem, S::kColumns);
+}
+
 // ------------------------------------------------------------- packing of rows
 constexpr int kScanThreads = 1024;
 
@@ -755,6 +973,23 @@ cudaError_t launch_product(const GemmParams& p, int64_t tiles, cudaStream_t st) 
   return cudaGetLastError();
 }
 
+template <int PASS, int N>
+cudaError_t launch_few_of(const GemmParams& p, float* acc, int64_t tiles, cudaStream_t st) {
+  constexpr int smem = FewShape<N>::kSmem;
+  const cudaError_t e = cudaFuncSetAttribute(lce_few_kernel<PASS, N>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (e != cudaSuccess) return e;
+  count_launch();
+  lce_few_kernel<PASS, N><<<(unsigned)(tiles < kNumSMs ? tiles : kNumSMs), kFewThreads, smem, st>>>(p, acc);
+  return cudaGetLastError();
+}
+// 16 columns keep three more stages in flight and shorten the epilogue; up to 64 rows otherwise.
+constexpr int few_columns(int64_t rows) { return rows <= 16 ? 16 : kLceFewRows; }
+template <int PASS>
+cudaError_t launch_few(const GemmParams& p, float* acc, int64_t tiles, cudaStream_t st) {
+  if (tiles > (int64_t(1) << 30)) return cudaErrorInvalidValue;
+  return few_columns(p.rows) == 16 ? launch_few_of<PASS, 16>(p, acc, tiles, st) : launch_few_of<PASS, kLceFewRows>(p, acc, tiles, st);
+}
+
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 int64_t tiles_of(int64_t n) { return (n + kTile - 1) / kTile; }
 
@@ -802,15 +1037,25 @@ cudaError_t launch_lce_forward(const LceArgs& a, int reduction, float* part, flo
   if (e != cudaSuccess || (e = make_context_current()) != cudaSuccess) return e;
   GemmParams p{};
   common_params(p, a);
-  if (!encode(&p.a, a.packed, a.hidden, p.padded, a.hidden, 128) || !encode(&p.b, a.w, a.hidden, a.vocab, a.w_stride, 128))
-    return cudaErrorInvalidValue;
   p.words = (int)a.vocab;
   p.part = reinterpret_cast<float2*>(part);
   p.picked = picked;
-  if ((e = launch_product<kStats>(p, tiles_of(a.rows) * tiles_of(a.vocab), st)) != cudaSuccess) return e;
+  int parts = (int)(2 * tiles_of(a.vocab));
+  if (a.rows <= kLceFewRows) {
+    if (!encode(&p.a, a.w, a.hidden, a.vocab, a.w_stride, 128) ||
+        !encode(&p.b, a.packed, a.hidden, p.padded, a.hidden, few_columns(a.rows)))
+      return cudaErrorInvalidValue;
+    parts = (int)((a.vocab + 127) / 128);
+    e = launch_few<kStats>(p, nullptr, parts, st);
+  } else {
+    if (!encode(&p.a, a.packed, a.hidden, p.padded, a.hidden, 128) || !encode(&p.b, a.w, a.hidden, a.vocab, a.w_stride, 128))
+      return cudaErrorInvalidValue;
+    e = launch_product<kStats>(p, tiles_of(a.rows) * tiles_of(a.vocab), st);
+  }
+  if (e != cudaSuccess) return e;
   count_launch();
   lce_join_kernel<<<(unsigned)lce_sum_doubles(a.rows), kJoinThreads, 0, st>>>(
-      p.part, (int)(2 * tiles_of(a.vocab)), a.rows, a.index, a.label, a.count, picked, a.inv, a.lse, reduction, sums, loss);
+      p.part, parts, a.rows, a.index, a.label, a.count, picked, a.inv, a.lse, reduction, sums, loss);
   return cudaGetLastError();
 }
 
@@ -821,7 +1066,21 @@ int64_t lce_default_piece(int64_t rows, int64_t hidden, int64_t vocab) {
 }
 
 int lce_splits(int64_t rows, int64_t hidden, int64_t vocab, int64_t piece) {
-  const int64_t tiles = tiles_of(rows) * tiles_of(hidden), steps = (piece < vocab ? piece : vocab) / kInner;
+  const int64_t steps = (piece < vocab ? piece : vocab) / kInner;
+  if (rows <= kLceFewRows) {
+    // the number that leaves the fewest SMs idle in the last round; each split is as much again
+    // of rows x hidden to write and read
+    const int64_t across = (hidden + 127) / 128;
+    int best = 1;
+    double most = 0.0;
+    for (int s = 1; s <= 16 && (s == 1 || s <= steps / 8); ++s) {
+      const int64_t tiles = across * s, rounds = (tiles + kNumSMs - 1) / kNumSMs;
+      const double busy = (double)tiles / (double)(rounds * kNumSMs);
+      if (busy > most + 0.02) most = busy, best = s;
+    }
+    return best;
+  }
+  const int64_t tiles = tiles_of(rows) * tiles_of(hidden);
   int64_t s = kNumSMs / 2 / tiles;
   if (s > steps / 8) s = steps / 8;
   return s < 1 ? 1 : (int)s;
@@ -845,8 +1104,16 @@ cudaError_t launch_lce_backward(const LceArgs& a, const LceGrad& g, cudaStream_t
   q.want_dh = g.gh != nullptr;
   q.want_dw = g.gw != nullptr;
   q.splits = g.splits;
-  if (!encode(&p.a, a.packed, a.hidden, p.padded, a.hidden, 128) || !encode(&p.b, a.w, a.hidden, a.vocab, a.w_stride, 128) ||
-      !encode(&q.b, a.w, a.hidden, a.vocab, a.w_stride, 64) || !encode(&q.b2, a.packed, a.hidden, p.padded, a.hidden, 64) ||
+  // few rows: `few` has the operands of dh, q those of dW alone
+  const bool is_few = a.rows <= kLceFewRows;
+  const int columns = few_columns(a.rows);
+  GemmParams few = q;
+  if (is_few) q.want_dh = 0;
+  p.d = (uint16_t*)g.d;
+  p.pitch = pitch;
+  if (!encode(is_few ? &p.b : &p.a, a.packed, a.hidden, p.padded, a.hidden, is_few ? columns : 128) ||
+      !encode(is_few ? &p.a : &p.b, a.w, a.hidden, a.vocab, a.w_stride, 128) ||
+      !encode(is_few ? &few.a : &q.b, a.w, a.hidden, a.vocab, a.w_stride, 64) || !encode(&q.b2, a.packed, a.hidden, p.padded, a.hidden, 64) ||
       (q.want_dw && !encode(&q.out, g.gw, a.hidden, a.vocab, a.hidden, 32)) ||
       (q.want_dh && !encode_acc(&q.out_acc, g.acc, a.hidden, p.padded, g.splits)))
     return cudaErrorInvalidValue;
@@ -854,10 +1121,19 @@ cudaError_t launch_lce_backward(const LceArgs& a, const LceGrad& g, cudaStream_t
     p.word0 = q.word0 = i * g.piece;
     p.words = q.words = (int)(a.vocab - p.word0 < g.piece ? a.vocab - p.word0 : g.piece);
     q.first = i == 0;
-    if (!encode(&p.out, g.d, q.words, p.padded, pitch, 32) || !encode(&q.a, g.d, q.words, p.padded, pitch, 128) ||
-        !encode(&q.a2, g.d, q.words, p.padded, pitch, 64))
-      return cudaErrorInvalidValue;
-    if ((e = launch_product<kLogitGrad>(p, tiles_of(a.rows) * tiles_of(p.words), st)) != cudaSuccess) return e;
+    if (!encode(&q.a2, g.d, q.words, p.padded, pitch, 64)) return cudaErrorInvalidValue;
+    if (is_few) {
+      few.word0 = q.word0;
+      few.words = q.words;
+      few.first = q.first;
+      if (!encode(&few.b, g.d, q.words, p.padded, pitch, columns)) return cudaErrorInvalidValue;
+      if ((e = launch_few<kLogitGrad>(p, nullptr, (p.words + 127) / 128, st)) != cudaSuccess) return e;
+      if (few.want_dh && (e = launch_few<kGrads>(few, g.acc, (a.hidden + 127) / 128 * g.splits, st)) != cudaSuccess) return e;
+    } else {
+      if (!encode(&p.out, g.d, q.words, p.padded, pitch, 32) || !encode(&q.a, g.d, q.words, p.padded, pitch, 128))
+        return cudaErrorInvalidValue;
+      if ((e = launch_product<kLogitGrad>(p, tiles_of(a.rows) * tiles_of(p.words), st)) != cudaSuccess) return e;
+    }
     const int64_t dh = q.want_dh ? tiles_of(a.rows) * tiles_of(a.hidden) * g.splits : 0;
     const int64_t dw = q.want_dw ? tiles_of(q.words) * tiles_of(a.hidden) : 0;
     if ((e = launch_product<kGrads>(q, dh + dw, st)) != cudaSuccess) return e;

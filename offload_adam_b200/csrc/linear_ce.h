@@ -6,6 +6,7 @@
 namespace oab {
 
 constexpr int kLceTile = 256;     // rows and columns of an output tile; a piece of the vocabulary is a multiple
+constexpr int kLceFewRows = 64;   // up to here the rows are the narrow side of the products
 constexpr int kLceRowPad = 64;    // the packed rows are padded with zeros to a multiple of this
 
 // Operands and workspaces of one loss.  `rows` are the rows of h; the kernels work on those whose

@@ -92,9 +92,9 @@ def _check(h, w, labels, g, reduction, **kw):
     return got
 
 
-# rows and words around a tile of one CTA (128) and of a pair (256), a padding of 64 rows, inner
-# sizes around a stage (64), pieces that end with one word
-SIZES = [(1, 8, 1), (1, 64, 257), (2, 72, 7), (63, 64, 128), (64, 128, 127), (65, 256, 129), (127, 264, 255),
+# rows and words around a tile of one CTA (128) and of a pair (256), rows around the few that run
+# the narrow products (16 and 64), inner sizes around a stage (64), pieces that end with one word
+SIZES = [(1, 8, 1), (1, 64, 257), (2, 72, 7), (16, 264, 300), (17, 72, 129), (63, 64, 128), (64, 128, 127), (64, 1032, 5000), (65, 256, 129), (127, 264, 255),
          (128, 8, 256), (129, 840, 513), (255, 64, 1000), (256, 256, 1024), (257, 520, 2049), (700, 136, 4099)]
 
 
@@ -107,6 +107,6 @@ def test_matches_64_bits(n, hidden, vocab, reduction, device):
 
 @gpu
 @pytest.mark.parametrize("piece", [1, 256, 300, 768, 4096, 1 << 20])
-@pytest.mark.parametrize("n,hidden,vocab", [(3, 64, 2561), (300, 200, 2560), (513, 96, 1025)])
+@pytest.mark.parametrize("n,hidden,vocab", [(3, 64, 2561), (40, 136, 2100), (300, 200, 2560), (513, 96, 1025)])
 def test_pieces(n, hidden, vocab, piece):
     _check(*_inputs(n, hidden, vocab, "cuda"), "mean", piece=piece)
