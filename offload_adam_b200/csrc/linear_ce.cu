@@ -178,38 +178,37 @@ struct Plan {
 // ------------------------------------------------------------------- epilogues
 // Every epilogue warp handles 32 rows (lanes) and 128 columns of the CTA's 128 x 256 tile.
 
+// They come 64 columns at a time: enough independent work for one warp to hide most of its own
+// latencies (an SM quarter has two of them).
 __device__ __forceinline__ void stats_tile(const GemmParams& p, const Tile& x, uint32_t tmem, int row, int n_rows, int half) {
   const int lab = row < n_rows ? p.label[row] : -1;
   float m = -INFINITY, s = 0.f;
 #pragma unroll 1
-  for (int c = 0; c < 4; ++c) {
-    float v[32];
-    tmem_load32(tmem + c * 32, v);
-    const int col = x.n + half * 128 + c * 32, left = p.words - col;
-    if (left < 32) {
+  for (int c = 0; c < 2; ++c) {
+    float v[64];
+    tmem_load64(tmem + c * 64, v);
+    const int col = x.n + half * 128 + c * 64, left = p.words - col;
+    if (left < 64) {
 #pragma unroll
-      for (int i = 0; i < 32; ++i)
+      for (int i = 0; i < 64; ++i)
         if (i >= left) v[i] = -INFINITY;
     }
     const int hit = lab - col;
-    if (hit >= 0 && hit < 32) {
+    if (hit >= 0 && hit < 64) {
       float z = v[0];
 #pragma unroll
-      for (int i = 1; i < 32; ++i)
+      for (int i = 1; i < 64; ++i)
         if (i == hit) z = v[i];
       p.picked[row] = z;
     }
-    float mn = m;
+    float top[4] = {m, m, m, m};
 #pragma unroll
-    for (int i = 0; i < 32; ++i) mn = fmaxf(mn, v[i]);
-    const float sh = finite_shift(mn);
-    float t0 = 0.f, t1 = 0.f;
+    for (int i = 0; i < 64; ++i) top[i & 3] = fmaxf(top[i & 3], v[i]);
+    const float mn = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])), sh = finite_shift(mn);
+    float t[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int i = 0; i < 32; i += 2) {
-      t0 = __fadd_rn(t0, exp_of(__fsub_rn(v[i], sh)));
-      t1 = __fadd_rn(t1, exp_of(__fsub_rn(v[i + 1], sh)));
-    }
-    s = __fadd_rn(__fmul_rn(s, exp_of(__fsub_rn(m, sh))), __fadd_rn(t0, t1));
+    for (int i = 0; i < 64; ++i) t[i & 3] = __fadd_rn(t[i & 3], exp_of(__fsub_rn(v[i], sh)));
+    s = __fadd_rn(__fmul_rn(s, exp_of(__fsub_rn(m, sh))), __fadd_rn(__fadd_rn(t[0], t[1]), __fadd_rn(t[2], t[3])));
     m = mn;
   }
   if (row < n_rows) p.part[(int64_t)(x.n / 128 + half) * p.rows + row] = make_float2(m, s);
@@ -227,10 +226,10 @@ __device__ __forceinline__ void stage_part(uint32_t staging, int lane, int c, ui
   st_shared16(staging + lane * 128 + ((c ^ (lane & 7)) << 4), w0, w1, w2, w3);
 }
 // 64 columns as bf16
-__device__ __forceinline__ void stage_bf16(uint32_t staging, int lane, int half32, const float (&v)[32]) {
+__device__ __forceinline__ void stage_bf16(uint32_t staging, int lane, const float (&v)[64]) {
 #pragma unroll
-  for (int c = 0; c < 4; ++c)
-    stage_part(staging, lane, half32 * 4 + c, f32x2_to_bf16x2_rne(v[8 * c], v[8 * c + 1]), f32x2_to_bf16x2_rne(v[8 * c + 2], v[8 * c + 3]),
+  for (int c = 0; c < 8; ++c)
+    stage_part(staging, lane, c, f32x2_to_bf16x2_rne(v[8 * c], v[8 * c + 1]), f32x2_to_bf16x2_rne(v[8 * c + 2], v[8 * c + 3]),
                f32x2_to_bf16x2_rne(v[8 * c + 4], v[8 * c + 5]), f32x2_to_bf16x2_rne(v[8 * c + 6], v[8 * c + 7]));
 }
 
@@ -238,33 +237,33 @@ __device__ __forceinline__ void logit_grad_tile(const GemmParams& p, const Tile&
                                                 uint32_t staging, int lane) {
   const bool in = row < n_rows;
   const int lab = in && p.label[row] >= 0 ? (int)(p.label[row] - p.word0) : -1;
-  const float lse = in ? p.lse[row] : 0.f;
-  const float g = !in ? 0.f : p.row_g != nullptr ? p.row_g[p.index[row]] : 1.f;
+  // the rows that pad the inner dimension of dW (their logits are 0) become zero
+  const float lse = in ? p.lse[row] : INFINITY;
+  const float g = in && p.row_g != nullptr ? p.row_g[p.index[row]] : 1.f;
 #pragma unroll 1
-  for (int c = 0; c < 4; ++c) {
-    float v[32];
-    tmem_load32(tmem + c * 32, v);
-    const int col = x.n + half * 128 + c * 32;
+  for (int c = 0; c < 2; ++c) {
+    float v[64];
+    tmem_load64(tmem + c * 64, v);
+    const int col = x.n + half * 128 + c * 64;
 #pragma unroll
-    for (int i = 0; i < 32; ++i) v[i] = exp_of(__fsub_rn(v[i], lse));
+    for (int i = 0; i < 64; ++i) v[i] = exp_of(__fsub_rn(v[i], lse));
     const int hit = lab - col;
-    if (lab >= 0 && hit >= 0 && hit < 32) {
+    if (lab >= 0 && hit >= 0 && hit < 64) {
 #pragma unroll
-      for (int i = 0; i < 32; ++i)
+      for (int i = 0; i < 64; ++i)
         if (i == hit) v[i] = __fsub_rn(v[i], 1.f);
     }
-    // rows that pad the inner dimension of dW are zero, whatever stands in them
+    if (p.row_g != nullptr) {
 #pragma unroll
-    for (int i = 0; i < 32; ++i) v[i] = in ? __fmul_rn(v[i], g) : 0.f;
-    if ((c & 1) == 0) stage_begin(lane);
-    stage_bf16(staging, lane, c & 1, v);
-    if ((c & 1) == 1) {
-      store_fence();
-      __syncwarp();
-      if (lane == 0) {
-        if (col - 32 < p.words && row < p.padded) tma_store(&p.out, staging, col - 32, row);
-        store_commit();
-      }
+      for (int i = 0; i < 64; ++i) v[i] = __fmul_rn(v[i], g);
+    }
+    stage_begin(lane);
+    stage_bf16(staging, lane, v);
+    store_fence();
+    __syncwarp();
+    if (lane == 0) {
+      if (col < p.words && row < p.padded) tma_store(&p.out, staging, col, row);
+      store_commit();
     }
   }
 }
@@ -297,22 +296,20 @@ __device__ __forceinline__ void dh_tile(const GemmParams& p, const Tile& x, uint
 __device__ __forceinline__ void dw_tile(const GemmParams& p, const Tile& x, uint32_t tmem, int row, int half, float scale,
                                         uint32_t staging, int lane) {
 #pragma unroll 1
-  for (int c = 0; c < 4; ++c) {
-    float v[32];
-    tmem_load32(tmem + c * 32, v);
-    const int col = x.n + half * 128 + c * 32;
+  for (int c = 0; c < 2; ++c) {
+    float v[64];
+    tmem_load64(tmem + c * 64, v);
+    const int col = x.n + half * 128 + c * 64;
     // no row that counts: nothing was summed
 #pragma unroll
-    for (int i = 0; i < 32; ++i) v[i] = x.steps != 0 ? __fmul_rn(v[i], scale) : 0.f;
-    if ((c & 1) == 0) stage_begin(lane);
-    stage_bf16(staging, lane, c & 1, v);
-    if ((c & 1) == 1) {
-      store_fence();
-      __syncwarp();
-      if (lane == 0) {
-        if (col - 32 < p.hidden && row < p.words) tma_store(&p.out, staging, col - 32, (int)p.word0 + row);
-        store_commit();
-      }
+    for (int i = 0; i < 64; ++i) v[i] = x.steps != 0 ? __fmul_rn(v[i], scale) : 0.f;
+    stage_begin(lane);
+    stage_bf16(staging, lane, v);
+    store_fence();
+    __syncwarp();
+    if (lane == 0) {
+      if (col < p.hidden && row < p.words) tma_store(&p.out, staging, col, (int)p.word0 + row);
+      store_commit();
     }
   }
 }
