@@ -34,8 +34,8 @@ constexpr int kInner = 64;                              // inner values of a sta
 constexpr int kStages = 6;
 constexpr int kHalfBytes = 128 * kInner * 2;            // one CTA's part of an operand's stage
 constexpr int kStageBytes = 2 * kHalfBytes;
-constexpr int kEpilogueWarps = 8;
-constexpr int kStagingBytes = 32 * 128;  // of an epilogue warp: 32 lines of 128 bytes on their way out
+constexpr int kEpilogueWarps = 16;       // eight for each accumulator
+constexpr int kStagingBytes = 32 * 64;   // of an epilogue warp: 32 lines of 64 bytes on their way out
 constexpr int kSmemBytes = kStages * kStageBytes + kEpilogueWarps * kStagingBytes + 1024;  // starts on 1024 bytes
 constexpr int kGemmThreads = 64 + 32 * kEpilogueWarps;
 constexpr int kGroup = 16;  // row tiles that share a column tile in turn: 4096 rows of h stay in L2
@@ -176,10 +176,12 @@ struct Plan {
 };
 
 // ------------------------------------------------------------------- epilogues
-// Every epilogue warp handles 32 rows (lanes) and 128 columns of the CTA's 128 x 256 tile.
+// Every epilogue warp handles 32 rows (lanes) and 128 columns of the CTA's 128 x 256 tile, and every
+// other tile of its pair.  Reading a tile out of tensor memory takes 1.1 us, as long as what
+// follows: with eight warps for all tiles the two came one after the other (2.3 us a tile, whatever
+// the product's length), with eight for each accumulator one half reads while the other computes
+// and stores.
 
-// They come 64 columns at a time: enough independent work for one warp to hide most of its own
-// latencies (an SM quarter has two of them).
 __device__ __forceinline__ void stats_tile(const GemmParams& p, const Tile& x, uint32_t tmem, int row, int n_rows, int half) {
   const int lab = row < n_rows ? p.label[row] : -1;
   float m = -INFINITY, s = 0.f;
@@ -214,23 +216,25 @@ __device__ __forceinline__ void stats_tile(const GemmParams& p, const Tile& x, u
   if (row < n_rows) p.part[(int64_t)(x.n / 128 + half) * p.rows + row] = make_float2(m, s);
 }
 
-// A warp's 32 lines of 128 bytes leave through its staging buffer, 16-byte parts swizzled as TMA
-// expects them (part c of line r at c ^ (r % 8), which also keeps the stores free of bank
-// conflicts).  A store a thread, straight from its row, touched 32 lines an instruction: a tile of
-// dW took longer to write than 10 stages to compute.
+// A warp's 32 lines of 64 bytes leave through its staging buffer, 16-byte parts swizzled as TMA
+// expects them (part c of line r at c ^ (r / 2 % 4), which also keeps the stores free of bank
+// conflicts).  A store a thread, straight from its row, touched 32 lines an instruction.
 __device__ __forceinline__ void stage_begin(int lane) {
   if (lane == 0) store_wait_read();
   __syncwarp();
 }
 __device__ __forceinline__ void stage_part(uint32_t staging, int lane, int c, uint32_t w0, uint32_t w1, uint32_t w2, uint32_t w3) {
-  st_shared16(staging + lane * 128 + ((c ^ (lane & 7)) << 4), w0, w1, w2, w3);
+  st_shared16(staging + lane * 64 + ((c ^ ((lane >> 1) & 3)) << 4), w0, w1, w2, w3);
 }
-// 64 columns as bf16
-__device__ __forceinline__ void stage_bf16(uint32_t staging, int lane, const float (&v)[64]) {
+// 32 columns as bf16
+__device__ __forceinline__ void stage_bf16(uint32_t staging, int lane, const float (&v)[32]) {
+  stage_begin(lane);
 #pragma unroll
-  for (int c = 0; c < 8; ++c)
+  for (int c = 0; c < 4; ++c)
     stage_part(staging, lane, c, f32x2_to_bf16x2_rne(v[8 * c], v[8 * c + 1]), f32x2_to_bf16x2_rne(v[8 * c + 2], v[8 * c + 3]),
                f32x2_to_bf16x2_rne(v[8 * c + 4], v[8 * c + 5]), f32x2_to_bf16x2_rne(v[8 * c + 6], v[8 * c + 7]));
+  store_fence();
+  __syncwarp();
 }
 
 __device__ __forceinline__ void logit_grad_tile(const GemmParams& p, const Tile& x, uint32_t tmem, int row, int n_rows, int half,
@@ -241,26 +245,23 @@ __device__ __forceinline__ void logit_grad_tile(const GemmParams& p, const Tile&
   const float lse = in ? p.lse[row] : INFINITY;
   const float g = in && p.row_g != nullptr ? p.row_g[p.index[row]] : 1.f;
 #pragma unroll 1
-  for (int c = 0; c < 2; ++c) {
-    float v[64];
-    tmem_load64(tmem + c * 64, v);
-    const int col = x.n + half * 128 + c * 64;
+  for (int c = 0; c < 4; ++c) {
+    float v[32];
+    tmem_load32(tmem + c * 32, v);
+    const int col = x.n + half * 128 + c * 32;
 #pragma unroll
-    for (int i = 0; i < 64; ++i) v[i] = exp_of(__fsub_rn(v[i], lse));
+    for (int i = 0; i < 32; ++i) v[i] = exp_of(__fsub_rn(v[i], lse));
     const int hit = lab - col;
-    if (lab >= 0 && hit >= 0 && hit < 64) {
+    if (lab >= 0 && hit >= 0 && hit < 32) {
 #pragma unroll
-      for (int i = 0; i < 64; ++i)
+      for (int i = 0; i < 32; ++i)
         if (i == hit) v[i] = __fsub_rn(v[i], 1.f);
     }
     if (p.row_g != nullptr) {
 #pragma unroll
-      for (int i = 0; i < 64; ++i) v[i] = __fmul_rn(v[i], g);
+      for (int i = 0; i < 32; ++i) v[i] = __fmul_rn(v[i], g);
     }
-    stage_begin(lane);
     stage_bf16(staging, lane, v);
-    store_fence();
-    __syncwarp();
     if (lane == 0) {
       if (col < p.words && row < p.padded) tma_store(&p.out, staging, col, row);
       store_commit();
@@ -271,17 +272,17 @@ __device__ __forceinline__ void logit_grad_tile(const GemmParams& p, const Tile&
 __device__ __forceinline__ void dh_tile(const GemmParams& p, const Tile& x, uint32_t tmem, int row, int n_rows, int half,
                                         uint32_t staging, int lane) {
 #pragma unroll 1
-  for (int c = 0; c < 4; ++c) {
-    float v[32];
-    tmem_load32(tmem + c * 32, v);
-    const int col = x.n + half * 128 + c * 32;
+  for (int c = 0; c < 8; ++c) {
+    float v[16];
+    tmem_load16(tmem + c * 16, v);
+    const int col = x.n + half * 128 + c * 16;
     if (x.steps == 0) {  // a last piece of fewer stages than splits: nothing was summed
 #pragma unroll
-      for (int i = 0; i < 32; ++i) v[i] = 0.f;
+      for (int i = 0; i < 16; ++i) v[i] = 0.f;
     }
     stage_begin(lane);
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
+    for (int i = 0; i < 4; ++i)
       stage_part(staging, lane, i, __float_as_uint(v[4 * i]), __float_as_uint(v[4 * i + 1]), __float_as_uint(v[4 * i + 2]),
                  __float_as_uint(v[4 * i + 3]));
     store_fence();
@@ -296,17 +297,14 @@ __device__ __forceinline__ void dh_tile(const GemmParams& p, const Tile& x, uint
 __device__ __forceinline__ void dw_tile(const GemmParams& p, const Tile& x, uint32_t tmem, int row, int half, float scale,
                                         uint32_t staging, int lane) {
 #pragma unroll 1
-  for (int c = 0; c < 2; ++c) {
-    float v[64];
-    tmem_load64(tmem + c * 64, v);
-    const int col = x.n + half * 128 + c * 64;
+  for (int c = 0; c < 4; ++c) {
+    float v[32];
+    tmem_load32(tmem + c * 32, v);
+    const int col = x.n + half * 128 + c * 32;
     // no row that counts: nothing was summed
 #pragma unroll
-    for (int i = 0; i < 64; ++i) v[i] = x.steps != 0 ? __fmul_rn(v[i], scale) : 0.f;
-    stage_begin(lane);
+    for (int i = 0; i < 32; ++i) v[i] = x.steps != 0 ? __fmul_rn(v[i], scale) : 0.f;
     stage_bf16(staging, lane, v);
-    store_fence();
-    __syncwarp();
     if (lane == 0) {
       if (col < p.hidden && row < p.words) tma_store(&p.out, staging, col, (int)p.word0 + row);
       store_commit();
@@ -335,7 +333,7 @@ lce_product_kernel(const __grid_constant__ GemmParams p) {
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(done0 + 8 * i, 1);
-      mbar_init(drained0 + 8 * i, 2 * kEpilogueWarps);
+      mbar_init(drained0 + 8 * i, kEpilogueWarps);  // eight warps of both CTAs
     }
     mbar_init_fence();
     prefetch_map(&p.a);
@@ -422,7 +420,7 @@ lce_product_kernel(const __grid_constant__ GemmParams p) {
     }
     __syncwarp();
   } else {
-    const int quarter = warp & 3, half = (warp - 2) >> 2;
+    const int quarter = warp & 3, half = ((warp - 2) >> 2) & 1, group = (warp - 2) >> 3;
     const uint32_t lead_drained0 = map_to_rank(drained0, 0);
     float scale = 1.f;
     if (PASS == kGrads) {
@@ -430,9 +428,9 @@ lce_product_kernel(const __grid_constant__ GemmParams p) {
       if (p.g != nullptr) scale = __fmul_rn(scale, *p.g);
     }
     const uint32_t staging = stages + kStages * kStageBytes + (warp - 2) * kStagingBytes;
-    for (int mine = 0, t; (t = plan.pick<PASS>(pair, mine)) >= 0; ++mine) {
+    for (int mine = group, t; (t = plan.pick<PASS>(pair, mine)) >= 0; mine += 2) {
       const Tile x = plan.at<PASS>(p, t);
-      const uint32_t acc = mine & 1;
+      const uint32_t acc = group;
       ok = mbar_wait(done0 + 8 * acc, (mine >> 1) & 1);
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
@@ -936,25 +934,25 @@ cudaError_t make_context_current() {
   return e != cudaSuccess ? e : cudaSetDevice(device);
 }
 
-// The fp32 sums of dh as (hidden, rows, splits) in boxes of 32 columns and 32 rows.
+// The fp32 sums of dh as (hidden, rows, splits) in boxes of 16 columns and 32 rows.
 bool encode_acc(CUtensorMap* map, float* base, int64_t hidden, int64_t padded, int splits) {
   const auto fn = encoder();
   if (fn == nullptr) return false;
   const cuuint64_t dims[3] = {(cuuint64_t)hidden, (cuuint64_t)padded, (cuuint64_t)splits};
   const cuuint64_t strides[2] = {(cuuint64_t)hidden * 4, (cuuint64_t)hidden * 4 * (cuuint64_t)padded};
-  const cuuint32_t box[3] = {32, 32, 1}, steps[3] = {1, 1, 1};
+  const cuuint32_t box[3] = {16, 32, 1}, steps[3] = {1, 1, 1};
   return fn(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 3, base, dims, strides, box, steps, CU_TENSOR_MAP_INTERLEAVE_NONE,
-            CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+            CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
-// Boxes of 64 contiguous values and `lines` lines of a bf16 matrix; what lies outside reads as zero
-// and is not written.
-bool encode(CUtensorMap* map, const void* base, int64_t inner, int64_t lines_all, int64_t stride, int lines) {
+// Boxes of `width` (64 to read, 32 to write) contiguous values and `lines` lines of a bf16 matrix;
+// what lies outside reads as zero and is not written.
+bool encode(CUtensorMap* map, const void* base, int64_t inner, int64_t lines_all, int64_t stride, int lines, int width = 64) {
   const auto fn = encoder();
   if (fn == nullptr) return false;
   const cuuint64_t dims[2] = {(cuuint64_t)inner, (cuuint64_t)lines_all}, strides[1] = {(cuuint64_t)stride * 2};
-  const cuuint32_t box[2] = {64, (cuuint32_t)lines}, steps[2] = {1, 1};
+  const cuuint32_t box[2] = {(cuuint32_t)width, (cuuint32_t)lines}, steps[2] = {1, 1};
   return fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(base), dims, strides, box, steps,
-            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+            CU_TENSOR_MAP_INTERLEAVE_NONE, width == 64 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
@@ -1111,7 +1109,7 @@ cudaError_t launch_lce_backward(const LceArgs& a, const LceGrad& g, cudaStream_t
   if (!encode(is_few ? &p.b : &p.a, a.packed, a.hidden, p.padded, a.hidden, is_few ? columns : 128) ||
       !encode(is_few ? &p.a : &p.b, a.w, a.hidden, a.vocab, a.w_stride, 128) ||
       !encode(is_few ? &few.a : &q.b, a.w, a.hidden, a.vocab, a.w_stride, 64) || !encode(&q.b2, a.packed, a.hidden, p.padded, a.hidden, 64) ||
-      (q.want_dw && !encode(&q.out, g.gw, a.hidden, a.vocab, a.hidden, 32)) ||
+      (q.want_dw && !encode(&q.out, g.gw, a.hidden, a.vocab, a.hidden, 32, 32)) ||
       (q.want_dh && !encode_acc(&q.out_acc, g.acc, a.hidden, p.padded, g.splits)))
     return cudaErrorInvalidValue;
   for (int64_t i = 0; i < pieces; ++i) {
@@ -1127,7 +1125,7 @@ cudaError_t launch_lce_backward(const LceArgs& a, const LceGrad& g, cudaStream_t
       if ((e = launch_few<kLogitGrad>(p, nullptr, (p.words + 127) / 128, st)) != cudaSuccess) return e;
       if (few.want_dh && (e = launch_few<kGrads>(few, g.acc, (a.hidden + 127) / 128 * g.splits, st)) != cudaSuccess) return e;
     } else {
-      if (!encode(&p.out, g.d, q.words, p.padded, pitch, 32) || !encode(&q.a, g.d, q.words, p.padded, pitch, 128))
+      if (!encode(&p.out, g.d, q.words, p.padded, pitch, 32, 32) || !encode(&q.a, g.d, q.words, p.padded, pitch, 128))
         return cudaErrorInvalidValue;
       if ((e = launch_product<kLogitGrad>(p, tiles_of(a.rows) * tiles_of(p.words), st)) != cudaSuccess) return e;
     }
