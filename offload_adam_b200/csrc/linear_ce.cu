@@ -177,18 +177,37 @@ struct Plan {
 
 // ------------------------------------------------------------------- epilogues
 // Every epilogue warp handles 32 rows (lanes) and 128 columns of the CTA's 128 x 256 tile, and every
-// other tile of its pair.  Reading a tile out of tensor memory takes 1.1 us, as long as what
-// follows: with eight warps for all tiles the two came one after the other (2.3 us a tile, whatever
-// the product's length), with eight for each accumulator one half reads while the other computes
-// and stores.
+// other tile of its pair.  A warp is a chain of latencies (the accumulator is done, its load, a
+// fence, the way out), so there are eight for each accumulator, and the accumulator is given
+// back (`release`) with the last load from it, before anything is computed from that.
 
-__device__ __forceinline__ void stats_tile(const GemmParams& p, const Tile& x, uint32_t tmem, int row, int n_rows, int half) {
-  const int lab = row < n_rows ? p.label[row] : -1;
+struct RowValues {  // of the packed row that a thread has in a tile
+  int label;
+  float lse, g;
+};
+template <int PASS>
+__device__ __forceinline__ RowValues row_values(const GemmParams& p, int row, int n_rows) {
+  RowValues r{-1, INFINITY, 1.f};
+  if (PASS != kGrads && row < n_rows) {
+    r.label = p.label[row];
+    if (PASS == kLogitGrad) {
+      r.lse = p.lse[row];
+      if (p.row_g != nullptr) r.g = p.row_g[p.index[row]];
+    }
+  }
+  return r;
+}
+
+template <class Release>
+__device__ __forceinline__ void stats_tile(const GemmParams& p, const Tile& x, uint32_t tmem, int row, int n_rows, int half,
+                                           const RowValues& values, const Release& release) {
+  const int lab = values.label;
   float m = -INFINITY, s = 0.f;
 #pragma unroll 1
   for (int c = 0; c < 2; ++c) {
     float v[64];
     tmem_load64(tmem + c * 64, v);
+    if (c == 1) release();
     const int col = x.n + half * 128 + c * 64, left = p.words - col;
     if (left < 64) {
 #pragma unroll
@@ -237,17 +256,17 @@ __device__ __forceinline__ void stage_bf16(uint32_t staging, int lane, const flo
   __syncwarp();
 }
 
-__device__ __forceinline__ void logit_grad_tile(const GemmParams& p, const Tile& x, uint32_t tmem, int row, int n_rows, int half,
-                                                uint32_t staging, int lane) {
-  const bool in = row < n_rows;
-  const int lab = in && p.label[row] >= 0 ? (int)(p.label[row] - p.word0) : -1;
-  // the rows that pad the inner dimension of dW (their logits are 0) become zero
-  const float lse = in ? p.lse[row] : INFINITY;
-  const float g = in && p.row_g != nullptr ? p.row_g[p.index[row]] : 1.f;
+template <class Release>
+__device__ __forceinline__ void logit_grad_tile(const GemmParams& p, const Tile& x, uint32_t tmem, int row, int half, uint32_t staging,
+                                                int lane, const RowValues& values, const Release& release) {
+  const int lab = values.label >= 0 ? (int)(values.label - p.word0) : -1;
+  // the rows that pad the inner dimension of dW become zero: their logits are 0, their lse infinite
+  const float lse = values.lse, g = values.g;
 #pragma unroll 1
   for (int c = 0; c < 4; ++c) {
     float v[32];
     tmem_load32(tmem + c * 32, v);
+    if (c == 3) release();
     const int col = x.n + half * 128 + c * 32;
 #pragma unroll
     for (int i = 0; i < 32; ++i) v[i] = exp_of(__fsub_rn(v[i], lse));
@@ -269,12 +288,14 @@ __device__ __forceinline__ void logit_grad_tile(const GemmParams& p, const Tile&
   }
 }
 
+template <class Release>
 __device__ __forceinline__ void dh_tile(const GemmParams& p, const Tile& x, uint32_t tmem, int row, int n_rows, int half,
-                                        uint32_t staging, int lane) {
+                                        uint32_t staging, int lane, const Release& release) {
 #pragma unroll 1
   for (int c = 0; c < 8; ++c) {
     float v[16];
     tmem_load16(tmem + c * 16, v);
+    if (c == 7) release();
     const int col = x.n + half * 128 + c * 16;
     if (x.steps == 0) {  // a last piece of fewer stages than splits: nothing was summed
 #pragma unroll
@@ -294,12 +315,14 @@ __device__ __forceinline__ void dh_tile(const GemmParams& p, const Tile& x, uint
   }
 }
 
+template <class Release>
 __device__ __forceinline__ void dw_tile(const GemmParams& p, const Tile& x, uint32_t tmem, int row, int half, float scale,
-                                        uint32_t staging, int lane) {
+                                        uint32_t staging, int lane, const Release& release) {
 #pragma unroll 1
   for (int c = 0; c < 4; ++c) {
     float v[32];
     tmem_load32(tmem + c * 32, v);
+    if (c == 3) release();
     const int col = x.n + half * 128 + c * 32;
     // no row that counts: nothing was summed
 #pragma unroll
@@ -431,19 +454,22 @@ lce_product_kernel(const __grid_constant__ GemmParams p) {
     for (int mine = group, t; (t = plan.pick<PASS>(pair, mine)) >= 0; mine += 2) {
       const Tile x = plan.at<PASS>(p, t);
       const uint32_t acc = group;
+      const int row = x.m + (int)rank * 128 + quarter * 32 + lane;
+      const RowValues values = row_values<PASS>(p, row, n_rows);  // on their way while the products run
       ok = mbar_wait(done0 + 8 * acc, (mine >> 1) & 1);
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
       fence_after();
       const uint32_t at = tmem + acc * kTile + half * 128 + ((uint32_t)(quarter * 32) << 16);
-      const int row = x.m + (int)rank * 128 + quarter * 32 + lane;
-      if (PASS == kStats) stats_tile(p, x, at, row, n_rows, half);
-      if (PASS == kLogitGrad) logit_grad_tile(p, x, at, row, n_rows, half, staging, lane);
-      if (PASS == kGrads && x.kind == 0) dh_tile(p, x, at, row, n_rows, half, staging, lane);
-      if (PASS == kGrads && x.kind == 1) dw_tile(p, x, at, row, half, scale, staging, lane);
-      fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive_cluster(lead_drained0 + 8 * acc);
+      const auto release = [&] {
+        fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive_cluster(lead_drained0 + 8 * acc);
+      };
+      if (PASS == kStats) stats_tile(p, x, at, row, n_rows, half, values, release);
+      if (PASS == kLogitGrad) logit_grad_tile(p, x, at, row, half, staging, lane, values, release);
+      if (PASS == kGrads && x.kind == 0) dh_tile(p, x, at, row, n_rows, half, staging, lane, release);
+      if (PASS == kGrads && x.kind == 1) dw_tile(p, x, at, row, half, scale, staging, lane, release);
     }
     if (PASS != kStats && lane == 0) store_wait();
     __syncwarp();
