@@ -68,6 +68,7 @@ struct GemmParams {
   // kGrads
   const float *inv, *g;  // each may be null (1)
   int want_dh, want_dw;
+  int narrow;            // at most 128 hidden columns: products of 128 columns
   int splits;
   int first;             // piece: its dh starts the sums
 };
@@ -384,13 +385,13 @@ lce_product_kernel(const __grid_constant__ GemmParams p) {
         const bool outer_a = PASS == kGrads && x.kind == 1, outer_b = PASS == kGrads;
         const CUtensorMap* ma = outer_a ? &p.a2 : &p.a;
         const CUtensorMap* mb = outer_a ? &p.b2 : &p.b;
-        const int am = x.m + rank * 128, bn = x.n + rank * 128;
+        const int am = x.m + rank * 128, bn = x.n + rank * (PASS == kGrads && p.narrow ? 64 : 128);
         // kLogitGrad: W's rows start at the piece; dh: so do the inner values of W
         const int b_row0 = PASS == kLogitGrad ? (int)p.word0 : 0, b_k0 = PASS == kGrads && x.kind == 0 ? (int)p.word0 : 0;
         for (int k = 0; k < x.steps; ++k, ++it) {
           const int s = it % kStages;
           if (!mbar_wait(empty0 + 8 * s, ((it / kStages) & 1) ^ 1)) { ok = false; break; }
-          if (rank == 0) mbar_expect_tx(full0 + 8 * s, 2 * kStageBytes);
+          if (rank == 0) mbar_expect_tx(full0 + 8 * s, PASS == kGrads && p.narrow ? 2 * kStageBytes - kHalfBytes : 2 * kStageBytes);
           const uint32_t at = stages + s * kStageBytes, bt = at + kHalfBytes, bar = lead_full0 + 8 * s;
           const int kk = x.k0 + k * kInner;
           if (outer_a) {
@@ -401,7 +402,7 @@ lce_product_kernel(const __grid_constant__ GemmParams p) {
           }
           if (outer_b) {
             tma_load_pair(bt, mb, bn, b_k0 + kk, bar);
-            tma_load_pair(bt + kHalfBytes / 2, mb, bn + 64, b_k0 + kk, bar);
+            if (!p.narrow) tma_load_pair(bt + kHalfBytes / 2, mb, bn + 64, b_k0 + kk, bar);
           } else {
             tma_load_pair(bt, mb, kk, b_row0 + bn, bar);
           }
@@ -421,7 +422,7 @@ lce_product_kernel(const __grid_constant__ GemmParams p) {
         const Tile x = plan.at<PASS>(p, t);
         const bool outer_a = PASS == kGrads && x.kind == 1;
         constexpr bool outer_b = PASS == kGrads;
-        const uint32_t idesc = instruction(kTile, kTile, outer_a, outer_b);
+        const uint32_t idesc = instruction(kTile, PASS == kGrads && p.narrow ? kTile / 2 : kTile, outer_a, outer_b);
         const uint32_t acc = mine & 1, d = tmem + acc * kTile;
         if (!mbar_wait(drained0 + 8 * acc, ((mine >> 1) & 1) ^ 1)) { ok = false; break; }
         fence_after();
@@ -1124,6 +1125,8 @@ cudaError_t launch_lce_backward(const LceArgs& a, const LceGrad& g, cudaStream_t
   q.g = g.reduction == kLceNone ? nullptr : g.g;
   q.want_dh = g.gh != nullptr;
   q.want_dw = g.gw != nullptr;
+  // Half of a tile would be products with zeros (2000 rows of 64, 5000 words: 19.6 us, so 18.0).
+  q.narrow = a.hidden <= kTile / 2;
   q.splits = g.splits;
   // few rows: `few` has the operands of dh, q those of dW alone
   const bool is_few = a.rows <= kLceFewRows;
