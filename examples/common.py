@@ -32,6 +32,9 @@ def add_common_args(p):
     p.add_argument("--liger-fused-linear-ce", action="store_true",
                    help="accepted so that the reference trainers' command lines keep working; the chunked linear "
                         "cross-entropy is the default here and needs no extra package")
+    p.add_argument("--ce-piece", type=int, default=None, metavar="WORDS",
+                   help="cross-entropy in pieces of that many words of the vocabulary (0: the package chooses), "
+                        "which keeps no logits; default: chunks of rows")
     p.add_argument("--layers", type=int, default=None, help="override the number of layers")
     p.add_argument("--mode", choices=MODES, default="fp32_master")
     p.add_argument("--tokens-per-sample", type=int, default=2048)
@@ -68,6 +71,8 @@ def validate(args):
     for name in ("tokens_per_sample", "grad_accum_steps", "steps"):
         if getattr(args, name) < 1:
             raise ValueError(f"--{name.replace('_', '-')} must be >= 1")
+    if args.ce_piece is not None and args.ce_piece < 0:
+        raise ValueError("--ce-piece must be >= 0")
     if not 0 <= args.warmup_steps < args.steps:
         raise ValueError("--warmup-steps must be in [0, --steps)")
 
@@ -76,18 +81,19 @@ class _HFCausalLM(torch.nn.Module):
     """Gives a HuggingFace causal LM the call signature the example loop uses
     (``model(ids, labels=ids)`` returns the loss) and keeps ``.config`` reachable.  The
     head and the loss run chunk by chunk (``offload_adam_b200.models.hf.causal_lm_loss``)
-    unless ``full_logits`` asks for the module's own loss."""
+    unless ``full_logits`` asks for the module's own loss; ``ce_piece``: its ``piece``."""
 
-    def __init__(self, hf, full_logits=False):
+    def __init__(self, hf, full_logits=False, ce_piece=None):
         super().__init__()
         self.hf = hf
         self.config = hf.config
         self.full_logits = full_logits
+        self.ce_piece = ce_piece
 
     def forward(self, ids, labels=None):
         if self.full_logits or labels is None:
             return self.hf(input_ids=ids, labels=labels).loss
-        return causal_lm_loss(self.hf, ids, labels)
+        return causal_lm_loss(self.hf, ids, labels, piece=self.ce_piece)
 
     def gradient_checkpointing_enable(self):
         self.hf.gradient_checkpointing_enable()
@@ -121,7 +127,8 @@ def build_hf_model(args, device):
     else:
         hf = AutoModelForCausalLM.from_pretrained(src, dtype=torch.bfloat16, attn_implementation="sdpa")
         hf.config.use_cache = False
-    model = _HFCausalLM(hf.to(torch.bfloat16).to(device), full_logits=getattr(args, "full_logits", False))
+    model = _HFCausalLM(hf.to(torch.bfloat16).to(device), full_logits=getattr(args, "full_logits", False),
+                        ce_piece=getattr(args, "ce_piece", None))
     model.train()
     if args.gradient_checkpointing:
         model.gradient_checkpointing_enable()
@@ -131,7 +138,7 @@ def build_hf_model(args, device):
 def build_model(args, device):
     if getattr(args, "hf_model", None):
         return build_hf_model(args, device)
-    cfg = MODELS[args.model_name]()
+    cfg = MODELS[args.model_name](ce_piece=getattr(args, "ce_piece", None))
     if args.layers is not None:
         cfg.num_layers = args.layers
     model = build_llama(cfg, device=device, dtype=torch.bfloat16, seed=args.seed)

@@ -39,7 +39,7 @@ def main():
                           transfer=args.transfer, grad_residency=args.grad_residency,
                           staging_bytes=common.staging_arg(args), **hp)
     else:
-        opt = Adam(model.parameters(), **hp)
+        opt = Adam(model.parameters(), max_grad_norm=args.max_grad_norm, **hp)
     print(f"model={args.model_name} device={torch.cuda.get_device_name(0)} "
           f"enable_offloading={args.enable_offloading} mode={args.mode}", flush=True)
     summary = common.train(args, model, opt, args.batch_size, device)

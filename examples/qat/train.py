@@ -67,7 +67,7 @@ def main():
                           transfer=args.transfer, grad_residency=args.grad_residency,
                           staging_bytes=common.staging_arg(args), **hp)
     else:
-        opt = Adam(model.parameters(), **hp)
+        opt = Adam(model.parameters(), max_grad_norm=args.max_grad_norm, **hp)
     hf = getattr(model, "hf", None)  # the HuggingFace module when --hf-model is given
     master_from = args.load_master_from
     if master_from is None and hf is not None and common.has_weights(args.hf_model):

@@ -732,7 +732,7 @@ lce_scan_kernel(const int64_t* __restrict__ labels, int64_t rows, int64_t vocab,
     if (in) {
       const int k = base + warps[warp] + __popc(mask & ((1u << lane) - 1u));
       const bool known = lab >= 0 && lab < vocab;
-      if (!known) *bad = lab;
+      if (!known) bad[lab < 0 ? 2 : 0] = lab;
       index[k] = (int)r;
       label[k] = known ? (int)lab : -1;
     } else if (row_loss != nullptr && r < rows) {
@@ -807,7 +807,7 @@ lce_scan_pack_kernel(const uint16_t* __restrict__ h, int64_t stride, const int64
     if (lab[i] != ignore) {
       if (k >= first && k < first + kPackRows) {
         const bool known = lab[i] >= 0 && lab[i] < vocab;
-        if (!known) *bad = lab[i];
+        if (!known) bad[lab[i] < 0 ? 2 : 0] = lab[i];
         source[k - first] = r;
         index[k] = r;
         label[k] = known ? (int)lab[i] : -1;

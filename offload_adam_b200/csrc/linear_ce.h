@@ -25,7 +25,7 @@ struct LceArgs {
   float* inv = nullptr;              // 1 / max(1, packed rows)
   float* lse = nullptr;              // (rows,) of the packed row
   void* packed = nullptr;            // bf16 (rows padded, hidden)
-  int64_t* report = nullptr;         // host memory: [0] a label outside the vocabulary, [1] a wait that gave up
+  int64_t* report = nullptr;         // host memory: [0] a label past the vocabulary, [1] a wait that gave up, [2] a negative label
 };
 
 // Rows of `packed` and of a piece of the logits' gradient.

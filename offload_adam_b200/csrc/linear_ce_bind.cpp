@@ -1,6 +1,7 @@
 // Autograd function of the cross entropy that keeps no logits, and its Python binding.
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/extension.h>
 
 #include <algorithm>
@@ -100,7 +101,9 @@ struct LinearCE : torch::autograd::Function<LinearCE> {
     const Tensor& g = grads[0];
     const bool want_h = ctx->needs_input_grad(0), want_w = ctx->needs_input_grad(1);
     if (!g.defined() || !(want_h || want_w)) return {Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
-    TORCH_CHECK(!at::GradMode::is_enabled(), "linear_cross_entropy has no second derivative (create_graph)");
+    // the gradients can be had with create_graph, but not differentiated again
+    const bool graph = at::GradMode::is_enabled();
+    at::NoGradGuard no_grad;
     const auto saved = ctx->get_saved_variables();
     const Tensor &w = saved[1], &labels = saved[2], kept = saved[3].contiguous();
     const int64_t reduction = ctx->saved_data["reduction"].toInt(), ignore = ctx->saved_data["ignore"].toInt();
@@ -134,6 +137,15 @@ struct LinearCE : torch::autograd::Function<LinearCE> {
       x.gw = gw.data_ptr();
     }
     ok(oab::launch_lce_backward(make_args(wc, lc, kept, ignore, packed), x, cur()), "linear_cross_entropy backward");
+    if (graph) {
+      const auto last = std::make_shared<torch::autograd::DelayedError>("linear_cross_entropy has no second derivative", 2);
+      for (Tensor* t : {&gh, &gw})
+        if (t->defined()) t->set_requires_grad(true);
+      at::AutoGradMode with_grad(true);
+      auto out = (*last)({gh, gw});
+      gh = out[0];
+      gw = out[1];
+    }
     return {gh, gw, Tensor(), Tensor(), Tensor(), Tensor()};
   }
 };

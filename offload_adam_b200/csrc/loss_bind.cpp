@@ -109,16 +109,17 @@ Tensor sum_bf16(const Tensor& acc, const Tensor& g, bool round, const std::optio
 // that kernel has run: the call itself returns NaN, and the next one (its backward, or the
 // next loss) raises.  PyTorch's operations end the context with a device assertion instead,
 // which the next call that looks reports as late.  [1]: not 0 when a kernel gave up a wait.
+// [2]: a negative label that is not the ignored one (linear_ce.cu), 0 for none.
 int64_t* oab::loss_report() {
   static int64_t* const at = [] {
     cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;  // the first call may be captured
     ok(cudaThreadExchangeStreamCaptureMode(&mode), "label report");
     void* p = nullptr;
-    const cudaError_t e = cudaHostAlloc(&p, 2 * sizeof(int64_t), cudaHostAllocPortable | cudaHostAllocMapped);
+    const cudaError_t e = cudaHostAlloc(&p, 3 * sizeof(int64_t), cudaHostAllocPortable | cudaHostAllocMapped);
     ok(cudaThreadExchangeStreamCaptureMode(&mode), "label report");
     ok(e, "label report");
     static_cast<int64_t*>(p)[0] = -1;
-    static_cast<int64_t*>(p)[1] = 0;
+    static_cast<int64_t*>(p)[1] = static_cast<int64_t*>(p)[2] = 0;
     return static_cast<int64_t*>(p);
   }();
   return at;
@@ -129,9 +130,11 @@ void oab::raise_loss_report() {
     __atomic_store_n(at + 1, int64_t(0), __ATOMIC_RELAXED);
     TORCH_CHECK(false, "a kernel of an earlier cross-entropy gave up waiting for its own pipeline; its results are not valid");
   }
-  if (__atomic_load_n(at, __ATOMIC_RELAXED) < 0) return;
-  const int64_t label = __atomic_exchange_n(at, int64_t(-1), __ATOMIC_RELAXED);
-  TORCH_CHECK_INDEX(label < 0, "label ", std::to_string(label), " of an earlier cross-entropy is outside its vocabulary; that loss is NaN");
+  int64_t label = -1;
+  if (__atomic_load_n(at, __ATOMIC_RELAXED) >= 0) label = __atomic_exchange_n(at, int64_t(-1), __ATOMIC_RELAXED);
+  else if (__atomic_load_n(at + 2, __ATOMIC_RELAXED) != 0) label = __atomic_exchange_n(at + 2, int64_t(0), __ATOMIC_RELAXED);
+  else return;
+  TORCH_CHECK_INDEX(false, "label ", std::to_string(label), " of an earlier cross-entropy is outside its vocabulary; that loss is NaN");
 }
 
 void bind_loss(py::module_& m) {

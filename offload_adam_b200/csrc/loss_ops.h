@@ -34,7 +34,7 @@ cudaError_t launch_ce_grad(const void* logits, int64_t pitch, const int64_t* lab
 cudaError_t launch_sum_bf16(const void* acc, bool acc_is_f32, const void* g, float* out_f32, void* out_bf16, int64_t n,
                             cudaStream_t st);
 
-// Two words of mapped host memory in which the loss kernels report (loss_bind.cpp), and the
+// Three words of mapped host memory in which the loss kernels report (loss_bind.cpp), and the
 // check that turns what stands there into an exception.
 int64_t* loss_report();
 void raise_loss_report();

@@ -10,7 +10,8 @@ the same for any HF causal LM that exposes its decoder as ``.model`` and an unbi
 usual, the head and the loss run a group of rows at a time through
 :func:`offload_adam_b200.models.llama.chunked_linear_cross_entropy`, which keeps at most
 four chunks of bf16 logits for the gradients of the hidden states and of the head
-weight.  Tied
+weight, or with ``piece`` through :func:`offload_adam_b200.ops.linear_ce.linear_cross_entropy`,
+which keeps none.  Tied
 embeddings work unchanged (the head weight is the embedding parameter; autograd adds
 both contributions)."""
 
@@ -18,6 +19,7 @@ from __future__ import annotations
 
 import torch
 
+from ..ops.linear_ce import linear_cross_entropy
 from .llama import chunked_linear_cross_entropy
 
 
@@ -37,10 +39,12 @@ def supports_chunked_loss(hf_model) -> bool:
     return True
 
 
-def causal_lm_loss(hf_model, input_ids, labels=None, chunk: int = 2048, **model_kwargs):
+def causal_lm_loss(hf_model, input_ids, labels=None, chunk: int = 2048, piece=None, **model_kwargs):
     """Mean next-token cross-entropy of ``hf_model`` on ``input_ids`` (labels shifted here,
-    ``-100`` ignored, as in HuggingFace's own loss).  Falls back to the module's own loss
-    when the model does not have the plain ``.model`` / ``.lm_head`` structure."""
+    ``-100`` ignored, as in HuggingFace's own loss).  ``chunk`` rows of the logits at a time, or
+    ``piece`` words of the vocabulary (0: the package chooses) without keeping logits.  Falls
+    back to the module's own loss when the model does not have the plain ``.model`` /
+    ``.lm_head`` structure."""
     labels = input_ids if labels is None else labels
     if not supports_chunked_loss(hf_model):
         return hf_model(input_ids=input_ids, labels=labels, **model_kwargs).loss
@@ -48,4 +52,6 @@ def causal_lm_loss(hf_model, input_ids, labels=None, chunk: int = 2048, **model_
     B, S, H = h.shape
     shift = torch.full_like(labels, -100)
     shift[:, :-1] = labels[:, 1:]
+    if piece is not None:
+        return linear_cross_entropy(h, hf_model.lm_head.weight, shift, piece=piece)
     return chunked_linear_cross_entropy(h.reshape(B * S, H), hf_model.lm_head.weight, shift.reshape(-1), chunk)

@@ -6,7 +6,8 @@ attention, gradient checkpointing and a fused linear cross-entropy
 ingredients without external model code: RMSNorm, rotary embeddings, grouped
 query attention through ``scaled_dot_product_attention``, SwiGLU, optional
 per-layer activation checkpointing and a chunked linear + cross-entropy head
-that holds the logits of a few thousand tokens at most, in bf16.
+that holds the logits of a few thousand tokens at most, in bf16, or with ``ce_piece``
+one that holds none.
 
 Parameter names and shapes match the HF Llama layout (``model.embed_tokens``,
 ``model.layers.N.self_attn.{q,k,v,o}_proj``, ``mlp.{gate,up,down}_proj``,
@@ -26,6 +27,7 @@ from torch.utils.checkpoint import checkpoint
 
 from .. import _ext
 from ..ops.dispatch import use_kernels
+from ..ops.linear_ce import linear_cross_entropy
 
 
 @dataclass
@@ -41,6 +43,9 @@ class LlamaConfig:
     tie_embeddings: bool = False
     init_std: float = 0.02
     ce_chunk: int = 2048  # rows of the logits that the loss head holds (see _CE_ROWS_PER_CHUNK)
+    # words of the vocabulary that the loss handles at a time, 0: the package chooses.  The loss then
+    # holds no logits (ops.linear_ce) and ce_chunk has no meaning; None: chunks of rows
+    ce_piece: Optional[int] = None
     head_dim_override: Optional[int] = None  # Qwen3: 128 whatever hidden_size / num_heads is
     qk_norm: bool = False  # Qwen3: RMSNorm over head_dim on queries and keys before RoPE
 
@@ -449,6 +454,8 @@ class LlamaForCausalLM(nn.Module):
         B, S, H = h.shape
         shift = torch.full_like(labels, -100)
         shift[:, :-1] = labels[:, 1:]
+        if self.config.ce_piece is not None:
+            return linear_cross_entropy(h, self.lm_head.weight, shift, piece=self.config.ce_piece)
         return chunked_linear_cross_entropy(h.reshape(B * S, H), self.lm_head.weight,
                                             shift.reshape(-1), self.config.ce_chunk)
 
