@@ -6,13 +6,22 @@
 // Rows whose label is ignored take no part: the others are packed first, so their work is saved
 // and nothing that stands in them (a padded batch's NaN) reaches a sum.
 //
+// Precision.  A confident row's loss is the small difference of two large numbers, so it is not
+// formed as one: packing computes the label's logit apart, in fp32 on the ordinary cores; the products'
+// statistics leave that word out; and with their m and s
+//     loss_i = log(1 + s exp(m - z_label)),    1 - p_label = 1 - exp(-loss_i)
+// in fp64.  The gradient of the logits is held apart from its size: with q_i = 1 - p_label,
+//     d_ij = q_i g_i (exp(z_ij - rest_i) - [j = label_i]),    rest_i = log sum_{j != label} exp z_ij
+// so the label's entry, which most of a row's gradient hangs on, is -1 exactly in bf16; q_i g_i is
+// applied to the fp32 sums of dh, and to the rows of h that go into dW.  tcgen05 cuts off what it adds to an accumulator (about half a unit, 2^-24, towards zero
+// each time: logits of 4096 terms came out 1.5e-5 too small, losses 2.5e-5 off), so the statistics
+// take their logits in chains of 32 additions (512 terms; 8 for few rows) that the epilogue adds up.
+//
 // Forward: one product whose epilogue keeps, per row and 128 words, the maximum and the sum of
 // exponentials (8 bytes for 256 bytes of bf16 logits), and a small kernel that joins them.
 // Backward, for each piece of the vocabulary: the product again, whose epilogue writes the
 // gradient of the piece's logits in bf16, and one launch for both products that read it; dh is
-// summed over the pieces in fp32 and rounded once.  Where the scale of the incoming gradient is one
-// number it is applied to the fp32 sums, so d holds p - [j = label] as it is: its largest
-// entries, near -1, lose least.
+// summed over the pieces in fp32 and rounded once.
 //
 // All three products are one pipeline: a CTA pair computes a 256 x 256 tile with tcgen05 (each CTA
 // 128 rows, half of B each), TMA fills six stages of 64 inner values, two accumulators in tensor
@@ -36,8 +45,9 @@ constexpr int kHalfBytes = 128 * kInner * 2;            // one CTA's part of an 
 constexpr int kStageBytes = 2 * kHalfBytes;
 constexpr int kEpilogueWarps = 16;       // eight for each accumulator
 constexpr int kStagingBytes = 32 * 64;   // of an epilogue warp: 32 lines of 64 bytes on their way out
-constexpr int kSmemBytes = kStages * kStageBytes + kEpilogueWarps * kStagingBytes + 1024;  // starts on 1024 bytes
+constexpr int smem_of(bool staging) { return kStages * kStageBytes + (staging ? kEpilogueWarps * kStagingBytes : 0) + 1024; }  // starts on 1024 bytes
 constexpr int kGemmThreads = 64 + 32 * kEpilogueWarps;
+constexpr int kChain = 8;   // stages of a chain of the statistics
 constexpr int kGroup = 16;  // row tiles that share a column tile in turn: 4096 rows of h stay in L2
 
 enum Pass { kStats = 0, kLogitGrad = 1, kGrads = 2 };
@@ -58,11 +68,8 @@ struct GemmParams {
   const int* label;
   // kStats
   float2* part;
-  float* picked;
   // kLogitGrad
-  const float* lse;
-  const float* row_g;  // by row, or null
-  const int* index;
+  const float* rest;
   uint16_t* d;           // few rows
   int64_t pitch;
   // kGrads
@@ -177,63 +184,50 @@ struct Plan {
 };
 
 // ------------------------------------------------------------------- epilogues
-// Every epilogue warp handles 32 rows (lanes) and 128 columns of the CTA's 128 x 256 tile, and every
-// other tile of its pair.  A warp is a chain of latencies (the accumulator is done, its load, a
-// fence, the way out), so there are eight for each accumulator, and the accumulator is given
-// back (`release`) with the last load from it, before anything is computed from that.
+// Of the gradients: every epilogue warp handles 32 rows (lanes) and 128 columns of the CTA's 128 x 256
+// tile, and every other tile of its pair.  A warp is a chain of latencies (the accumulator is
+// done, its load, a fence, the way out), so there are eight for each accumulator, and the accumulator
+// is given back (`release`) with the last load from it, before anything is computed from that.
+// Of the statistics: all sixteen take 64 columns of every tile, chain by chain.
 
 struct RowValues {  // of the packed row that a thread has in a tile
   int label;
-  float lse, g;
+  float rest;
 };
 template <int PASS>
 __device__ __forceinline__ RowValues row_values(const GemmParams& p, int row, int n_rows) {
-  RowValues r{-1, INFINITY, 1.f};
+  RowValues r{-1, INFINITY};
   if (PASS != kGrads && row < n_rows) {
     r.label = p.label[row];
-    if (PASS == kLogitGrad) {
-      r.lse = p.lse[row];
-      if (p.row_g != nullptr) r.g = p.row_g[p.index[row]];
-    }
+    if (PASS == kLogitGrad) r.rest = p.rest[row];
   }
   return r;
 }
 
-template <class Release>
-__device__ __forceinline__ void stats_tile(const GemmParams& p, const Tile& x, uint32_t tmem, int row, int n_rows, int half,
-                                           const RowValues& values, const Release& release) {
-  const int lab = values.label;
-  float m = -INFINITY, s = 0.f;
-#pragma unroll 1
-  for (int c = 0; c < 2; ++c) {
-    float v[64];
-    tmem_load64(tmem + c * 64, v);
-    if (c == 1) release();
-    const int col = x.n + half * 128 + c * 64, left = p.words - col;
-    if (left < 64) {
+// {max, sum of exponentials} of a row's 64 logits from column `col` on, without the label's.
+__device__ __forceinline__ float2 stats_of(float (&v)[64], int col, int words, int label) {
+  const int left = words - col, hit = label - col;
+  if (left < 64 || (hit >= 0 && hit < 64)) {
 #pragma unroll
-      for (int i = 0; i < 64; ++i)
-        if (i >= left) v[i] = -INFINITY;
-    }
-    const int hit = lab - col;
-    if (hit >= 0 && hit < 64) {
-      float z = v[0];
-#pragma unroll
-      for (int i = 1; i < 64; ++i)
-        if (i == hit) z = v[i];
-      p.picked[row] = z;
-    }
-    float top[4] = {m, m, m, m};
-#pragma unroll
-    for (int i = 0; i < 64; ++i) top[i & 3] = fmaxf(top[i & 3], v[i]);
-    const float mn = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])), sh = finite_shift(mn);
-    float t[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int i = 0; i < 64; ++i) t[i & 3] = __fadd_rn(t[i & 3], exp_of(__fsub_rn(v[i], sh)));
-    s = __fadd_rn(__fmul_rn(s, exp_of(__fsub_rn(m, sh))), __fadd_rn(__fadd_rn(t[0], t[1]), __fadd_rn(t[2], t[3])));
-    m = mn;
+    for (int i = 0; i < 64; ++i)
+      if (i >= left || i == hit) v[i] = -INFINITY;
   }
-  if (row < n_rows) p.part[(int64_t)(x.n / 128 + half) * p.rows + row] = make_float2(m, s);
+  float top[4] = {v[0], v[1], v[2], v[3]};
+#pragma unroll
+  for (int i = 4; i < 64; ++i) top[i & 3] = fmaxf(top[i & 3], v[i]);
+  const float m = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])), sh = finite_shift(m);
+  float t[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int i = 0; i < 64; ++i) t[i & 3] = __fadd_rn(t[i & 3], exp_of(__fsub_rn(v[i], sh)));
+  return make_float2(m, __fadd_rn(__fadd_rn(t[0], t[1]), __fadd_rn(t[2], t[3])));
+}
+__device__ __forceinline__ float2 join4(const float2* a, int stride) {
+  const float2 w[4] = {a[0], a[stride], a[2 * stride], a[3 * stride]};
+  const float m = fmaxf(fmaxf(w[0].x, w[1].x), fmaxf(w[2].x, w[3].x)), sh = finite_shift(m);
+  float s = 0.f;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) s = __fadd_rn(s, __fmul_rn(w[i].y, exp_of(__fsub_rn(w[i].x, sh))));
+  return make_float2(m, s);
 }
 
 // A warp's 32 lines of 64 bytes leave through its staging buffer, 16-byte parts swizzled as TMA
@@ -261,8 +255,7 @@ template <class Release>
 __device__ __forceinline__ void logit_grad_tile(const GemmParams& p, const Tile& x, uint32_t tmem, int row, int half, uint32_t staging,
                                                 int lane, const RowValues& values, const Release& release) {
   const int lab = values.label >= 0 ? (int)(values.label - p.word0) : -1;
-  // the rows that pad the inner dimension of dW become zero: their logits are 0, their lse infinite
-  const float lse = values.lse, g = values.g;
+  const float rest = values.rest;
 #pragma unroll 1
   for (int c = 0; c < 4; ++c) {
     float v[32];
@@ -270,16 +263,12 @@ __device__ __forceinline__ void logit_grad_tile(const GemmParams& p, const Tile&
     if (c == 3) release();
     const int col = x.n + half * 128 + c * 32;
 #pragma unroll
-    for (int i = 0; i < 32; ++i) v[i] = exp_of(__fsub_rn(v[i], lse));
+    for (int i = 0; i < 32; ++i) v[i] = exp_of(__fsub_rn(v[i], rest));
     const int hit = lab - col;
     if (lab >= 0 && hit >= 0 && hit < 32) {
 #pragma unroll
       for (int i = 0; i < 32; ++i)
-        if (i == hit) v[i] = __fsub_rn(v[i], 1.f);
-    }
-    if (p.row_g != nullptr) {
-#pragma unroll
-      for (int i = 0; i < 32; ++i) v[i] = __fmul_rn(v[i], g);
+        if (i == hit) v[i] = -1.f;
     }
     stage_bf16(staging, lane, v);
     if (lane == 0) {
@@ -344,6 +333,8 @@ lce_product_kernel(const __grid_constant__ GemmParams p) {
   __shared__ uint64_t full[kStages], empty[kStages], done[2], drained[2];
   __shared__ uint32_t tmem_at;
   __shared__ int gave_up;
+  __shared__ float2 row_part[PASS == kStats ? 2 : 1][4][PASS == kStats ? 128 : 1];  // by turn, columns and row
+  __shared__ volatile int stop[4][2];  // of the epilogue warps of the same 32 rows, by turn
   const uint32_t stages = (smem_addr(smem_raw) + 1023u) & ~1023u;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = cluster_rank();
@@ -351,13 +342,14 @@ lce_product_kernel(const __grid_constant__ GemmParams p) {
 
   if (threadIdx.x == 0) {
     gave_up = 0;
+    for (int i = 0; i < 8; ++i) stop[i >> 1][i & 1] = 0;
     for (int i = 0; i < kStages; ++i) {
       mbar_init(full0 + 8 * i, 1);
       mbar_init(empty0 + 8 * i, 1);
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(done0 + 8 * i, 1);
-      mbar_init(drained0 + 8 * i, kEpilogueWarps);  // eight warps of both CTAs
+      mbar_init(drained0 + 8 * i, PASS == kStats ? 2 * kEpilogueWarps : kEpilogueWarps);  // of both CTAs
     }
     mbar_init_fence();
     prefetch_map(&p.a);
@@ -417,32 +409,79 @@ lce_product_kernel(const __grid_constant__ GemmParams p) {
     __syncwarp();
   } else if (warp == 1) {
     if (rank == 0 && elect_one()) {
-      int it = 0;
+      int it = 0, chains = 0;
       for (int mine = 0, t; ok && (t = plan.pick<PASS>(pair, mine)) >= 0; ++mine) {
         const Tile x = plan.at<PASS>(p, t);
         const bool outer_a = PASS == kGrads && x.kind == 1;
         constexpr bool outer_b = PASS == kGrads;
         const uint32_t idesc = instruction(kTile, PASS == kGrads && p.narrow ? kTile / 2 : kTile, outer_a, outer_b);
-        const uint32_t acc = mine & 1, d = tmem + acc * kTile;
-        if (!mbar_wait(drained0 + 8 * acc, ((mine >> 1) & 1) ^ 1)) { ok = false; break; }
-        fence_after();
-        for (int k = 0; k < x.steps; ++k, ++it) {
-          const int s = it % kStages;
-          if (!mbar_wait(full0 + 8 * s, (it / kStages) & 1)) { ok = false; break; }
+        int k = 0;
+        do {  // one chain; a tile of no stage has an empty one
+          const int last = PASS == kStats && k + kChain < x.steps ? k + kChain : x.steps;
+          const uint32_t acc = chains & 1, d = tmem + acc * kTile;
+          if (!mbar_wait(drained0 + 8 * acc, ((chains >> 1) & 1) ^ 1)) { ok = false; break; }
           fence_after();
-          const uint32_t at = stages + s * kStageBytes, bt = at + kHalfBytes;
-          const uint64_t da = outer_a ? operand(at, kHalfBytes / 2, 1024) : operand(at, 16, 1024);
-          const uint64_t db = outer_b ? operand(bt, kHalfBytes / 2, 1024) : operand(bt, 16, 1024);
-          // 16 inner values further: 32 bytes along a row, or 16 lines of 128 bytes
-          const uint64_t step_a = outer_a ? 2048 >> 4 : 32 >> 4, step_b = outer_b ? 2048 >> 4 : 32 >> 4;
+          for (bool begun = false; k < last; ++k, ++it) {
+            const int s = it % kStages;
+            if (!mbar_wait(full0 + 8 * s, (it / kStages) & 1)) { ok = false; break; }
+            fence_after();
+            const uint32_t at = stages + s * kStageBytes, bt = at + kHalfBytes;
+            const uint64_t da = outer_a ? operand(at, kHalfBytes / 2, 1024) : operand(at, 16, 1024);
+            const uint64_t db = outer_b ? operand(bt, kHalfBytes / 2, 1024) : operand(bt, 16, 1024);
+            // 16 inner values further: 32 bytes along a row, or 16 lines of 128 bytes
+            const uint64_t step_a = outer_a ? 2048 >> 4 : 32 >> 4, step_b = outer_b ? 2048 >> 4 : 32 >> 4;
 #pragma unroll
-          for (int q = 0; q < kInner / 16; ++q) mma_pair(d, da + q * step_a, db + q * step_b, idesc, k > 0 || q > 0);
-          commit_pair(empty0 + 8 * s);
-        }
-        commit_pair(done0 + 8 * acc);
+            for (int q = 0; q < kInner / 16; ++q) {
+              mma_pair(d, da + q * step_a, db + q * step_b, idesc, begun);
+              begun = true;
+            }
+            commit_pair(empty0 + 8 * s);
+          }
+          commit_pair(done0 + 8 * acc);
+          ++chains;
+        } while (ok && k < x.steps);
       }
     }
     __syncwarp();
+  } else if constexpr (PASS == kStats) {
+    const int quarter = warp & 3, part = (warp - 2) >> 2, in_cta = quarter * 32 + lane;
+    const uint32_t lead_drained0 = map_to_rank(drained0, 0);
+    int chains = 0;
+    for (int mine = 0, t; (t = plan.pick<PASS>(pair, mine)) >= 0; ++mine) {
+      const Tile x = plan.at<PASS>(p, t);
+      const int row = x.m + (int)rank * 128 + in_cta, turn = mine & 1;
+      const RowValues values = row_values<PASS>(p, row, n_rows);  // on their way while the products run
+      float v[64];
+      for (int k = 0; k < x.steps && ok; k += kChain, ++chains) {
+        const uint32_t acc = chains & 1, at = tmem + acc * kTile + part * 64 + ((uint32_t)(quarter * 32) << 16);
+        ok = mbar_wait(done0 + 8 * acc, (chains >> 1) & 1);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        fence_after();
+        if (k == 0) {
+          tmem_load64(at, v);
+        } else {
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            float more[16];
+            tmem_load16(at + c * 16, more);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) v[c * 16 + i] = __fadd_rn(v[c * 16 + i], more[i]);
+          }
+        }
+        fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive_cluster(lead_drained0 + 8 * acc);
+      }
+      // The four warps of these rows join.  One that gave up comes here, too, and they all leave:
+      // what belongs to a turn is written again two turns later, when they have met once more.
+      if (ok) row_part[turn][part][in_cta] = stats_of(v, x.n + part * 64, p.words, values.label);
+      else stop[quarter][turn] = 1;
+      asm volatile("bar.sync %0, 128;" ::"r"(1 + quarter) : "memory");
+      ok = stop[quarter][turn] == 0;
+      if (!ok) break;
+      if (part == 0 && row < n_rows) p.part[(int64_t)(x.n / kTile) * p.rows + row] = join4(&row_part[turn][0][in_cta], 128);
+    }
   } else {
     const int quarter = warp & 3, half = ((warp - 2) >> 2) & 1, group = (warp - 2) >> 3;
     const uint32_t lead_drained0 = map_to_rank(drained0, 0);
@@ -467,12 +506,11 @@ lce_product_kernel(const __grid_constant__ GemmParams p) {
         __syncwarp();
         if (lane == 0) mbar_arrive_cluster(lead_drained0 + 8 * acc);
       };
-      if (PASS == kStats) stats_tile(p, x, at, row, n_rows, half, values, release);
       if (PASS == kLogitGrad) logit_grad_tile(p, x, at, row, half, staging, lane, values, release);
       if (PASS == kGrads && x.kind == 0) dh_tile(p, x, at, row, n_rows, half, staging, lane, release);
       if (PASS == kGrads && x.kind == 1) dw_tile(p, x, at, row, half, scale, staging, lane, release);
     }
-    if (PASS != kStats && lane == 0) store_wait();
+    if (lane == 0) store_wait();
     __syncwarp();
   }
   if (!ok) gave_up = 1;
@@ -495,8 +533,9 @@ constexpr int kFewThreads = 64 + 128;
 template <int N>
 struct FewShape {
   static constexpr int kStage = kHalfBytes + N * 128, kCount = (220 * 1024) / kStage, kSmem = kCount * kStage + 1024;
-  static constexpr int kColumns = 2 * N < 32 ? 32 : 2 * N;  // of tensor memory: two accumulators
+  static constexpr int kAccs = 4, kColumns = kAccs * N;  // accumulators in tensor memory
 };
+constexpr int kFewChain = 2;  // stages
 template <int N>
 __device__ __forceinline__ void tmem_load_rows(uint32_t at, float (&v)[N]) {
   if constexpr (N == 16) {
@@ -512,12 +551,12 @@ __global__ void __launch_bounds__(kFewThreads, 1)
 lce_few_kernel(const __grid_constant__ GemmParams p, float* acc) {
   using S = FewShape<N>;
   extern __shared__ uint8_t smem_raw[];
-  __shared__ uint64_t full[S::kCount], empty[S::kCount], done[2], drained[2];
+  __shared__ uint64_t full[S::kCount], empty[S::kCount], done[S::kAccs], drained[S::kAccs];
   __shared__ uint32_t tmem_at;
   __shared__ int gave_up;
   __shared__ volatile int stop;  // of the epilogue warps
   __shared__ int label_of[N];
-  __shared__ float lse_of[N], g_of[N];
+  __shared__ float rest_of[N];
   __shared__ float2 warp_part[4][N];
   const uint32_t stages = (smem_addr(smem_raw) + 1023u) & ~1023u;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -530,7 +569,7 @@ lce_few_kernel(const __grid_constant__ GemmParams p, float* acc) {
       mbar_init(full0 + 8 * i, 1);
       mbar_init(empty0 + 8 * i, 1);
     }
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < S::kAccs; ++i) {
       mbar_init(done0 + 8 * i, 1);
       mbar_init(drained0 + 8 * i, 4);
     }
@@ -541,10 +580,7 @@ lce_few_kernel(const __grid_constant__ GemmParams p, float* acc) {
   if (PASS != kGrads && threadIdx.x < N) {
     const int r = threadIdx.x;
     label_of[r] = r < n_rows ? p.label[r] : -1;
-    if (PASS == kLogitGrad) {
-      lse_of[r] = r < n_rows ? p.lse[r] : 0.f;
-      g_of[r] = r < n_rows && p.row_g != nullptr ? p.row_g[p.index[r]] : 1.f;
-    }
+    if (PASS == kLogitGrad) rest_of[r] = r < n_rows ? p.rest[r] : INFINITY;
   }
   if (warp == 1) tmem_alloc(smem_addr(&tmem_at), S::kColumns);
   fence_before();
@@ -593,45 +629,66 @@ lce_few_kernel(const __grid_constant__ GemmParams p, float* acc) {
   } else if (warp == 1) {
     if (elect_one()) {
       constexpr uint32_t idesc = instruction(128, N, PASS == kGrads, false);
-      int it = 0, mine = 0;
-      for (int t = blockIdx.x; t < total && ok; t += gridDim.x, ++mine) {
+      int it = 0, chains = 0;
+      for (int t = blockIdx.x; t < total && ok; t += gridDim.x) {
         int first;
         const int steps = share(t, first);
-        const uint32_t buf = mine & 1, d = tmem + buf * N;
-        if (!mbar_wait(drained0 + 8 * buf, ((mine >> 1) & 1) ^ 1)) { ok = false; break; }
-        fence_after();
-        for (int k = 0; k < steps; ++k, ++it) {
-          const int s = it % S::kCount;
-          if (!mbar_wait(full0 + 8 * s, (it / S::kCount) & 1)) { ok = false; break; }
+        int k = 0;
+        do {  // one chain; a tile of no stage has an empty one
+          const int last = PASS == kStats && k + kFewChain < steps ? k + kFewChain : steps;
+          const uint32_t buf = chains % S::kAccs, d = tmem + buf * N;
+          if (!mbar_wait(drained0 + 8 * buf, ((chains / S::kAccs) & 1) ^ 1)) { ok = false; break; }
           fence_after();
-          const uint32_t at = stages + s * S::kStage;
-          const uint64_t da = PASS == kGrads ? operand(at, kHalfBytes / 2, 1024) : operand(at, 16, 1024);
-          const uint64_t db = operand(at + kHalfBytes, 16, 1024);
-          constexpr uint64_t step_a = PASS == kGrads ? 2048 >> 4 : 32 >> 4;
+          for (bool begun = false; k < last; ++k, ++it) {
+            const int s = it % S::kCount;
+            if (!mbar_wait(full0 + 8 * s, (it / S::kCount) & 1)) { ok = false; break; }
+            fence_after();
+            const uint32_t at = stages + s * S::kStage;
+            const uint64_t da = PASS == kGrads ? operand(at, kHalfBytes / 2, 1024) : operand(at, 16, 1024);
+            const uint64_t db = operand(at + kHalfBytes, 16, 1024);
+            constexpr uint64_t step_a = PASS == kGrads ? 2048 >> 4 : 32 >> 4;
 #pragma unroll
-          for (int q = 0; q < kInner / 16; ++q) mma(d, da + q * step_a, db + q * (32 >> 4), idesc, k > 0 || q > 0);
-          commit(empty0 + 8 * s);
-        }
-        commit(done0 + 8 * buf);
+            for (int q = 0; q < kInner / 16; ++q) {
+              mma(d, da + q * step_a, db + q * (32 >> 4), idesc, begun);
+              begun = true;
+            }
+            commit(empty0 + 8 * s);
+          }
+          commit(done0 + 8 * buf);
+          ++chains;
+        } while (ok && k < steps);
       }
     }
     __syncwarp();
   } else {
     const int quarter = warp & 3;
-    int mine = 0;
-    for (int t = blockIdx.x; t < total; t += gridDim.x, ++mine) {
+    int chains = 0;
+    for (int t = blockIdx.x; t < total; t += gridDim.x) {
       int first;
-      const int steps = share(t, first), m = t % across * 128;
-      const uint32_t buf = mine & 1;
-      ok = mbar_wait(done0 + 8 * buf, (mine >> 1) & 1);
-      ok = __all_sync(0xffffffffu, ok);
-      if (PASS != kStats && !ok) break;
-      fence_after();
+      const int steps = share(t, first), m = t % across * 128, length = PASS == kStats ? kFewChain : steps;
       float v[N];
-      tmem_load_rows<N>(tmem + buf * N + ((uint32_t)(quarter * 32) << 16), v);
-      fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(drained0 + 8 * buf);
+      int k = 0;
+      do {
+        const uint32_t buf = chains % S::kAccs, from = tmem + buf * N + ((uint32_t)(quarter * 32) << 16);
+        ok = mbar_wait(done0 + 8 * buf, (chains / S::kAccs) & 1);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        fence_after();
+        if (k == 0) {
+          tmem_load_rows<N>(from, v);
+        } else {
+          float more[N];
+          tmem_load_rows<N>(from, more);
+#pragma unroll
+          for (int r = 0; r < N; ++r) v[r] = __fadd_rn(v[r], more[r]);
+        }
+        fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(drained0 + 8 * buf);
+        ++chains;
+        k += length;
+      } while (k < steps);
+      if (PASS != kStats && !ok) break;
       const int at = m + quarter * 32 + lane;  // this lane's word of the piece, or hidden column
       if (PASS == kStats) {
         if (!ok) stop = 1;
@@ -640,8 +697,7 @@ lce_few_kernel(const __grid_constant__ GemmParams p, float* acc) {
 #pragma unroll
         for (int r = 0; r < N; ++r) {
           if (r >= n_rows) break;
-          const float z = in ? v[r] : -INFINITY;
-          if (in && label_of[r] == at) p.picked[r] = z;
+          const float z = in && label_of[r] != at ? v[r] : -INFINITY;  // the label's is known apart
           float top = z;
 #pragma unroll
           for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
@@ -658,13 +714,7 @@ lce_few_kernel(const __grid_constant__ GemmParams p, float* acc) {
         if (!ok) break;
         const int r = threadIdx.x - 64;
         if (r < n_rows) {
-          float top = -INFINITY, sum = 0.f;
-#pragma unroll
-          for (int w = 0; w < 4; ++w) top = fmaxf(top, warp_part[w][r].x);
-#pragma unroll
-          for (int w = 0; w < 4; ++w)
-            sum = __fadd_rn(sum, __fmul_rn(warp_part[w][r].y, exp_of(__fsub_rn(warp_part[w][r].x, finite_shift(top)))));
-          p.part[(int64_t)(m / 128) * p.rows + r] = make_float2(top, sum);
+          p.part[(int64_t)(m / 128) * p.rows + r] = join4(&warp_part[0][r], N);
         }
         asm volatile("bar.sync 1, 128;" ::: "memory");  // before warp_part is written again
       } else if (PASS == kLogitGrad) {
@@ -672,10 +722,8 @@ lce_few_kernel(const __grid_constant__ GemmParams p, float* acc) {
         if (at < p.words) {
 #pragma unroll
           for (int r = 0; r < N; ++r) {
-            float d = exp_of(__fsub_rn(v[r], lse_of[r]));
-            if (label_of[r] == word) d = __fsub_rn(d, 1.f);
-            // the rows that pad the inner dimension of dW are zero
-            d = r < n_rows ? __fmul_rn(d, g_of[r]) : 0.f;
+            float d = label_of[r] == word ? -1.f : exp_of(__fsub_rn(v[r], rest_of[r]));
+            if (r >= n_rows) d = 0.f;  // the rows that pad the inner dimension of dW
             p.d[(int64_t)r * p.pitch + at] = (uint16_t)f32_to_bf16_rne_bits(d);
           }
           for (int r = N; r < kLceRowPad; ++r) p.d[(int64_t)r * p.pitch + at] = 0;
@@ -748,35 +796,61 @@ lce_scan_kernel(const int64_t* __restrict__ labels, int64_t rows, int64_t vocab,
   }
 }
 
-// packed[k] = h[index[k]], zero rows up to the next multiple of kLceRowPad.  A warp a row.
+// packed[k] = h[index[k]], zero rows up to the next multiple of kLceRowPad, and the logit of its
+// label.  A warp a row.
 constexpr int kPackThreads = 256, kPackRows = kPackThreads / 32;
-__device__ __forceinline__ void pack_row(const uint16_t* h, int64_t stride, int64_t from_row, bool copy, bool zero, int hidden, uint16_t* to) {
-  const int vecs = hidden >> 3, lane = threadIdx.x & 31;
-  uint4* t = reinterpret_cast<uint4*>(to);
-  if (copy) {
-    const uint4* f = reinterpret_cast<const uint4*>(h + from_row * stride);
+struct PackArgs {
+  const uint16_t* h;
+  int64_t h_stride;
+  const uint16_t* w;
+  int64_t w_stride;
+  int hidden;
+  uint16_t* packed;
+  float* picked;
+};
+__device__ __forceinline__ float dot2(uint32_t a, uint32_t b, float c) {  // of two bf16 pairs
+  c = __fmaf_rn(__uint_as_float(a << 16), __uint_as_float(b << 16), c);
+  return __fmaf_rn(__uint_as_float(a & 0xffff0000u), __uint_as_float(b & 0xffff0000u), c);
+}
+// n: how many rows are packed; `row`, `label`: of packed row k < n
+__device__ __forceinline__ void pack_row(const PackArgs& a, int64_t k, int n, int row, int label) {
+  const int vecs = a.hidden >> 3, lane = threadIdx.x & 31;
+  uint4* to = reinterpret_cast<uint4*>(a.packed + k * a.hidden);
+  if (k < n) {
+    const uint4* from = reinterpret_cast<const uint4*>(a.h + row * a.h_stride);
+    const uint4* word = reinterpret_cast<const uint4*>(a.w + (label < 0 ? 0 : label) * a.w_stride);
+    float x[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 4
-    for (int v = lane; v < vecs; v += 32) t[v] = f[v];
-  } else if (zero) {
-    for (int v = lane; v < vecs; v += 32) t[v] = make_uint4(0, 0, 0, 0);
+    for (int v = lane; v < vecs; v += 32) {
+      const uint4 f = from[v], g = word[v];
+      to[v] = f;
+      x[0] = dot2(f.x, g.x, x[0]);
+      x[1] = dot2(f.y, g.y, x[1]);
+      x[2] = dot2(f.z, g.z, x[2]);
+      x[3] = dot2(f.w, g.w, x[3]);
+    }
+    float z = __fadd_rn(__fadd_rn(x[0], x[1]), __fadd_rn(x[2], x[3]));
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) z = __fadd_rn(z, __shfl_xor_sync(0xffffffffu, z, o));
+    if (lane == 0) a.picked[k] = z;
+  } else if (k < (n + kLceRowPad - 1) / kLceRowPad * kLceRowPad) {
+    for (int v = lane; v < vecs; v += 32) to[v] = make_uint4(0, 0, 0, 0);
   }
 }
 __global__ void __launch_bounds__(kPackThreads)
-lce_pack_kernel(const uint16_t* __restrict__ h, int64_t stride, const int* __restrict__ index, const int* __restrict__ count,
-                int hidden, uint16_t* packed) {
+lce_pack_kernel(const PackArgs a, const int* __restrict__ index, const int* __restrict__ label, const int* __restrict__ count) {
   const int64_t k = (int64_t)blockIdx.x * kPackRows + (threadIdx.x >> 5);
   const int n = *count;
-  pack_row(h, stride, k < n ? index[k] : 0, k < n, k < (n + kLceRowPad - 1) / kLceRowPad * kLceRowPad, hidden, packed + k * hidden);
+  pack_row(a, k, n, k < n ? index[k] : 0, k < n ? label[k] : 0);
 }
 
 // Both in one launch for up to kScanPackRows rows: every block looks through all labels (32 KB at
 // most, from L2) for the eight rows that it packs.  One row: 13 -> 7 us for the two.
 constexpr int kScanPackRows = 4096, kScanPackEach = kScanPackRows / kPackThreads;
 __global__ void __launch_bounds__(kPackThreads)
-lce_scan_pack_kernel(const uint16_t* __restrict__ h, int64_t stride, const int64_t* __restrict__ labels, int rows, int64_t vocab,
-                     int64_t ignore, int* index, int* label, int* count, float* inv, float* row_loss, volatile int64_t* bad,
-                     int hidden, uint16_t* packed) {
-  __shared__ int warps[kPackThreads / 32], source[kPackRows];
+lce_scan_pack_kernel(const PackArgs a, const int64_t* __restrict__ labels, int rows, int64_t vocab, int64_t ignore, int* index,
+                     int* label, int* count, float* inv, float* row_loss, volatile int64_t* bad) {
+  __shared__ int warps[kPackThreads / 32], source[kPackRows], source_label[kPackRows];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, first = blockIdx.x * kPackRows;
   const int each = (rows + kPackThreads - 1) / kPackThreads, r0 = threadIdx.x * each;
   int64_t lab[kScanPackEach];
@@ -793,7 +867,7 @@ lce_scan_pack_kernel(const uint16_t* __restrict__ h, int64_t stride, const int64
     if (lane >= o) x += y;
   }
   if (lane == 31) warps[warp] = x;
-  if (threadIdx.x < kPackRows) source[threadIdx.x] = 0;
+  if (threadIdx.x < kPackRows) source[threadIdx.x] = source_label[threadIdx.x] = 0;
   __syncthreads();
   int k = x - c, n = 0;
 #pragma unroll
@@ -808,9 +882,8 @@ lce_scan_pack_kernel(const uint16_t* __restrict__ h, int64_t stride, const int64
       if (k >= first && k < first + kPackRows) {
         const bool known = lab[i] >= 0 && lab[i] < vocab;
         if (!known) bad[lab[i] < 0 ? 2 : 0] = lab[i];
-        source[k - first] = r;
-        index[k] = r;
-        label[k] = known ? (int)lab[i] : -1;
+        source[k - first] = index[k] = r;
+        source_label[k - first] = label[k] = known ? (int)lab[i] : -1;
       }
       ++k;
     } else if (row_loss != nullptr && r >= first && r < first + kPackRows && i < each && r < rows) {
@@ -823,8 +896,28 @@ lce_scan_pack_kernel(const uint16_t* __restrict__ h, int64_t stride, const int64
     *inv = __fdiv_rn(1.f, (float)(n < 1 ? 1 : n));
   }
   __syncthreads();
-  k = first + warp;
-  pack_row(h, stride, source[warp], k < n, k < (n + kLceRowPad - 1) / kLceRowPad * kLceRowPad, hidden, packed + (int64_t)k * hidden);
+  pack_row(a, first + warp, n, source[warp], source_label[warp]);
+}
+
+// scaled[k] = packed[k] (1 - p_label) g, the rows of h as dW takes them; padded likewise.
+__global__ void __launch_bounds__(kPackThreads)
+lce_scale_kernel(const uint16_t* __restrict__ packed, const int* __restrict__ index, const int* __restrict__ count,
+                 const float* __restrict__ miss, const float* __restrict__ row_g, int hidden, uint16_t* scaled) {
+  const int64_t k = (int64_t)blockIdx.x * kPackRows + (threadIdx.x >> 5);
+  const int n = *count, vecs = hidden >> 3, lane = threadIdx.x & 31;
+  if (k >= (n + kLceRowPad - 1) / kLceRowPad * kLceRowPad) return;
+  float c = k < n ? miss[k] : 0.f;
+  if (k < n && row_g != nullptr) c = __fmul_rn(c, row_g[index[k]]);
+  const uint4* from = reinterpret_cast<const uint4*>(packed + k * hidden);  // zeros beyond n
+  uint4* to = reinterpret_cast<uint4*>(scaled + k * hidden);
+  auto both = [c](uint32_t w) {
+    return f32x2_to_bf16x2_rne(__fmul_rn(__uint_as_float(w << 16), c), __fmul_rn(__uint_as_float(w & 0xffff0000u), c));
+  };
+#pragma unroll 4
+  for (int v = lane; v < vecs; v += 32) {
+    const uint4 f = from[v];
+    to[v] = make_uint4(both(f.x), both(f.y), both(f.z), both(f.w));
+  }
 }
 
 // ------------------------------------------------------------ joining the sums
@@ -840,8 +933,9 @@ __device__ __forceinline__ void join(float& m, float& s, float m2, float s2) {
 __global__ void __launch_bounds__(kJoinThreads)
 lce_join_kernel(const float2* __restrict__ part, int parts, int64_t rows, const int* __restrict__ index,
                 const int* __restrict__ label, int* count, const float* __restrict__ picked, const float* __restrict__ inv,
-                float* lse, int reduction, double* sums, float* loss) {
-  __shared__ float sm[kJoinSlices][kJoinRows], ss[kJoinSlices][kJoinRows], one[kJoinRows];
+                float* rest_out, float* miss, int reduction, double* sums, float* loss) {
+  __shared__ float sm[kJoinSlices][kJoinRows], ss[kJoinSlices][kJoinRows];
+  __shared__ double one[kJoinRows];
   __shared__ int is_last;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int n = *count, of = threadIdx.x % kJoinRows, slice = threadIdx.x / kJoinRows;
@@ -879,13 +973,16 @@ lce_join_kernel(const float2* __restrict__ part, int parts, int64_t rows, const 
     }
     const int64_t at = (int64_t)blockIdx.x * kJoinRows + warp;
     if (lane == 0) {
-      float loss_of = 0.f;
+      double loss_of = 0.0;
       if (at < n) {
-        const bool known = label[at] >= 0;
-        const float l = !known ? NAN : isinf(m) ? m : __fadd_rn(m, logf(s));
-        loss_of = known ? __fsub_rn(l, picked[at]) : NAN;
-        lse[at] = l;
-        if (reduction == kLceNone) loss[index[at]] = loss_of;
+        const double z = picked[at], top = m, rest = s;
+        // an infinite logit of the label's own has no loss, as in PyTorch
+        if (label[at] < 0 || z == INFINITY) loss_of = NAN;
+        else if (z >= top) loss_of = log1p(rest * exp(top - z));
+        else loss_of = top - z + log(rest + exp(z - top));
+        rest_out[at] = m == -INFINITY ? 0.f : (float)(top + log(rest));  // exp(-inf - rest) is 0, too, where all others are
+        miss[at] = (float)-expm1(-loss_of);
+        if (reduction == kLceNone) loss[index[at]] = (float)loss_of;
       }
       one[warp] = loss_of;
     }
@@ -922,15 +1019,17 @@ __device__ __forceinline__ void store_bf16x8(uint16_t* at, const float* v, float
 // Rows whose label is ignored become zero.
 __global__ void __launch_bounds__(128)
 lce_join_grad_kernel(const float* __restrict__ acc, int splits, int64_t padded, const int* __restrict__ index,
-                     const int64_t* __restrict__ labels, int64_t ignore, const int* __restrict__ count, int hidden, const float* inv,
-                     const float* g, uint16_t* gh) {
+                     const int64_t* __restrict__ labels, int64_t ignore, const int* __restrict__ count, int hidden,
+                     const float* __restrict__ miss, const float* inv, const float* g, const float* row_g, uint16_t* gh) {
   const int64_t k = blockIdx.x;
   const int col = (blockIdx.y * 128 + threadIdx.x) * 8;
   if (col >= hidden) return;
   if (labels[k] == ignore) *reinterpret_cast<uint4*>(gh + k * hidden + col) = make_uint4(0, 0, 0, 0);
   if (k >= *count) return;
-  float scale = inv != nullptr ? *inv : 1.f;
+  float scale = miss[k];
+  if (inv != nullptr) scale = __fmul_rn(scale, *inv);
   if (g != nullptr) scale = __fmul_rn(scale, *g);
+  if (row_g != nullptr) scale = __fmul_rn(scale, row_g[index[k]]);
   float v[8] = {};
   for (int s = 0; s < splits; ++s) {
     const V8 x = ld32(acc + ((int64_t)s * padded + k) * hidden + col);
@@ -987,11 +1086,12 @@ template <int PASS>
 cudaError_t launch_product(const GemmParams& p, int64_t tiles, cudaStream_t st) {
   if (tiles <= 0) return cudaSuccess;
   if (tiles > (int64_t(1) << 30)) return cudaErrorInvalidValue;
-  const cudaError_t e = cudaFuncSetAttribute(lce_product_kernel<PASS>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes);
+  constexpr int smem = smem_of(PASS != kStats);
+  const cudaError_t e = cudaFuncSetAttribute(lce_product_kernel<PASS>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   if (e != cudaSuccess) return e;
   const int pairs = (int)(tiles < kNumSMs / 2 ? tiles : kNumSMs / 2);
   count_launch();
-  lce_product_kernel<PASS><<<2 * pairs, kGemmThreads, kSmemBytes, st>>>(p);
+  lce_product_kernel<PASS><<<2 * pairs, kGemmThreads, smem, st>>>(p);
   return cudaGetLastError();
 }
 
@@ -1030,12 +1130,13 @@ void common_params(GemmParams& p, const LceArgs& a) {
   p.vocab = a.vocab;
   p.report = a.report;
   p.label = a.label;
-  p.index = a.index;
 }
 
 }  // namespace
 
-int64_t lce_part_floats(int64_t rows, int64_t vocab) { return 4 * tiles_of(vocab) * rows; }
+int64_t lce_part_floats(int64_t rows, int64_t vocab) {
+  return 2 * rows * (rows <= kLceFewRows ? (vocab + 127) / 128 : tiles_of(vocab));
+}
 int64_t lce_sum_doubles(int64_t rows) { return (rows + kJoinRows - 1) / kJoinRows; }
 
 cudaError_t launch_lce_forward(const LceArgs& a, int reduction, float* part, float* picked, double* sums, float* loss,
@@ -1043,17 +1144,16 @@ cudaError_t launch_lce_forward(const LceArgs& a, int reduction, float* part, flo
   if (!args_ok(a) || a.h_stride % 8 != 0 || !aligned16(a.h)) return cudaErrorInvalidValue;
   float* const row_loss = reduction == kLceNone ? loss : nullptr;
   const unsigned blocks = (unsigned)(lce_padded(a.rows) / kPackRows);
+  const PackArgs k{(const uint16_t*)a.h, a.h_stride, (const uint16_t*)a.w, a.w_stride, (int)a.hidden, (uint16_t*)a.packed, picked};
   if (a.rows <= kScanPackRows) {
     count_launch();
-    lce_scan_pack_kernel<<<blocks, kPackThreads, 0, st>>>((const uint16_t*)a.h, a.h_stride, a.labels, (int)a.rows, a.vocab, a.ignore,
-                                                          a.index, a.label, a.count, a.inv, row_loss, a.report, (int)a.hidden,
-                                                          (uint16_t*)a.packed);
+    lce_scan_pack_kernel<<<blocks, kPackThreads, 0, st>>>(k, a.labels, (int)a.rows, a.vocab, a.ignore, a.index, a.label, a.count, a.inv,
+                                                          row_loss, a.report);
   } else {
     count_launch(2);
     lce_scan_kernel<<<1, kScanThreads, 0, st>>>(a.labels, a.rows, a.vocab, a.ignore, a.index, a.label, a.count, a.inv, row_loss,
                                                 a.report);
-    lce_pack_kernel<<<blocks, kPackThreads, 0, st>>>((const uint16_t*)a.h, a.h_stride, a.index, a.count, (int)a.hidden,
-                                                     (uint16_t*)a.packed);
+    lce_pack_kernel<<<blocks, kPackThreads, 0, st>>>(k, a.index, a.label, a.count);
   }
   cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess || (e = make_context_current()) != cudaSuccess) return e;
@@ -1061,8 +1161,7 @@ cudaError_t launch_lce_forward(const LceArgs& a, int reduction, float* part, flo
   common_params(p, a);
   p.words = (int)a.vocab;
   p.part = reinterpret_cast<float2*>(part);
-  p.picked = picked;
-  int parts = (int)(2 * tiles_of(a.vocab));
+  int parts = (int)tiles_of(a.vocab);
   if (a.rows <= kLceFewRows) {
     if (!encode(&p.a, a.w, a.hidden, a.vocab, a.w_stride, 128) ||
         !encode(&p.b, a.packed, a.hidden, p.padded, a.hidden, few_columns(a.rows)))
@@ -1077,7 +1176,7 @@ cudaError_t launch_lce_forward(const LceArgs& a, int reduction, float* part, flo
   if (e != cudaSuccess) return e;
   count_launch();
   lce_join_kernel<<<(unsigned)lce_sum_doubles(a.rows), kJoinThreads, 0, st>>>(
-      p.part, parts, a.rows, a.index, a.label, a.count, picked, a.inv, a.lse, reduction, sums, loss);
+      p.part, parts, a.rows, a.index, a.label, a.count, picked, a.inv, a.rest, a.miss, reduction, sums, loss);
   return cudaGetLastError();
 }
 
@@ -1111,16 +1210,16 @@ int lce_splits(int64_t rows, int64_t hidden, int64_t vocab, int64_t piece) {
 cudaError_t launch_lce_backward(const LceArgs& a, const LceGrad& g, cudaStream_t st) {
   if (!args_ok(a) || g.piece <= 0 || g.piece % kTile != 0 || g.splits < 1 || g.g == nullptr) return cudaErrorInvalidValue;
   if (g.gh == nullptr && g.gw == nullptr) return cudaSuccess;
-  if (g.d == nullptr || (g.gh != nullptr && g.acc == nullptr)) return cudaErrorInvalidValue;
+  if (g.d == nullptr || (g.gh != nullptr && g.acc == nullptr) || (g.gw != nullptr && g.scaled == nullptr)) return cudaErrorInvalidValue;
   cudaError_t e = make_context_current();
   if (e != cudaSuccess) return e;
   const int64_t pieces = lce_pieces(a.vocab, g.piece), pitch = lce_piece_pitch(a.vocab, g.piece);
   GemmParams p{};
   common_params(p, a);
-  p.lse = a.lse;
-  p.row_g = g.reduction == kLceNone ? g.g : nullptr;
+  p.rest = a.rest;
   GemmParams q{};
   common_params(q, a);
+  const float* const row_g = g.reduction == kLceNone ? g.g : nullptr;
   q.inv = g.reduction == kLceMean ? a.inv : nullptr;
   q.g = g.reduction == kLceNone ? nullptr : g.g;
   q.want_dh = g.gh != nullptr;
@@ -1128,6 +1227,12 @@ cudaError_t launch_lce_backward(const LceArgs& a, const LceGrad& g, cudaStream_t
   // Half of a tile would be products with zeros (2000 rows of 64, 5000 words: 19.6 us, so 18.0).
   q.narrow = a.hidden <= kTile / 2;
   q.splits = g.splits;
+  if (g.gw != nullptr) {
+    count_launch();
+    lce_scale_kernel<<<(unsigned)(p.padded / kPackRows), kPackThreads, 0, st>>>((const uint16_t*)a.packed, a.index, a.count, a.miss, row_g,
+                                                                                (int)a.hidden, (uint16_t*)g.scaled);
+    if ((e = cudaGetLastError()) != cudaSuccess) return e;
+  }
   // few rows: `few` has the operands of dh, q those of dW alone
   const bool is_few = a.rows <= kLceFewRows;
   const int columns = few_columns(a.rows);
@@ -1137,7 +1242,7 @@ cudaError_t launch_lce_backward(const LceArgs& a, const LceGrad& g, cudaStream_t
   p.pitch = pitch;
   if (!encode(is_few ? &p.b : &p.a, a.packed, a.hidden, p.padded, a.hidden, is_few ? columns : 128) ||
       !encode(is_few ? &p.a : &p.b, a.w, a.hidden, a.vocab, a.w_stride, 128) ||
-      !encode(is_few ? &few.a : &q.b, a.w, a.hidden, a.vocab, a.w_stride, 64) || !encode(&q.b2, a.packed, a.hidden, p.padded, a.hidden, 64) ||
+      !encode(is_few ? &few.a : &q.b, a.w, a.hidden, a.vocab, a.w_stride, 64) || (q.want_dw && !encode(&q.b2, g.scaled, a.hidden, p.padded, a.hidden, 64)) ||
       (q.want_dw && !encode(&q.out, g.gw, a.hidden, a.vocab, a.hidden, 32, 32)) ||
       (q.want_dh && !encode_acc(&q.out_acc, g.acc, a.hidden, p.padded, g.splits)))
     return cudaErrorInvalidValue;
@@ -1165,7 +1270,7 @@ cudaError_t launch_lce_backward(const LceArgs& a, const LceGrad& g, cudaStream_t
   if (g.gh != nullptr) {
     count_launch();
     lce_join_grad_kernel<<<dim3((unsigned)a.rows, (unsigned)((a.hidden + 1023) / 1024)), 128, 0, st>>>(
-        g.acc, g.splits, p.padded, a.index, a.labels, a.ignore, a.count, (int)a.hidden, q.inv, q.g, (uint16_t*)g.gh);
+        g.acc, g.splits, p.padded, a.index, a.labels, a.ignore, a.count, (int)a.hidden, a.miss, q.inv, q.g, row_g, (uint16_t*)g.gh);
     e = cudaGetLastError();
   }
   return e;

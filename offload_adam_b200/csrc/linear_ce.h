@@ -23,7 +23,8 @@ struct LceArgs {
   int* label = nullptr;              // (rows,) label of the packed row, -1: outside the vocabulary
   int* count = nullptr;              // [0] packed rows, [1] ticket
   float* inv = nullptr;              // 1 / max(1, packed rows)
-  float* lse = nullptr;              // (rows,) of the packed row
+  float* rest = nullptr;             // (rows,) log-sum-exp of the packed row without its label
+  float* miss = nullptr;             // (rows,) 1 - probability of its label
   void* packed = nullptr;            // bf16 (rows padded, hidden)
   int64_t* report = nullptr;         // host memory: [0] a label past the vocabulary, [1] a wait that gave up, [2] a negative label
 };
@@ -47,6 +48,7 @@ struct LceGrad {
   void* gw = nullptr;         // bf16 (vocab, hidden) contiguous, or null
   int64_t piece = 0;          // words at a time, a multiple of kLceTile
   void* d = nullptr;          // bf16 (padded rows, lce_piece_pitch)
+  void* scaled = nullptr;     // bf16 (padded rows, hidden), for gw
   int splits = 1;             // of the sum over the words in gh
   float* acc = nullptr;       // fp32 (splits, padded rows, hidden), for gh
 };

@@ -27,9 +27,9 @@ Tensor rows_layout(const Tensor& t) {
 }
 int64_t row_stride(const Tensor& t) { return t.size(0) == 1 ? t.size(1) : t.stride(0); }
 
-// What backward needs of forward, in one int32 tensor: index, label and lse of the packed rows,
-// their number with the ticket, 1 / number.
-int64_t kept_words(int64_t rows) { return 3 * rows + 4; }
+// What backward needs of forward, in one int32 tensor: index, label, rest and miss of the packed
+// rows, their number with the ticket, 1 / number.
+int64_t kept_words(int64_t rows) { return 4 * rows + 4; }
 oab::LceArgs make_args(const Tensor& w, const Tensor& labels, const Tensor& kept, int64_t ignore, const Tensor& packed) {
   oab::LceArgs a;
   a.w = w.data_ptr();
@@ -42,9 +42,10 @@ oab::LceArgs make_args(const Tensor& w, const Tensor& labels, const Tensor& kept
   int* k = kept.data_ptr<int>();
   a.index = k;
   a.label = k + a.rows;
-  a.lse = reinterpret_cast<float*>(k + 2 * a.rows);
-  a.count = k + 3 * a.rows;
-  a.inv = reinterpret_cast<float*>(k + 3 * a.rows + 2);
+  a.rest = reinterpret_cast<float*>(k + 2 * a.rows);
+  a.miss = reinterpret_cast<float*>(k + 3 * a.rows);
+  a.count = k + 4 * a.rows;
+  a.inv = reinterpret_cast<float*>(k + 4 * a.rows + 2);
   a.packed = packed.data_ptr();
   a.report = oab::loss_report();
   return a;
@@ -125,6 +126,7 @@ struct LinearCE : torch::autograd::Function<LinearCE> {
     Scratch t;
     const int64_t d = t.add(2 * oab::lce_padded(rows) * oab::lce_piece_pitch(vocab, piece));
     const int64_t acc = t.add(want_h ? 4 * x.splits * oab::lce_padded(rows) * hidden : 0);
+    const int64_t scaled = t.add(want_w ? 2 * oab::lce_padded(rows) * hidden : 0);
     t.take(w);
     x.d = t.at_byte<void>(d);
     if (want_h) {
@@ -135,6 +137,7 @@ struct LinearCE : torch::autograd::Function<LinearCE> {
     if (want_w) {
       gw = at::empty({vocab, hidden}, w.options());
       x.gw = gw.data_ptr();
+      x.scaled = t.at_byte<void>(scaled);
     }
     ok(oab::launch_lce_backward(make_args(wc, lc, kept, ignore, packed), x, cur()), "linear_cross_entropy backward");
     if (graph) {

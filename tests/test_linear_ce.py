@@ -59,14 +59,16 @@ def _exact(h, w, labels, g, reduction, ignore=-100):
     gh[rows] = d @ w
     gw = d.T @ x
     result = {"none": losses, "sum": losses.sum(), "mean": losses.sum() / max(1, len(rows))}[reduction]
-    # each entry of d and the result round to bf16, by up to 2^-8 of their value; an error of e in
-    # a logit is one of e in d relative to p = d + [label], and of 4 e with the sum's
+    # each entry of d and the result round to bf16, by up to 2^-8 of their value, and so do the rows
+    # of h, times 1 - p and g, that go into gw; an error of e in a logit is one of e in d relative
+    # to p = d + [label], and of 4 e with the sum's
     e = _logit_error(h.shape[1], z)
     p = (d.abs() + torch.zeros_like(d).index_put_((at, lab), scale.abs().expand(len(rows)))) * 4 * e
     off = 2.0 ** -8 * d.abs() + p
     tol_h = torch.zeros_like(h)
     tol_h[rows] = off @ w.abs()
-    return result, gh, gw, tol_h + 2.0 ** -8 * gh.abs() + 1e-30, off.T @ x.abs() + 2.0 ** -8 * gw.abs() + 1e-30
+    return result, gh, gw, tol_h + 2.0 ** -8 * gh.abs() + 1e-30, \
+        (off + 2.0 ** -8 * (1 + 2.0 ** -8) * d.abs()).T @ x.abs() + 2.0 ** -8 * gw.abs() + 1e-30
 
 
 def _logit_error(hidden, z):
