@@ -70,6 +70,10 @@ struct GemmParams {
   float2* part;
   // kLogitGrad
   const float* rest;
+  const float *miss, *row_g;  // the latter by row, or null
+  const int* index;
+  const uint16_t* packed;
+  uint16_t* scaled;           // null: not wanted (again)
   uint16_t* d;           // few rows
   int64_t pitch;
   // kGrads
@@ -188,7 +192,8 @@ struct Plan {
 // tile, and every other tile of its pair.  A warp is a chain of latencies (the accumulator is
 // done, its load, a fence, the way out), so there are eight for each accumulator, and the accumulator
 // is given back (`release`) with the last load from it, before anything is computed from that.
-// Of the statistics: all sixteen take 64 columns of every tile, chain by chain.
+// Of the statistics likewise, unless the sums come in several chains: then all sixteen take 64 columns
+// of every tile.  (4096 rows of 128, 32000 words: 55 us by halves, 78 all together.)
 
 struct RowValues {  // of the packed row that a thread has in a tile
   int label;
@@ -221,13 +226,9 @@ __device__ __forceinline__ float2 stats_of(float (&v)[64], int col, int words, i
   for (int i = 0; i < 64; ++i) t[i & 3] = __fadd_rn(t[i & 3], exp_of(__fsub_rn(v[i], sh)));
   return make_float2(m, __fadd_rn(__fadd_rn(t[0], t[1]), __fadd_rn(t[2], t[3])));
 }
-__device__ __forceinline__ float2 join4(const float2* a, int stride) {
-  const float2 w[4] = {a[0], a[stride], a[2 * stride], a[3 * stride]};
-  const float m = fmaxf(fmaxf(w[0].x, w[1].x), fmaxf(w[2].x, w[3].x)), sh = finite_shift(m);
-  float s = 0.f;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) s = __fadd_rn(s, __fmul_rn(w[i].y, exp_of(__fsub_rn(w[i].x, sh))));
-  return make_float2(m, s);
+__device__ __forceinline__ float2 join2(const float2& a, const float2& b) {
+  const float m = fmaxf(a.x, b.x), sh = finite_shift(m);
+  return make_float2(m, __fadd_rn(__fmul_rn(a.y, exp_of(__fsub_rn(a.x, sh))), __fmul_rn(b.y, exp_of(__fsub_rn(b.x, sh)))));
 }
 
 // A warp's 32 lines of 64 bytes leave through its staging buffer, 16-byte parts swizzled as TMA
@@ -249,6 +250,27 @@ __device__ __forceinline__ void stage_bf16(uint32_t staging, int lane, const flo
                f32x2_to_bf16x2_rne(v[8 * c + 4], v[8 * c + 5]), f32x2_to_bf16x2_rne(v[8 * c + 6], v[8 * c + 7]));
   store_fence();
   __syncwarp();
+}
+
+// scaled[k] = packed[k] (1 - p_label) g, the rows of h as dW takes them, rounded to bf16; padded with
+// zeros likewise.  The epilogue warps of the gradient of the logits do it while the first products
+// run: the `mine`-th of `all` warps.
+__device__ __forceinline__ void scale_rows(const GemmParams& p, int n_rows, int mine, int all) {
+  const int vecs = p.hidden >> 3, lane = threadIdx.x & 31;
+  for (int k = mine; k < (n_rows + kLceRowPad - 1) / kLceRowPad * kLceRowPad; k += all) {
+    float c = k < n_rows ? p.miss[k] : 0.f;
+    if (k < n_rows && p.row_g != nullptr) c = __fmul_rn(c, p.row_g[p.index[k]]);
+    const uint4* from = reinterpret_cast<const uint4*>(p.packed + (int64_t)k * p.hidden);  // zeros beyond n_rows
+    uint4* to = reinterpret_cast<uint4*>(p.scaled + (int64_t)k * p.hidden);
+    auto both = [c](uint32_t w) {
+      return f32x2_to_bf16x2_rne(__fmul_rn(__uint_as_float(w << 16), c), __fmul_rn(__uint_as_float(w & 0xffff0000u), c));
+    };
+#pragma unroll 4
+    for (int v = lane; v < vecs; v += 32) {
+      const uint4 f = from[v];
+      to[v] = make_uint4(both(f.x), both(f.y), both(f.z), both(f.w));
+    }
+  }
 }
 
 template <class Release>
@@ -334,22 +356,23 @@ lce_product_kernel(const __grid_constant__ GemmParams p) {
   __shared__ uint32_t tmem_at;
   __shared__ int gave_up;
   __shared__ float2 row_part[PASS == kStats ? 2 : 1][4][PASS == kStats ? 128 : 1];  // by turn, columns and row
-  __shared__ volatile int stop[4][2];  // of the epilogue warps of the same 32 rows, by turn
+  __shared__ volatile int stop[8][2];  // of two epilogue warps of the same 32 rows, by turn
   const uint32_t stages = (smem_addr(smem_raw) + 1023u) & ~1023u;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = cluster_rank();
   const uint32_t full0 = smem_addr(full), empty0 = smem_addr(empty), done0 = smem_addr(done), drained0 = smem_addr(drained);
+  const bool chained = p.hidden > kChain * kInner;  // the statistics' sums
 
   if (threadIdx.x == 0) {
     gave_up = 0;
-    for (int i = 0; i < 8; ++i) stop[i >> 1][i & 1] = 0;
+    for (int i = 0; i < 16; ++i) stop[i >> 1][i & 1] = 0;
     for (int i = 0; i < kStages; ++i) {
       mbar_init(full0 + 8 * i, 1);
       mbar_init(empty0 + 8 * i, 1);
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(done0 + 8 * i, 1);
-      mbar_init(drained0 + 8 * i, PASS == kStats ? 2 * kEpilogueWarps : kEpilogueWarps);  // of both CTAs
+      mbar_init(drained0 + 8 * i, PASS == kStats && chained ? 2 * kEpilogueWarps : kEpilogueWarps);  // of both CTAs
     }
     mbar_init_fence();
     prefetch_map(&p.a);
@@ -443,8 +466,9 @@ lce_product_kernel(const __grid_constant__ GemmParams p) {
       }
     }
     __syncwarp();
-  } else if constexpr (PASS == kStats) {
-    const int quarter = warp & 3, part = (warp - 2) >> 2, in_cta = quarter * 32 + lane;
+  } else if (PASS == kStats && chained) {
+    // warps 2 to 17: four rows of 32, four of 64 columns; the sums of a tile stay in registers
+    const int quarter = warp & 3, part = (warp - 2) >> 2, in_cta = quarter * 32 + lane, mates = quarter + (part >> 1) * 4;
     const uint32_t lead_drained0 = map_to_rank(drained0, 0);
     int chains = 0;
     for (int mine = 0, t; (t = plan.pick<PASS>(pair, mine)) >= 0; ++mine) {
@@ -473,14 +497,15 @@ lce_product_kernel(const __grid_constant__ GemmParams p) {
         __syncwarp();
         if (lane == 0) mbar_arrive_cluster(lead_drained0 + 8 * acc);
       }
-      // The four warps of these rows join.  One that gave up comes here, too, and they all leave:
-      // what belongs to a turn is written again two turns later, when they have met once more.
+      // The two warps of these rows and 128 columns join.  One that gave up comes here, too, and both
+      // leave: what belongs to a turn is written again two turns later, when they have met once more.
       if (ok) row_part[turn][part][in_cta] = stats_of(v, x.n + part * 64, p.words, values.label);
-      else stop[quarter][turn] = 1;
-      asm volatile("bar.sync %0, 128;" ::"r"(1 + quarter) : "memory");
-      ok = stop[quarter][turn] == 0;
+      else stop[mates][turn] = 1;
+      asm volatile("bar.sync %0, 64;" ::"r"(1 + mates) : "memory");
+      ok = stop[mates][turn] == 0;
       if (!ok) break;
-      if (part == 0 && row < n_rows) p.part[(int64_t)(x.n / kTile) * p.rows + row] = join4(&row_part[turn][0][in_cta], 128);
+      if ((part & 1) == 0 && row < n_rows)
+        p.part[(int64_t)(x.n / 128 + (part >> 1)) * p.rows + row] = join2(row_part[turn][part][in_cta], row_part[turn][part + 1][in_cta]);
     }
   } else {
     const int quarter = warp & 3, half = ((warp - 2) >> 2) & 1, group = (warp - 2) >> 3;
@@ -491,6 +516,7 @@ lce_product_kernel(const __grid_constant__ GemmParams p) {
       if (p.g != nullptr) scale = __fmul_rn(scale, *p.g);
     }
     const uint32_t staging = stages + kStages * kStageBytes + (warp - 2) * kStagingBytes;
+    if (PASS == kLogitGrad && p.scaled != nullptr) scale_rows(p, n_rows, blockIdx.x * kEpilogueWarps + warp - 2, gridDim.x * kEpilogueWarps);
     for (int mine = group, t; (t = plan.pick<PASS>(pair, mine)) >= 0; mine += 2) {
       const Tile x = plan.at<PASS>(p, t);
       const uint32_t acc = group;
@@ -506,11 +532,22 @@ lce_product_kernel(const __grid_constant__ GemmParams p) {
         __syncwarp();
         if (lane == 0) mbar_arrive_cluster(lead_drained0 + 8 * acc);
       };
+      if (PASS == kStats) {
+        float2 both[2];
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          float v[64];
+          tmem_load64(at + c * 64, v);
+          if (c == 1) release();
+          both[c] = stats_of(v, x.n + half * 128 + c * 64, p.words, values.label);
+        }
+        if (row < n_rows) p.part[(int64_t)(x.n / 128 + half) * p.rows + row] = join2(both[0], both[1]);
+      }
       if (PASS == kLogitGrad) logit_grad_tile(p, x, at, row, half, staging, lane, values, release);
       if (PASS == kGrads && x.kind == 0) dh_tile(p, x, at, row, n_rows, half, staging, lane, release);
       if (PASS == kGrads && x.kind == 1) dw_tile(p, x, at, row, half, scale, staging, lane, release);
     }
-    if (lane == 0) store_wait();
+    if (PASS != kStats && lane == 0) store_wait();
     __syncwarp();
   }
   if (!ok) gave_up = 1;
@@ -533,7 +570,7 @@ constexpr int kFewThreads = 64 + 128;
 template <int N>
 struct FewShape {
   static constexpr int kStage = kHalfBytes + N * 128, kCount = (220 * 1024) / kStage, kSmem = kCount * kStage + 1024;
-  static constexpr int kAccs = 4, kColumns = kAccs * N;  // accumulators in tensor memory
+  static constexpr int kAccs = 8, kColumns = kAccs * N;  // accumulators in tensor memory
 };
 constexpr int kFewChain = 2;  // stages
 template <int N>
@@ -663,6 +700,7 @@ lce_few_kernel(const __grid_constant__ GemmParams p, float* acc) {
   } else {
     const int quarter = warp & 3;
     int chains = 0;
+    if (PASS == kLogitGrad && p.scaled != nullptr) scale_rows(p, n_rows, blockIdx.x * 4 + warp - 2, gridDim.x * 4);
     for (int t = blockIdx.x; t < total; t += gridDim.x) {
       int first;
       const int steps = share(t, first), m = t % across * 128, length = PASS == kStats ? kFewChain : steps;
@@ -714,7 +752,7 @@ lce_few_kernel(const __grid_constant__ GemmParams p, float* acc) {
         if (!ok) break;
         const int r = threadIdx.x - 64;
         if (r < n_rows) {
-          p.part[(int64_t)(m / 128) * p.rows + r] = join4(&warp_part[0][r], N);
+          p.part[(int64_t)(m / 128) * p.rows + r] = join2(join2(warp_part[0][r], warp_part[1][r]), join2(warp_part[2][r], warp_part[3][r]));
         }
         asm volatile("bar.sync 1, 128;" ::: "memory");  // before warp_part is written again
       } else if (PASS == kLogitGrad) {
@@ -797,7 +835,7 @@ lce_scan_kernel(const int64_t* __restrict__ labels, int64_t rows, int64_t vocab,
 }
 
 // packed[k] = h[index[k]], zero rows up to the next multiple of kLceRowPad, and the logit of its
-// label.  A warp a row.
+// label.  THREADS a row: a warp, or a block where there are few rows (32 of 8192: 20 us with a warp).
 constexpr int kPackThreads = 256, kPackRows = kPackThreads / 32;
 struct PackArgs {
   const uint16_t* h;
@@ -813,15 +851,16 @@ __device__ __forceinline__ float dot2(uint32_t a, uint32_t b, float c) {  // of 
   return __fmaf_rn(__uint_as_float(a & 0xffff0000u), __uint_as_float(b & 0xffff0000u), c);
 }
 // n: how many rows are packed; `row`, `label`: of packed row k < n
+template <int THREADS>
 __device__ __forceinline__ void pack_row(const PackArgs& a, int64_t k, int n, int row, int label) {
-  const int vecs = a.hidden >> 3, lane = threadIdx.x & 31;
+  const int vecs = a.hidden >> 3, lane = threadIdx.x % THREADS;
   uint4* to = reinterpret_cast<uint4*>(a.packed + k * a.hidden);
   if (k < n) {
     const uint4* from = reinterpret_cast<const uint4*>(a.h + row * a.h_stride);
     const uint4* word = reinterpret_cast<const uint4*>(a.w + (label < 0 ? 0 : label) * a.w_stride);
     float x[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 4
-    for (int v = lane; v < vecs; v += 32) {
+    for (int v = lane; v < vecs; v += THREADS) {
       const uint4 f = from[v], g = word[v];
       to[v] = f;
       x[0] = dot2(f.x, g.x, x[0]);
@@ -830,33 +869,40 @@ __device__ __forceinline__ void pack_row(const PackArgs& a, int64_t k, int n, in
       x[3] = dot2(f.w, g.w, x[3]);
     }
     float z = __fadd_rn(__fadd_rn(x[0], x[1]), __fadd_rn(x[2], x[3]));
+    if constexpr (THREADS == 32) {
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) z = __fadd_rn(z, __shfl_xor_sync(0xffffffffu, z, o));
+      for (int o = 16; o > 0; o >>= 1) z = __fadd_rn(z, __shfl_xor_sync(0xffffffffu, z, o));
+    } else {  // k is the whole block's
+      __shared__ float red[THREADS / 32];
+      z = block_sum<THREADS>(z, red);
+    }
     if (lane == 0) a.picked[k] = z;
   } else if (k < (n + kLceRowPad - 1) / kLceRowPad * kLceRowPad) {
-    for (int v = lane; v < vecs; v += 32) to[v] = make_uint4(0, 0, 0, 0);
+    for (int v = lane; v < vecs; v += THREADS) to[v] = make_uint4(0, 0, 0, 0);
   }
 }
 __global__ void __launch_bounds__(kPackThreads)
 lce_pack_kernel(const PackArgs a, const int* __restrict__ index, const int* __restrict__ label, const int* __restrict__ count) {
   const int64_t k = (int64_t)blockIdx.x * kPackRows + (threadIdx.x >> 5);
   const int n = *count;
-  pack_row(a, k, n, k < n ? index[k] : 0, k < n ? label[k] : 0);
+  pack_row<32>(a, k, n, k < n ? index[k] : 0, k < n ? label[k] : 0);
 }
 
 // Both in one launch for up to kScanPackRows rows: every block looks through all labels (32 KB at
 // most, from L2) for the eight rows that it packs.  One row: 13 -> 7 us for the two.
-constexpr int kScanPackRows = 4096, kScanPackEach = kScanPackRows / kPackThreads;
+constexpr int kScanPackRows = 4096, kScanPackBlockRows = 512;  // the latter: a block a row
+template <int THREADS>
 __global__ void __launch_bounds__(kPackThreads)
 lce_scan_pack_kernel(const PackArgs a, const int64_t* __restrict__ labels, int rows, int64_t vocab, int64_t ignore, int* index,
                      int* label, int* count, float* inv, float* row_loss, volatile int64_t* bad) {
-  __shared__ int warps[kPackThreads / 32], source[kPackRows], source_label[kPackRows];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, first = blockIdx.x * kPackRows;
+  constexpr int kOwn = kPackThreads / THREADS, kEach = (THREADS == 32 ? kScanPackRows : kScanPackBlockRows) / kPackThreads;
+  __shared__ int warps[kPackThreads / 32], source[kOwn], source_label[kOwn];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, first = blockIdx.x * kOwn;
   const int each = (rows + kPackThreads - 1) / kPackThreads, r0 = threadIdx.x * each;
-  int64_t lab[kScanPackEach];
+  int64_t lab[kEach];
   int c = 0;
 #pragma unroll
-  for (int i = 0; i < kScanPackEach; ++i) {
+  for (int i = 0; i < kEach; ++i) {
     lab[i] = i < each && r0 + i < rows ? labels[r0 + i] : ignore;
     c += lab[i] != ignore;
   }
@@ -867,7 +913,7 @@ lce_scan_pack_kernel(const PackArgs a, const int64_t* __restrict__ labels, int r
     if (lane >= o) x += y;
   }
   if (lane == 31) warps[warp] = x;
-  if (threadIdx.x < kPackRows) source[threadIdx.x] = source_label[threadIdx.x] = 0;
+  if (threadIdx.x < kOwn) source[threadIdx.x] = source_label[threadIdx.x] = 0;
   __syncthreads();
   int k = x - c, n = 0;
 #pragma unroll
@@ -876,17 +922,17 @@ lce_scan_pack_kernel(const PackArgs a, const int64_t* __restrict__ labels, int r
     n += warps[w];
   }
 #pragma unroll
-  for (int i = 0; i < kScanPackEach; ++i) {
+  for (int i = 0; i < kEach; ++i) {
     const int r = r0 + i;
     if (lab[i] != ignore) {
-      if (k >= first && k < first + kPackRows) {
+      if (k >= first && k < first + kOwn) {
         const bool known = lab[i] >= 0 && lab[i] < vocab;
         if (!known) bad[lab[i] < 0 ? 2 : 0] = lab[i];
         source[k - first] = index[k] = r;
         source_label[k - first] = label[k] = known ? (int)lab[i] : -1;
       }
       ++k;
-    } else if (row_loss != nullptr && r >= first && r < first + kPackRows && i < each && r < rows) {
+    } else if (row_loss != nullptr && r >= first && r < first + kOwn && i < each && r < rows) {
       row_loss[r] = 0.f;
     }
   }
@@ -896,28 +942,8 @@ lce_scan_pack_kernel(const PackArgs a, const int64_t* __restrict__ labels, int r
     *inv = __fdiv_rn(1.f, (float)(n < 1 ? 1 : n));
   }
   __syncthreads();
-  pack_row(a, first + warp, n, source[warp], source_label[warp]);
-}
-
-// scaled[k] = packed[k] (1 - p_label) g, the rows of h as dW takes them; padded likewise.
-__global__ void __launch_bounds__(kPackThreads)
-lce_scale_kernel(const uint16_t* __restrict__ packed, const int* __restrict__ index, const int* __restrict__ count,
-                 const float* __restrict__ miss, const float* __restrict__ row_g, int hidden, uint16_t* scaled) {
-  const int64_t k = (int64_t)blockIdx.x * kPackRows + (threadIdx.x >> 5);
-  const int n = *count, vecs = hidden >> 3, lane = threadIdx.x & 31;
-  if (k >= (n + kLceRowPad - 1) / kLceRowPad * kLceRowPad) return;
-  float c = k < n ? miss[k] : 0.f;
-  if (k < n && row_g != nullptr) c = __fmul_rn(c, row_g[index[k]]);
-  const uint4* from = reinterpret_cast<const uint4*>(packed + k * hidden);  // zeros beyond n
-  uint4* to = reinterpret_cast<uint4*>(scaled + k * hidden);
-  auto both = [c](uint32_t w) {
-    return f32x2_to_bf16x2_rne(__fmul_rn(__uint_as_float(w << 16), c), __fmul_rn(__uint_as_float(w & 0xffff0000u), c));
-  };
-#pragma unroll 4
-  for (int v = lane; v < vecs; v += 32) {
-    const uint4 f = from[v];
-    to[v] = make_uint4(both(f.x), both(f.y), both(f.z), both(f.w));
-  }
+  const int own = threadIdx.x / THREADS;
+  pack_row<THREADS>(a, first + own, n, source[own], source_label[own]);
 }
 
 // ------------------------------------------------------------ joining the sums
@@ -1135,7 +1161,7 @@ void common_params(GemmParams& p, const LceArgs& a) {
 }  // namespace
 
 int64_t lce_part_floats(int64_t rows, int64_t vocab) {
-  return 2 * rows * (rows <= kLceFewRows ? (vocab + 127) / 128 : tiles_of(vocab));
+  return 2 * rows * (rows <= kLceFewRows ? (vocab + 127) / 128 : 2 * tiles_of(vocab));
 }
 int64_t lce_sum_doubles(int64_t rows) { return (rows + kJoinRows - 1) / kJoinRows; }
 
@@ -1145,10 +1171,14 @@ cudaError_t launch_lce_forward(const LceArgs& a, int reduction, float* part, flo
   float* const row_loss = reduction == kLceNone ? loss : nullptr;
   const unsigned blocks = (unsigned)(lce_padded(a.rows) / kPackRows);
   const PackArgs k{(const uint16_t*)a.h, a.h_stride, (const uint16_t*)a.w, a.w_stride, (int)a.hidden, (uint16_t*)a.packed, picked};
-  if (a.rows <= kScanPackRows) {
+  if (a.rows <= kScanPackBlockRows) {
     count_launch();
-    lce_scan_pack_kernel<<<blocks, kPackThreads, 0, st>>>(k, a.labels, (int)a.rows, a.vocab, a.ignore, a.index, a.label, a.count, a.inv,
-                                                          row_loss, a.report);
+    lce_scan_pack_kernel<kPackThreads><<<(unsigned)lce_padded(a.rows), kPackThreads, 0, st>>>(
+        k, a.labels, (int)a.rows, a.vocab, a.ignore, a.index, a.label, a.count, a.inv, row_loss, a.report);
+  } else if (a.rows <= kScanPackRows) {
+    count_launch();
+    lce_scan_pack_kernel<32><<<blocks, kPackThreads, 0, st>>>(k, a.labels, (int)a.rows, a.vocab, a.ignore, a.index, a.label, a.count,
+                                                              a.inv, row_loss, a.report);
   } else {
     count_launch(2);
     lce_scan_kernel<<<1, kScanThreads, 0, st>>>(a.labels, a.rows, a.vocab, a.ignore, a.index, a.label, a.count, a.inv, row_loss,
@@ -1161,7 +1191,7 @@ cudaError_t launch_lce_forward(const LceArgs& a, int reduction, float* part, flo
   common_params(p, a);
   p.words = (int)a.vocab;
   p.part = reinterpret_cast<float2*>(part);
-  int parts = (int)tiles_of(a.vocab);
+  int parts = (int)(2 * tiles_of(a.vocab));
   if (a.rows <= kLceFewRows) {
     if (!encode(&p.a, a.w, a.hidden, a.vocab, a.w_stride, 128) ||
         !encode(&p.b, a.packed, a.hidden, p.padded, a.hidden, few_columns(a.rows)))
@@ -1217,9 +1247,13 @@ cudaError_t launch_lce_backward(const LceArgs& a, const LceGrad& g, cudaStream_t
   GemmParams p{};
   common_params(p, a);
   p.rest = a.rest;
+  p.miss = a.miss;
+  p.row_g = g.reduction == kLceNone ? g.g : nullptr;
+  p.index = a.index;
+  p.packed = (const uint16_t*)a.packed;
+  p.scaled = g.gw != nullptr ? (uint16_t*)g.scaled : nullptr;
   GemmParams q{};
   common_params(q, a);
-  const float* const row_g = g.reduction == kLceNone ? g.g : nullptr;
   q.inv = g.reduction == kLceMean ? a.inv : nullptr;
   q.g = g.reduction == kLceNone ? nullptr : g.g;
   q.want_dh = g.gh != nullptr;
@@ -1227,12 +1261,6 @@ cudaError_t launch_lce_backward(const LceArgs& a, const LceGrad& g, cudaStream_t
   // Half of a tile would be products with zeros (2000 rows of 64, 5000 words: 19.6 us, so 18.0).
   q.narrow = a.hidden <= kTile / 2;
   q.splits = g.splits;
-  if (g.gw != nullptr) {
-    count_launch();
-    lce_scale_kernel<<<(unsigned)(p.padded / kPackRows), kPackThreads, 0, st>>>((const uint16_t*)a.packed, a.index, a.count, a.miss, row_g,
-                                                                                (int)a.hidden, (uint16_t*)g.scaled);
-    if ((e = cudaGetLastError()) != cudaSuccess) return e;
-  }
   // few rows: `few` has the operands of dh, q those of dW alone
   const bool is_few = a.rows <= kLceFewRows;
   const int columns = few_columns(a.rows);
@@ -1263,6 +1291,7 @@ cudaError_t launch_lce_backward(const LceArgs& a, const LceGrad& g, cudaStream_t
         return cudaErrorInvalidValue;
       if ((e = launch_product<kLogitGrad>(p, tiles_of(a.rows) * tiles_of(p.words), st)) != cudaSuccess) return e;
     }
+    p.scaled = nullptr;  // the first piece has done it
     const int64_t dh = q.want_dh ? tiles_of(a.rows) * tiles_of(a.hidden) * g.splits : 0;
     const int64_t dw = q.want_dw ? tiles_of(q.words) * tiles_of(a.hidden) : 0;
     if ((e = launch_product<kGrads>(q, dh + dw, st)) != cudaSuccess) return e;
@@ -1270,7 +1299,7 @@ cudaError_t launch_lce_backward(const LceArgs& a, const LceGrad& g, cudaStream_t
   if (g.gh != nullptr) {
     count_launch();
     lce_join_grad_kernel<<<dim3((unsigned)a.rows, (unsigned)((a.hidden + 1023) / 1024)), 128, 0, st>>>(
-        g.acc, g.splits, p.padded, a.index, a.labels, a.ignore, a.count, (int)a.hidden, a.miss, q.inv, q.g, row_g, (uint16_t*)g.gh);
+        g.acc, g.splits, p.padded, a.index, a.labels, a.ignore, a.count, (int)a.hidden, a.miss, q.inv, q.g, p.row_g, (uint16_t*)g.gh);
     e = cudaGetLastError();
   }
   return e;
