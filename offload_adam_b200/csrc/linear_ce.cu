@@ -15,7 +15,7 @@
 // so the label's entry, which most of a row's gradient hangs on, is -1 exactly in bf16; q_i g_i is
 // applied to the fp32 sums of dh, and to the rows of h that go into dW.  tcgen05 cuts off what it adds to an accumulator (about half a unit, 2^-24, towards zero
 // each time: logits of 4096 terms came out 1.5e-5 too small, losses 2.5e-5 off), so the statistics
-// take their logits in chains of 32 additions (512 terms; 8 for few rows) that the epilogue adds up.
+// take their logits in chains of 32 additions (512 terms; 16 for few rows) that the epilogue adds up.
 //
 // Forward: one product whose epilogue keeps, per row and 128 words, the maximum and the sum of
 // exponentials (8 bytes for 256 bytes of bf16 logits), and a small kernel that joins them.
@@ -572,7 +572,9 @@ struct FewShape {
   static constexpr int kStage = kHalfBytes + N * 128, kCount = (220 * 1024) / kStage, kSmem = kCount * kStage + 1024;
   static constexpr int kAccs = 8, kColumns = kAccs * N;  // accumulators in tensor memory
 };
-constexpr int kFewChain = 2;  // stages
+// Stages of a chain of the statistics.  One row of 128256 words x 4096: 174 us without chains, 179 with
+// four stages, 186 with two; the loss of a confident row up to 25, 1.0 and 0.8e-6 off 64 bits.
+constexpr int kFewChain = 4;
 template <int N>
 __device__ __forceinline__ void tmem_load_rows(uint32_t at, float (&v)[N]) {
   if constexpr (N == 16) {
