@@ -29,6 +29,8 @@
 // takes tiles in turn.
 #include <cudaTypedefs.h>
 
+#include <atomic>
+
 #include "common.cuh"
 #include "linear_ce.h"
 #include "umma.cuh"
@@ -74,6 +76,9 @@ struct GemmParams {
   const int* index;
   const uint16_t* packed;
   uint16_t* scaled;           // null: not wanted (again)
+  uint16_t* gh;               // kLogitGrad: its ignored rows become zero; kGrads: dh goes out; null: neither
+  const int64_t* labels;
+  int64_t ignore;
   uint16_t* d;           // few rows
   int64_t pitch;
   // kGrads
@@ -252,11 +257,19 @@ __device__ __forceinline__ void stage_bf16(uint32_t staging, int lane, const flo
   __syncwarp();
 }
 
-// scaled[k] = packed[k] (1 - p_label) g, the rows of h as dW takes them, rounded to bf16; padded with
-// zeros likewise.  The epilogue warps of the gradient of the logits do it while the first products
-// run: the `mine`-th of `all` warps.
-__device__ __forceinline__ void scale_rows(const GemmParams& p, int n_rows, int mine, int all) {
+// What the epilogue warps of the gradient of the logits do while the first products run, the
+// `mine`-th of `all` warps: scaled[k] = packed[k] (1 - p_label) g, the rows of h as dW takes them,
+// rounded to bf16 and padded with zeros likewise; and the zero rows of gh.
+__device__ __forceinline__ void prepare_rows(const GemmParams& p, int n_rows, int mine, int all) {
   const int vecs = p.hidden >> 3, lane = threadIdx.x & 31;
+  if (p.gh != nullptr) {
+    for (int64_t r = mine; r < p.rows; r += all) {
+      if (p.labels[r] != p.ignore) continue;
+      uint4* to = reinterpret_cast<uint4*>(p.gh + r * p.hidden);
+      for (int v = lane; v < vecs; v += 32) to[v] = make_uint4(0, 0, 0, 0);
+    }
+  }
+  if (p.scaled == nullptr) return;
   for (int k = mine; k < (n_rows + kLceRowPad - 1) / kLceRowPad * kLceRowPad; k += all) {
     float c = k < n_rows ? p.miss[k] : 0.f;
     if (k < n_rows && p.row_g != nullptr) c = __fmul_rn(c, p.row_g[p.index[k]]);
@@ -300,15 +313,45 @@ __device__ __forceinline__ void logit_grad_tile(const GemmParams& p, const Tile&
   }
 }
 
+__device__ __forceinline__ void store_bf16x8(uint16_t* at, const float* v, float scale) {
+  uint4 o;
+  o.x = f32x2_to_bf16x2_rne(__fmul_rn(v[0], scale), __fmul_rn(v[1], scale));
+  o.y = f32x2_to_bf16x2_rne(__fmul_rn(v[2], scale), __fmul_rn(v[3], scale));
+  o.z = f32x2_to_bf16x2_rne(__fmul_rn(v[4], scale), __fmul_rn(v[5], scale));
+  o.w = f32x2_to_bf16x2_rne(__fmul_rn(v[6], scale), __fmul_rn(v[7], scale));
+  *reinterpret_cast<uint4*>(at) = o;
+}
+// What all rows of dh, and dW, are multiplied by.
+__device__ __forceinline__ float all_scale(const GemmParams& p) {
+  float scale = 1.f;
+  if (p.inv != nullptr) scale = *p.inv;
+  return p.g != nullptr ? __fmul_rn(scale, *p.g) : scale;
+}
+// What packed row k of dh is multiplied by, beside the scale of all rows.
+__device__ __forceinline__ float row_scale(const GemmParams& p, int k, float scale) {
+  scale = __fmul_rn(scale, p.miss[k]);
+  return p.row_g != nullptr ? __fmul_rn(scale, p.row_g[p.index[k]]) : scale;
+}
+
 template <class Release>
-__device__ __forceinline__ void dh_tile(const GemmParams& p, const Tile& x, uint32_t tmem, int row, int n_rows, int half,
+__device__ __forceinline__ void dh_tile(const GemmParams& p, const Tile& x, uint32_t tmem, int row, int n_rows, int half, float scale,
                                         uint32_t staging, int lane, const Release& release) {
+  uint16_t* out = nullptr;
+  if (p.gh != nullptr && row < n_rows) {  // one piece, one split: these are the whole sums
+    out = p.gh + (int64_t)p.index[row] * p.hidden;
+    scale = row_scale(p, row, scale);
+  }
 #pragma unroll 1
   for (int c = 0; c < 8; ++c) {
     float v[16];
     tmem_load16(tmem + c * 16, v);
     if (c == 7) release();
     const int col = x.n + half * 128 + c * 16;
+    if (p.gh != nullptr) {
+      if (out != nullptr && col < p.hidden) store_bf16x8(out + col, v, scale);
+      if (out != nullptr && col + 8 < p.hidden) store_bf16x8(out + col + 8, v + 8, scale);
+      continue;
+    }
     if (x.steps == 0) {  // a last piece of fewer stages than splits: nothing was summed
 #pragma unroll
       for (int i = 0; i < 16; ++i) v[i] = 0.f;
@@ -510,13 +553,9 @@ lce_product_kernel(const __grid_constant__ GemmParams p) {
   } else {
     const int quarter = warp & 3, half = ((warp - 2) >> 2) & 1, group = (warp - 2) >> 3;
     const uint32_t lead_drained0 = map_to_rank(drained0, 0);
-    float scale = 1.f;
-    if (PASS == kGrads) {
-      if (p.inv != nullptr) scale = *p.inv;
-      if (p.g != nullptr) scale = __fmul_rn(scale, *p.g);
-    }
+    const float scale = PASS == kGrads ? all_scale(p) : 1.f;
     const uint32_t staging = stages + kStages * kStageBytes + (warp - 2) * kStagingBytes;
-    if (PASS == kLogitGrad && p.scaled != nullptr) scale_rows(p, n_rows, blockIdx.x * kEpilogueWarps + warp - 2, gridDim.x * kEpilogueWarps);
+    if (PASS == kLogitGrad) prepare_rows(p, n_rows, blockIdx.x * kEpilogueWarps + warp - 2, gridDim.x * kEpilogueWarps);
     for (int mine = group, t; (t = plan.pick<PASS>(pair, mine)) >= 0; mine += 2) {
       const Tile x = plan.at<PASS>(p, t);
       const uint32_t acc = group;
@@ -544,7 +583,7 @@ lce_product_kernel(const __grid_constant__ GemmParams p) {
         if (row < n_rows) p.part[(int64_t)(x.n / 128 + half) * p.rows + row] = join2(both[0], both[1]);
       }
       if (PASS == kLogitGrad) logit_grad_tile(p, x, at, row, half, staging, lane, values, release);
-      if (PASS == kGrads && x.kind == 0) dh_tile(p, x, at, row, n_rows, half, staging, lane, release);
+      if (PASS == kGrads && x.kind == 0) dh_tile(p, x, at, row, n_rows, half, scale, staging, lane, release);
       if (PASS == kGrads && x.kind == 1) dw_tile(p, x, at, row, half, scale, staging, lane, release);
     }
     if (PASS != kStats && lane == 0) store_wait();
@@ -595,7 +634,8 @@ lce_few_kernel(const __grid_constant__ GemmParams p, float* acc) {
   __shared__ int gave_up;
   __shared__ volatile int stop;  // of the epilogue warps
   __shared__ int label_of[N];
-  __shared__ float rest_of[N];
+  __shared__ float rest_of[N], scale_of[N];
+  __shared__ int row_of[N];
   __shared__ float2 warp_part[4][N];
   const uint32_t stages = (smem_addr(smem_raw) + 1023u) & ~1023u;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -620,6 +660,11 @@ lce_few_kernel(const __grid_constant__ GemmParams p, float* acc) {
     const int r = threadIdx.x;
     label_of[r] = r < n_rows ? p.label[r] : -1;
     if (PASS == kLogitGrad) rest_of[r] = r < n_rows ? p.rest[r] : INFINITY;
+  }
+  if (PASS == kGrads && p.gh != nullptr && threadIdx.x < n_rows) {
+    const int r = threadIdx.x;
+    row_of[r] = p.index[r];
+    scale_of[r] = row_scale(p, r, all_scale(p));
   }
   if (warp == 1) tmem_alloc(smem_addr(&tmem_at), S::kColumns);
   fence_before();
@@ -702,7 +747,7 @@ lce_few_kernel(const __grid_constant__ GemmParams p, float* acc) {
   } else {
     const int quarter = warp & 3;
     int chains = 0;
-    if (PASS == kLogitGrad && p.scaled != nullptr) scale_rows(p, n_rows, blockIdx.x * 4 + warp - 2, gridDim.x * 4);
+    if (PASS == kLogitGrad) prepare_rows(p, n_rows, blockIdx.x * 4 + warp - 2, gridDim.x * 4);
     for (int t = blockIdx.x; t < total; t += gridDim.x) {
       int first;
       const int steps = share(t, first), m = t % across * 128, length = PASS == kStats ? kFewChain : steps;
@@ -767,6 +812,12 @@ lce_few_kernel(const __grid_constant__ GemmParams p, float* acc) {
             p.d[(int64_t)r * p.pitch + at] = (uint16_t)f32_to_bf16_rne_bits(d);
           }
           for (int r = N; r < kLceRowPad; ++r) p.d[(int64_t)r * p.pitch + at] = 0;
+        }
+      } else if (at < p.hidden && p.gh != nullptr) {  // one piece, one split: the whole sums
+#pragma unroll
+        for (int r = 0; r < N; ++r) {
+          if (r >= n_rows) break;
+          p.gh[(int64_t)row_of[r] * p.hidden + at] = (uint16_t)f32_to_bf16_rne_bits(__fmul_rn(v[r], scale_of[r]));
         }
       } else if (at < p.hidden) {
         float* to = acc + (int64_t)(t / across) * p.padded * p.hidden + at;
@@ -1036,14 +1087,6 @@ lce_join_kernel(const float2* __restrict__ part, int parts, int64_t rows, const 
 }
 
 // -------------------------------------------------- dh: splits joined, rounded
-__device__ __forceinline__ void store_bf16x8(uint16_t* at, const float* v, float scale) {
-  uint4 o;
-  o.x = f32x2_to_bf16x2_rne(__fmul_rn(v[0], scale), __fmul_rn(v[1], scale));
-  o.y = f32x2_to_bf16x2_rne(__fmul_rn(v[2], scale), __fmul_rn(v[3], scale));
-  o.z = f32x2_to_bf16x2_rne(__fmul_rn(v[4], scale), __fmul_rn(v[5], scale));
-  o.w = f32x2_to_bf16x2_rne(__fmul_rn(v[6], scale), __fmul_rn(v[7], scale));
-  *reinterpret_cast<uint4*>(at) = o;
-}
 // Rows whose label is ignored become zero.
 __global__ void __launch_bounds__(128)
 lce_join_grad_kernel(const float* __restrict__ acc, int splits, int64_t padded, const int* __restrict__ index,
@@ -1110,12 +1153,25 @@ bool encode(CUtensorMap* map, const void* base, int64_t inner, int64_t lines_all
             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+// Once for each kernel and device.
+cudaError_t allow_smem(std::atomic<uint64_t>& done, const void* kernel, int bytes) {
+  int device = 0;
+  cudaError_t e = cudaGetDevice(&device);
+  if (e != cudaSuccess) return e;
+  const uint64_t bit = uint64_t(1) << (device & 63);
+  if ((done.load(std::memory_order_relaxed) & bit) != 0 && device < 64) return cudaSuccess;
+  e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e == cudaSuccess) done.fetch_or(bit, std::memory_order_relaxed);
+  return e;
+}
+
 template <int PASS>
 cudaError_t launch_product(const GemmParams& p, int64_t tiles, cudaStream_t st) {
   if (tiles <= 0) return cudaSuccess;
   if (tiles > (int64_t(1) << 30)) return cudaErrorInvalidValue;
   constexpr int smem = smem_of(PASS != kStats);
-  const cudaError_t e = cudaFuncSetAttribute(lce_product_kernel<PASS>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  static std::atomic<uint64_t> done{0};
+  const cudaError_t e = allow_smem(done, (const void*)lce_product_kernel<PASS>, smem);
   if (e != cudaSuccess) return e;
   const int pairs = (int)(tiles < kNumSMs / 2 ? tiles : kNumSMs / 2);
   count_launch();
@@ -1126,7 +1182,8 @@ cudaError_t launch_product(const GemmParams& p, int64_t tiles, cudaStream_t st) 
 template <int PASS, int N>
 cudaError_t launch_few_of(const GemmParams& p, float* acc, int64_t tiles, cudaStream_t st) {
   constexpr int smem = FewShape<N>::kSmem;
-  const cudaError_t e = cudaFuncSetAttribute(lce_few_kernel<PASS, N>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  static std::atomic<uint64_t> done{0};
+  const cudaError_t e = allow_smem(done, (const void*)lce_few_kernel<PASS, N>, smem);
   if (e != cudaSuccess) return e;
   count_launch();
   lce_few_kernel<PASS, N><<<(unsigned)(tiles < kNumSMs ? tiles : kNumSMs), kFewThreads, smem, st>>>(p, acc);
@@ -1220,6 +1277,7 @@ int64_t lce_default_piece(int64_t rows, int64_t hidden, int64_t vocab) {
 
 int lce_splits(int64_t rows, int64_t hidden, int64_t vocab, int64_t piece) {
   const int64_t steps = (piece < vocab ? piece : vocab) / kInner;
+  if (vocab <= piece && steps <= 32) return 1;  // up to 9 us; a launch to join the splits is longer
   if (rows <= kLceFewRows) {
     // the number that leaves the fewest SMs idle in the last round; each split is as much again
     // of rows x hidden to write and read
@@ -1242,7 +1300,7 @@ int lce_splits(int64_t rows, int64_t hidden, int64_t vocab, int64_t piece) {
 cudaError_t launch_lce_backward(const LceArgs& a, const LceGrad& g, cudaStream_t st) {
   if (!args_ok(a) || g.piece <= 0 || g.piece % kTile != 0 || g.splits < 1 || g.g == nullptr) return cudaErrorInvalidValue;
   if (g.gh == nullptr && g.gw == nullptr) return cudaSuccess;
-  if (g.d == nullptr || (g.gh != nullptr && g.acc == nullptr) || (g.gw != nullptr && g.scaled == nullptr)) return cudaErrorInvalidValue;
+  if (g.d == nullptr || (g.gh != nullptr && g.acc == nullptr && !lce_direct(a.vocab, g.piece, g.splits)) || (g.gw != nullptr && g.scaled == nullptr)) return cudaErrorInvalidValue;
   cudaError_t e = make_context_current();
   if (e != cudaSuccess) return e;
   const int64_t pieces = lce_pieces(a.vocab, g.piece), pitch = lce_piece_pitch(a.vocab, g.piece);
@@ -1258,6 +1316,13 @@ cudaError_t launch_lce_backward(const LceArgs& a, const LceGrad& g, cudaStream_t
   common_params(q, a);
   q.inv = g.reduction == kLceMean ? a.inv : nullptr;
   q.g = g.reduction == kLceNone ? nullptr : g.g;
+  const bool direct = lce_direct(a.vocab, g.piece, g.splits);
+  p.gh = q.gh = direct ? (uint16_t*)g.gh : nullptr;
+  p.labels = a.labels;
+  p.ignore = a.ignore;
+  q.miss = a.miss;
+  q.index = a.index;
+  q.row_g = p.row_g;
   q.want_dh = g.gh != nullptr;
   q.want_dw = g.gw != nullptr;
   // Half of a tile would be products with zeros (2000 rows of 64, 5000 words: 19.6 us, so 18.0).
@@ -1274,7 +1339,7 @@ cudaError_t launch_lce_backward(const LceArgs& a, const LceGrad& g, cudaStream_t
       !encode(is_few ? &p.a : &p.b, a.w, a.hidden, a.vocab, a.w_stride, 128) ||
       !encode(is_few ? &few.a : &q.b, a.w, a.hidden, a.vocab, a.w_stride, 64) || (q.want_dw && !encode(&q.b2, g.scaled, a.hidden, p.padded, a.hidden, 64)) ||
       (q.want_dw && !encode(&q.out, g.gw, a.hidden, a.vocab, a.hidden, 32, 32)) ||
-      (q.want_dh && !encode_acc(&q.out_acc, g.acc, a.hidden, p.padded, g.splits)))
+      (q.want_dh && !direct && !encode_acc(&q.out_acc, g.acc, a.hidden, p.padded, g.splits)))
     return cudaErrorInvalidValue;
   for (int64_t i = 0; i < pieces; ++i) {
     p.word0 = q.word0 = i * g.piece;
@@ -1293,12 +1358,12 @@ cudaError_t launch_lce_backward(const LceArgs& a, const LceGrad& g, cudaStream_t
         return cudaErrorInvalidValue;
       if ((e = launch_product<kLogitGrad>(p, tiles_of(a.rows) * tiles_of(p.words), st)) != cudaSuccess) return e;
     }
-    p.scaled = nullptr;  // the first piece has done it
+    p.scaled = p.gh = nullptr;  // the first piece has done it
     const int64_t dh = q.want_dh ? tiles_of(a.rows) * tiles_of(a.hidden) * g.splits : 0;
     const int64_t dw = q.want_dw ? tiles_of(q.words) * tiles_of(a.hidden) : 0;
     if ((e = launch_product<kGrads>(q, dh + dw, st)) != cudaSuccess) return e;
   }
-  if (g.gh != nullptr) {
+  if (g.gh != nullptr && !direct) {
     count_launch();
     lce_join_grad_kernel<<<dim3((unsigned)a.rows, (unsigned)((a.hidden + 1023) / 1024)), 128, 0, st>>>(
         g.acc, g.splits, p.padded, a.index, a.labels, a.ignore, a.count, (int)a.hidden, a.miss, q.inv, q.g, p.row_g, (uint16_t*)g.gh);

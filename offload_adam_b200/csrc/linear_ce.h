@@ -50,10 +50,12 @@ struct LceGrad {
   void* d = nullptr;          // bf16 (padded rows, lce_piece_pitch)
   void* scaled = nullptr;     // bf16 (padded rows, hidden), for gw
   int splits = 1;             // of the sum over the words in gh
-  float* acc = nullptr;       // fp32 (splits, padded rows, hidden), for gh
+  float* acc = nullptr;       // fp32 (splits, padded rows, hidden), for gh unless lce_direct
 };
 inline int64_t lce_pieces(int64_t vocab, int64_t piece) { return (vocab + piece - 1) / piece; }
 inline int64_t lce_piece_pitch(int64_t vocab, int64_t piece) { return ((vocab < piece ? vocab : piece) + 15) / 16 * 16; }
+// gh goes straight out: its sums are whole after one launch.
+inline bool lce_direct(int64_t vocab, int64_t piece, int splits) { return vocab <= piece && splits == 1; }
 // Words at a time, and splits, when the caller leaves them to the package.
 int64_t lce_default_piece(int64_t rows, int64_t hidden, int64_t vocab);
 int lce_splits(int64_t rows, int64_t hidden, int64_t vocab, int64_t piece);

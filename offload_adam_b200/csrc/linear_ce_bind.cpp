@@ -27,10 +27,12 @@ Tensor rows_layout(const Tensor& t) {
 }
 int64_t row_stride(const Tensor& t) { return t.size(0) == 1 ? t.size(1) : t.stride(0); }
 
-// What backward needs of forward, in one int32 tensor: index, label, rest and miss of the packed
-// rows, their number with the ticket, 1 / number.
-int64_t kept_words(int64_t rows) { return 4 * rows + 4; }
-oab::LceArgs make_args(const Tensor& w, const Tensor& labels, const Tensor& kept, int64_t ignore, const Tensor& packed) {
+// What backward needs of forward, in one tensor of bytes: the packed rows of h (backward needs them in
+// any case, so keeping them instead of h leaves its peak), then index, label, rest and miss of each,
+// their number with the ticket, 1 / number.
+int64_t packed_bytes(int64_t rows, int64_t hidden) { return 2 * oab::lce_padded(rows) * hidden; }
+int64_t kept_bytes(int64_t rows, int64_t hidden) { return packed_bytes(rows, hidden) + 4 * (4 * rows + 4); }
+oab::LceArgs make_args(const Tensor& w, const Tensor& labels, const Tensor& kept, int64_t ignore) {
   oab::LceArgs a;
   a.w = w.data_ptr();
   a.w_stride = row_stride(w);
@@ -39,14 +41,14 @@ oab::LceArgs make_args(const Tensor& w, const Tensor& labels, const Tensor& kept
   a.hidden = w.size(1);
   a.vocab = w.size(0);
   a.ignore = ignore;
-  int* k = kept.data_ptr<int>();
+  a.packed = kept.data_ptr();
+  int* k = reinterpret_cast<int*>(static_cast<char*>(kept.data_ptr()) + packed_bytes(a.rows, a.hidden));
   a.index = k;
   a.label = k + a.rows;
   a.rest = reinterpret_cast<float*>(k + 2 * a.rows);
   a.miss = reinterpret_cast<float*>(k + 3 * a.rows);
   a.count = k + 4 * a.rows;
   a.inv = reinterpret_cast<float*>(k + 4 * a.rows + 2);
-  a.packed = packed.data_ptr();
   a.report = oab::loss_report();
   return a;
 }
@@ -78,20 +80,18 @@ struct LinearCE : torch::autograd::Function<LinearCE> {
     const Tensor hc = rows_layout(h), wc = rows_layout(w);
     const int64_t rows = h.size(0);
     const auto f32 = h.options().dtype(at::kFloat);
-    Tensor kept = at::empty({kept_words(rows)}, h.options().dtype(at::kInt));
+    Tensor kept = at::empty({kept_bytes(rows, h.size(1))}, h.options().dtype(at::kByte));
     Tensor loss = reduction == oab::kLceNone ? at::empty({rows}, f32) : at::empty({}, f32);
-    const Tensor packed = at::empty({oab::lce_padded(rows), h.size(1)}, h.options());
     Scratch x;
     const int64_t part = x.add(4 * oab::lce_part_floats(rows, w.size(0))), picked = x.add(4 * rows), sums = x.add(8 * oab::lce_sum_doubles(rows));
     x.take(h);
-    auto a = make_args(wc, labels, kept, ignore, packed);
+    auto a = make_args(wc, labels, kept, ignore);
     a.h = hc.data_ptr();
     a.h_stride = row_stride(hc);
     ok(oab::launch_lce_forward(a, (int)reduction, x.at_byte<float>(part), x.at_byte<float>(picked), x.at_byte<double>(sums),
                                loss.data_ptr<float>(), cur()),
        "linear_cross_entropy");
-    // the packed rows, not h: backward needs them in any case, so its peak is the same
-    ctx->save_for_backward({packed, w, labels, kept});
+    ctx->save_for_backward({w, labels, kept});
     ctx->saved_data["reduction"] = reduction;
     ctx->saved_data["ignore"] = ignore;
     ctx->saved_data["piece"] = piece;
@@ -106,12 +106,13 @@ struct LinearCE : torch::autograd::Function<LinearCE> {
     const bool graph = at::GradMode::is_enabled();
     at::NoGradGuard no_grad;
     const auto saved = ctx->get_saved_variables();
-    const Tensor &w = saved[1], &labels = saved[2], kept = saved[3].contiguous();
+    const Tensor &w = saved[0], &labels = saved[1];
     const int64_t reduction = ctx->saved_data["reduction"].toInt(), ignore = ctx->saved_data["ignore"].toInt();
     c10::cuda::CUDAGuard guard(w.device());
     oab::raise_loss_report();
     // hooks on saved tensors may have returned copies of another layout
-    const Tensor packed = rows_layout(saved[0].contiguous()), wc = rows_layout(w), lc = labels.contiguous();
+    const bool whole = saved[2].is_contiguous() && (reinterpret_cast<uintptr_t>(saved[2].data_ptr()) & 15u) == 0;
+    const Tensor kept = whole ? saved[2] : saved[2].clone(at::MemoryFormat::Contiguous), wc = rows_layout(w), lc = labels.contiguous();
     const Tensor gc = g.to(at::kFloat).contiguous();
     const int64_t rows = labels.size(0), hidden = w.size(1), vocab = w.size(0);
     int64_t piece = ctx->saved_data["piece"].toInt();
@@ -125,7 +126,7 @@ struct LinearCE : torch::autograd::Function<LinearCE> {
     Tensor gh, gw;
     Scratch t;
     const int64_t d = t.add(2 * oab::lce_padded(rows) * oab::lce_piece_pitch(vocab, piece));
-    const int64_t acc = t.add(want_h ? 4 * x.splits * oab::lce_padded(rows) * hidden : 0);
+    const int64_t acc = t.add(want_h && !oab::lce_direct(vocab, piece, x.splits) ? 4 * x.splits * oab::lce_padded(rows) * hidden : 0);
     const int64_t scaled = t.add(want_w ? 2 * oab::lce_padded(rows) * hidden : 0);
     t.take(w);
     x.d = t.at_byte<void>(d);
@@ -139,7 +140,7 @@ struct LinearCE : torch::autograd::Function<LinearCE> {
       x.gw = gw.data_ptr();
       x.scaled = t.at_byte<void>(scaled);
     }
-    ok(oab::launch_lce_backward(make_args(wc, lc, kept, ignore, packed), x, cur()), "linear_cross_entropy backward");
+    ok(oab::launch_lce_backward(make_args(wc, lc, kept, ignore), x, cur()), "linear_cross_entropy backward");
     if (graph) {
       const auto last = std::make_shared<torch::autograd::DelayedError>("linear_cross_entropy has no second derivative", 2);
       for (Tensor* t : {&gh, &gw})
