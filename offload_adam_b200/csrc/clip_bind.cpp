@@ -1,6 +1,7 @@
 // Python bindings of the global gradient norm and clipping.
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
+#include <torch/csrc/autograd/python_variable.h>
 #include <torch/extension.h>
 
 #include <algorithm>
@@ -97,22 +98,23 @@ Tensor grad_norm(const std::vector<Tensor>& grads, int64_t norm, double max_norm
   return out;
 }
 
-// The same for the gradients of `params`; nothing (and nothing done) when one of them is not a
-// plain gradient of one CUDA device that the kernels take, or when there is none.
-std::optional<Tensor> param_grad_norm(const std::vector<Tensor>& params, int64_t norm, double max_norm, bool scale) {
+// The same for the gradients of `params`; None (and nothing done) when one of them is not a plain
+// gradient of one CUDA device that the kernels take, or when there is none.
+py::object param_grad_norm(const py::list& params, int64_t norm, double max_norm, bool scale) {
   std::vector<Tensor> grads;
   grads.reserve(params.size());
-  for (const Tensor& p : params) {
-    const Tensor& g = p.grad();
+  for (const py::handle& h : params) {
+    TORCH_CHECK_TYPE(THPVariable_Check(h.ptr()), "parameters must be tensors");
+    const Tensor& g = THPVariable_Unpack(h.ptr()).grad();
     if (!g.defined()) continue;
     const auto t = g.scalar_type();
     if (!g.is_cuda() || g.layout() != at::kStrided || g.key_set().has(c10::DispatchKey::Python) ||
-        (t != at::kBFloat16 && t != at::kHalf && t != at::kFloat) || g.get_device() != (grads.empty() ? g : grads[0]).get_device())
-      return std::nullopt;
+        (t != at::kBFloat16 && t != at::kHalf && t != at::kFloat) || (!grads.empty() && g.get_device() != grads[0].get_device()))
+      return py::none();
     grads.push_back(g);
   }
-  if (grads.empty()) return std::nullopt;
-  return grad_norm(grads, norm, max_norm, scale);
+  if (grads.empty()) return py::none();
+  return py::cast(grad_norm(grads, norm, max_norm, scale));
 }
 
 // The gradients times `coef`, one fp32 value on their device.

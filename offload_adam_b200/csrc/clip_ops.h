@@ -24,9 +24,9 @@ int64_t clip_partials(int64_t count);
 // The norm over all tensors.  out[0] = min(1, max_norm / (norm + 1e-6)), out[1] = norm.
 // With `scale`, every value is then multiplied by out[0] in fp32 and rounded once, in place;
 // nothing is touched where out[0] is 1.
-cudaError_t launch_grad_norm(ClipEntry* entries, int64_t count, int norm, float max_norm, bool scale, double* partials,
+cudaError_t launch_grad_norm(const ClipEntry* entries, int64_t count, int norm, float max_norm, bool scale, double* partials,
                              float* out, cudaStream_t st);
 // The second half alone: coef is read from the device.
-cudaError_t launch_grad_scale(ClipEntry* entries, int64_t count, const float* coef, cudaStream_t st);
+cudaError_t launch_grad_scale(const ClipEntry* entries, int64_t count, const float* coef, cudaStream_t st);
 
 }  // namespace oab

@@ -72,7 +72,7 @@ def _run(parameters, norm_type, max_norm, scale):
     code = _norm_code(norm_type)
     parameters = [parameters] if isinstance(parameters, torch.Tensor) else list(parameters)
     # hundreds of small tensors are bound by what the host does for each of them: the usual case
-    # is looked over in C++ (291 tensors: 163 us a call, 26 with it)
+    # is looked over in C++ (291 tensors: 163 us a call without, 43 with it)
     if torch.cuda.is_available() and eager():
         out = _ext.load(required=True).param_grad_norm(parameters, code, max_norm, scale)
         if out is not None:
