@@ -8,6 +8,8 @@ namespace oab {
 constexpr int kLceTile = 256;     // rows and columns of an output tile; a piece of the vocabulary is a multiple
 constexpr int kLceFewRows = 64;   // up to here the rows are the narrow side of the products
 constexpr int kLceRowPad = 64;    // the packed rows are padded with zeros to a multiple of this
+// Sizes that the kernels take.
+constexpr int64_t kLceMaxRows = int64_t(1) << 24, kLceMaxHidden = int64_t(1) << 18, kLceMaxVocab = int64_t(1) << 26;
 
 // Operands and workspaces of one loss.  `rows` are the rows of h; the kernels work on those whose
 // label counts, packed in order: how many there are is known on the device only.

@@ -160,5 +160,9 @@ void bind_linear_ce(py::module_& m) {
   m.def("linear_ce", [](const Tensor& h, const Tensor& w, const Tensor& labels, int64_t reduction, int64_t ignore, int64_t piece) {
     return LinearCE::apply(h, w, labels, reduction, ignore, piece);
   });
+  m.def("linear_ce_takes", [](int64_t rows, int64_t hidden, int64_t vocab) {
+    return rows > 0 && rows <= oab::kLceMaxRows && hidden % 8 == 0 && hidden > 0 && hidden <= oab::kLceMaxHidden && vocab > 0 &&
+           vocab <= oab::kLceMaxVocab;
+  });
   m.def("linear_ce_piece", &oab::lce_default_piece, py::arg("rows"), py::arg("hidden"), py::arg("vocab"));
 }

@@ -26,6 +26,11 @@ class _PlainLinearCE(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, h, weight, labels, reduction, ignore_index, piece):
+        with torch.autocast(h.device.type, enabled=False):
+            return _PlainLinearCE._forward(ctx, h, weight, labels, reduction, ignore_index, piece)
+
+    @staticmethod
+    def _forward(ctx, h, weight, labels, reduction, ignore_index, piece):
         wide = torch.float64 if h.dtype == torch.float64 else torch.float32
         valid = labels != ignore_index
         rows = valid.nonzero(as_tuple=True)[0]
@@ -57,6 +62,11 @@ class _PlainLinearCE(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, g):
+        with torch.autocast(g.device.type, enabled=False):
+            return _PlainLinearCE._backward(ctx, g)
+
+    @staticmethod
+    def _backward(ctx, g):
         h, weight, labels, lse = ctx.saved_tensors
         reduction, ignore_index, piece = ctx.args
         rows = (labels != ignore_index).nonzero(as_tuple=True)[0]
@@ -87,7 +97,8 @@ def linear_cross_entropy(h, weight, labels, reduction="mean", ignore_index=-100,
 
     Args:
         h: hidden states, ``(..., hidden)``.
-        weight: the head, ``(vocab, hidden)``, of the dtype of ``h``; a dense tensor.
+        weight: the head, ``(vocab, hidden)``, a dense tensor of the dtype of ``h`` (under autocast
+            both are cast to its dtype).
         labels: int64, of the shape of ``h`` without its last dimension.
         reduction: ``"mean"`` over the rows that count (0 when there are none), ``"sum"``, or
             ``"none"``: one loss a row, of the shape of ``labels``, 0 for ignored rows.
@@ -97,8 +108,11 @@ def linear_cross_entropy(h, weight, labels, reduction="mean", ignore_index=-100,
             to a multiple of 256 where the kernels run.  ``None`` or 0: as many as take 256 MB.
 
     The result is fp32 (fp64 for fp64 inputs) and differentiable once with respect to ``h`` and
-    ``weight``.  Plain bf16 CUDA tensors whose ``hidden`` is a multiple of 8 run the
-    kernels (``csrc/linear_ce.cu``); everything else runs operations of PyTorch piece by piece.
+    ``weight``.  Plain bf16 CUDA tensors whose ``hidden`` is a multiple of 8 (2^18 at most; 2^24 rows,
+    2^26 words) run the kernels (``csrc/linear_ce.cu``); everything else runs operations of PyTorch
+    piece by piece.  Beside the gradients the kernels take a copy of the rows that count, until
+    backward, ``rows * vocab / 16`` bytes in forward, and in backward one piece, a second copy of
+    the rows and the fp32 sums of the hidden states' gradient.
 
     A label outside the vocabulary is an ``IndexError``.  The kernels see it when they run: the
     loss of that call is NaN, and the next call that looks (its backward, or the next loss)
@@ -115,6 +129,8 @@ def linear_cross_entropy(h, weight, labels, reduction="mean", ignore_index=-100,
     if labels.shape != h.shape[:-1] or labels.dtype != torch.int64:
         raise ValueError(f"linear_cross_entropy: int64 labels of shape {tuple(h.shape[:-1])} are needed, not "
                          f"{labels.dtype} of {tuple(labels.shape)}")
+    if torch.is_autocast_enabled(h.device.type):
+        h, weight = (t.to(torch.get_autocast_dtype(h.device.type)) for t in (h, weight))
     if not h.is_floating_point() or h.dtype != weight.dtype:
         raise ValueError(f"linear_cross_entropy: hidden states of {h.dtype} and a head of {weight.dtype}")
     if not (h.device == weight.device == labels.device):
@@ -122,7 +138,8 @@ def linear_cross_entropy(h, weight, labels, reduction="mean", ignore_index=-100,
     shape = labels.shape
     if len(shape) != 1:
         h, labels = h.reshape(-1, h.shape[-1]), labels.reshape(-1)
-    if use_kernels(h, weight) and type(labels) is torch.Tensor and h.shape[1] % 8 == 0 and h.numel() > 0:
+    if (use_kernels(h, weight) and type(labels) is torch.Tensor
+            and _ext.load(required=True).linear_ce_takes(*h.shape, weight.shape[0])):
         out = _ext.load(required=True).linear_ce(h, weight, labels.contiguous(), _REDUCTIONS[reduction], ignore_index,
                                                  piece or 0)
     else:

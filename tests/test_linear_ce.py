@@ -431,6 +431,20 @@ def test_refusals_on_the_gpu():
     _check(h, w, labels, g, "mean")
 
 
+@pytest.mark.parametrize("device", DEVICES)
+def test_under_autocast(device):
+    h, w, labels, g = _inputs(40, 64, 300, device)
+    plain = _run(h, w, labels, g, "mean")
+    x, y = h.float().requires_grad_(True), w.float().requires_grad_(True)
+    with torch.autocast(device, dtype=torch.bfloat16):
+        loss = linear_cross_entropy(x, y, labels)
+    loss.backward(g[0])
+    assert x.grad.dtype == y.grad.dtype == torch.float32
+    assert abs(loss - plain[0]) <= 1e-5 * plain[0]
+    for a, b in ((x.grad, plain[1]), (y.grad, plain[2])):
+        assert (a - b.float()).norm() <= 3 * 2.0 ** -8 * b.float().norm()
+
+
 # ------------------------------------------------------------------ as it is used
 def _tiny(device, **kw):
     from offload_adam_b200.models.llama import build_llama, tiny_llama
