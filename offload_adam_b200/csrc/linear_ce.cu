@@ -80,6 +80,7 @@ struct GemmParams {
   const float *miss, *row_g;  // the latter by row, or null
   const int* index;
   const uint16_t* packed;
+  int64_t row_pitch;          // of packed and scaled
   uint16_t* scaled;           // null: not wanted (again)
   uint16_t* gh;               // kLogitGrad: its ignored rows become zero; kGrads: dh goes out; null: neither
   const int64_t* labels;
@@ -279,8 +280,8 @@ __device__ __forceinline__ void prepare_rows(const GemmParams& p, int n_rows, in
   for (int k = mine; k < (n_rows + kLceRowPad - 1) / kLceRowPad * kLceRowPad; k += all) {
     float c = k < n_rows ? p.miss[k] : 0.f;
     if (k < n_rows && p.row_g != nullptr) c = __fmul_rn(c, p.row_g[p.index[k]]);
-    const uint4* from = reinterpret_cast<const uint4*>(p.packed + (int64_t)k * p.hidden);  // zeros beyond n_rows
-    uint4* to = reinterpret_cast<uint4*>(p.scaled + (int64_t)k * p.hidden);
+    const uint4* from = reinterpret_cast<const uint4*>(p.packed + (int64_t)k * p.row_pitch);  // zeros beyond n_rows
+    uint4* to = reinterpret_cast<uint4*>(p.scaled + (int64_t)k * p.row_pitch);
     auto both = [c](uint32_t w) {
       return f32x2_to_bf16x2_rne(__fmul_rn(__uint_as_float(w << 16), c), __fmul_rn(__uint_as_float(w & 0xffff0000u), c));
     };
@@ -826,12 +827,12 @@ lce_few_kernel(const __grid_constant__ GemmParams p, float* acc) {
           p.gh[(int64_t)row_of[r] * p.hidden + at] = (uint16_t)f32_to_bf16_rne_bits(__fmul_rn(v[r], scale_of[r]));
         }
       } else if (at < p.hidden) {
-        float* to = acc + (int64_t)(t / across) * p.padded * p.hidden + at;
+        float* to = acc + (int64_t)(t / across) * p.padded * p.row_pitch + at;
 #pragma unroll
         for (int r = 0; r < N; ++r) {
           if (r >= n_rows) break;
           const float x = steps != 0 ? v[r] : 0.f;
-          to[(int64_t)r * p.hidden] = p.first ? x : __fadd_rn(to[(int64_t)r * p.hidden], x);
+          to[(int64_t)r * p.row_pitch] = p.first ? x : __fadd_rn(to[(int64_t)r * p.row_pitch], x);
         }
       }
     }
@@ -903,6 +904,7 @@ struct PackArgs {
   int64_t w_stride;
   int hidden;
   uint16_t* packed;
+  int64_t packed_pitch;
   float* picked;
 };
 __device__ __forceinline__ float dot2(uint32_t a, uint32_t b, float c) {  // of two bf16 pairs
@@ -913,7 +915,7 @@ __device__ __forceinline__ float dot2(uint32_t a, uint32_t b, float c) {  // of 
 template <int THREADS>
 __device__ __forceinline__ void pack_row(const PackArgs& a, int64_t k, int n, int row, int label) {
   const int vecs = a.hidden >> 3, lane = threadIdx.x % THREADS;
-  uint4* to = reinterpret_cast<uint4*>(a.packed + k * a.hidden);
+  uint4* to = reinterpret_cast<uint4*>(a.packed + k * a.packed_pitch);
   if (k < n) {
     const uint4* from = reinterpret_cast<const uint4*>(a.h + row * a.h_stride);
     const uint4* word = reinterpret_cast<const uint4*>(a.w + (label < 0 ? 0 : label) * a.w_stride);
@@ -1095,7 +1097,7 @@ lce_join_kernel(const float2* __restrict__ part, int parts, int64_t rows, const 
 // -------------------------------------------------- dh: splits joined, rounded
 // Rows whose label is ignored become zero.
 __global__ void __launch_bounds__(128)
-lce_join_grad_kernel(const float* __restrict__ acc, int splits, int64_t padded, const int* __restrict__ index,
+lce_join_grad_kernel(const float* __restrict__ acc, int splits, int64_t padded, int64_t pitch, const int* __restrict__ index,
                      const int64_t* __restrict__ labels, int64_t ignore, const int* __restrict__ count, int hidden,
                      const float* __restrict__ miss, const float* inv, const float* g, const float* row_g, uint16_t* gh) {
   const int64_t k = blockIdx.x;
@@ -1109,7 +1111,7 @@ lce_join_grad_kernel(const float* __restrict__ acc, int splits, int64_t padded, 
   if (row_g != nullptr) scale = __fmul_rn(scale, row_g[index[k]]);
   float v[8] = {};
   for (int s = 0; s < splits; ++s) {
-    const V8 x = ld32(acc + ((int64_t)s * padded + k) * hidden + col);
+    const V8 x = ld32(acc + ((int64_t)s * padded + k) * pitch + col);
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[i] = __fadd_rn(v[i], __uint_as_float(x.w[i]));
   }
@@ -1138,11 +1140,11 @@ cudaError_t make_context_current() {
 }
 
 // The fp32 sums of dh as (hidden, rows, splits) in boxes of 16 columns and 32 rows.
-bool encode_acc(CUtensorMap* map, float* base, int64_t hidden, int64_t padded, int splits) {
+bool encode_acc(CUtensorMap* map, float* base, int64_t hidden, int64_t pitch, int64_t padded, int splits) {
   const auto fn = encoder();
   if (fn == nullptr) return false;
   const cuuint64_t dims[3] = {(cuuint64_t)hidden, (cuuint64_t)padded, (cuuint64_t)splits};
-  const cuuint64_t strides[2] = {(cuuint64_t)hidden * 4, (cuuint64_t)hidden * 4 * (cuuint64_t)padded};
+  const cuuint64_t strides[2] = {(cuuint64_t)pitch * 4, (cuuint64_t)pitch * 4 * (cuuint64_t)padded};
   const cuuint32_t box[3] = {16, 32, 1}, steps[3] = {1, 1, 1};
   return fn(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 3, base, dims, strides, box, steps, CU_TENSOR_MAP_INTERLEAVE_NONE,
             CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
@@ -1218,6 +1220,7 @@ void common_params(GemmParams& p, const LceArgs& a) {
   p.rows = a.rows;
   p.padded = lce_padded(a.rows);
   p.hidden = (int)a.hidden;
+  p.row_pitch = lce_row_pitch(a.hidden);
   p.report = a.report;
   p.label = a.label;
 }
@@ -1234,7 +1237,7 @@ cudaError_t launch_lce_forward(const LceArgs& a, int reduction, float* part, flo
   if (!args_ok(a) || a.h_stride % 8 != 0 || !aligned16(a.h)) return cudaErrorInvalidValue;
   float* const row_loss = reduction == kLceNone ? loss : nullptr;
   const unsigned blocks = (unsigned)(lce_padded(a.rows) / kPackRows);
-  const PackArgs k{(const uint16_t*)a.h, a.h_stride, (const uint16_t*)a.w, a.w_stride, (int)a.hidden, (uint16_t*)a.packed, picked};
+  const PackArgs k{(const uint16_t*)a.h, a.h_stride, (const uint16_t*)a.w, a.w_stride, (int)a.hidden, (uint16_t*)a.packed, lce_row_pitch(a.hidden), picked};
   if (a.rows <= kScanPackBlockRows) {
     count_launch();
     lce_scan_pack_kernel<kPackThreads><<<(unsigned)lce_padded(a.rows), kPackThreads, 0, st>>>(
@@ -1258,12 +1261,12 @@ cudaError_t launch_lce_forward(const LceArgs& a, int reduction, float* part, flo
   int parts = (int)(2 * tiles_of(a.vocab));
   if (a.rows <= kLceFewRows) {
     if (!encode(&p.a, a.w, a.hidden, a.vocab, a.w_stride, 128) ||
-        !encode(&p.b, a.packed, a.hidden, p.padded, a.hidden, few_columns(a.rows)))
+        !encode(&p.b, a.packed, a.hidden, p.padded, p.row_pitch, few_columns(a.rows)))
       return cudaErrorInvalidValue;
     parts = (int)((a.vocab + 127) / 128);
     e = launch_few<kStats>(p, nullptr, parts, st);
   } else {
-    if (!encode(&p.a, a.packed, a.hidden, p.padded, a.hidden, 128) || !encode(&p.b, a.w, a.hidden, a.vocab, a.w_stride, 128))
+    if (!encode(&p.a, a.packed, a.hidden, p.padded, p.row_pitch, 128) || !encode(&p.b, a.w, a.hidden, a.vocab, a.w_stride, 128))
       return cudaErrorInvalidValue;
     e = launch_product<kStats>(p, tiles_of(a.rows) * tiles_of(a.vocab), st);
   }
@@ -1340,11 +1343,11 @@ cudaError_t launch_lce_backward(const LceArgs& a, const LceGrad& g, cudaStream_t
   if (is_few) q.want_dh = 0;
   p.d = (uint16_t*)g.d;
   p.pitch = pitch;
-  if (!encode(is_few ? &p.b : &p.a, a.packed, a.hidden, p.padded, a.hidden, is_few ? columns : 128) ||
+  if (!encode(is_few ? &p.b : &p.a, a.packed, a.hidden, p.padded, p.row_pitch, is_few ? columns : 128) ||
       !encode(is_few ? &p.a : &p.b, a.w, a.hidden, a.vocab, a.w_stride, 128) ||
-      !encode(is_few ? &few.a : &q.b, a.w, a.hidden, a.vocab, a.w_stride, 64) || (q.want_dw && !encode(&q.b2, g.scaled, a.hidden, p.padded, a.hidden, 64)) ||
+      !encode(is_few ? &few.a : &q.b, a.w, a.hidden, a.vocab, a.w_stride, 64) || (q.want_dw && !encode(&q.b2, g.scaled, a.hidden, p.padded, p.row_pitch, 64)) ||
       (q.want_dw && !encode(&q.out, g.gw, a.hidden, a.vocab, a.hidden, 32, 32)) ||
-      (q.want_dh && !direct && !encode_acc(&q.out_acc, g.acc, a.hidden, p.padded, g.splits)))
+      (q.want_dh && !direct && !encode_acc(&q.out_acc, g.acc, a.hidden, p.row_pitch, p.padded, g.splits)))
     return cudaErrorInvalidValue;
   for (int64_t i = 0; i < pieces; ++i) {
     p.word0 = q.word0 = i * g.piece;
@@ -1371,7 +1374,7 @@ cudaError_t launch_lce_backward(const LceArgs& a, const LceGrad& g, cudaStream_t
   if (g.gh != nullptr && !direct) {
     count_launch();
     lce_join_grad_kernel<<<dim3((unsigned)a.rows, (unsigned)((a.hidden + 1023) / 1024)), 128, 0, st>>>(
-        g.acc, g.splits, p.padded, a.index, a.labels, a.ignore, a.count, (int)a.hidden, a.miss, q.inv, q.g, p.row_g, (uint16_t*)g.gh);
+        g.acc, g.splits, p.padded, p.row_pitch, a.index, a.labels, a.ignore, a.count, (int)a.hidden, a.miss, q.inv, q.g, p.row_g, (uint16_t*)g.gh);
     e = cudaGetLastError();
   }
   return e;

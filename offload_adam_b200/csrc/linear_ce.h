@@ -27,12 +27,16 @@ struct LceArgs {
   float* inv = nullptr;              // 1 / max(1, packed rows)
   float* rest = nullptr;             // (rows,) log-sum-exp of the packed row without its label
   float* miss = nullptr;             // (rows,) 1 - probability of its label
-  void* packed = nullptr;            // bf16 (rows padded, hidden)
+  void* packed = nullptr;            // bf16 (rows padded, lce_row_pitch)
   int64_t* report = nullptr;         // host memory: [0] a label past the vocabulary, [1] a wait that gave up, [2] a negative label
 };
 
 // Rows of `packed` and of a piece of the logits' gradient.
 inline int64_t lce_padded(int64_t rows) { return (rows + kLceRowPad - 1) / kLceRowPad * kLceRowPad; }
+
+// Values from one of their rows to the next: whole 128-byte lines, which TMA reads and writes faster
+// (640 rows of 840: the statistics 45 us, of 832 or 896 37), whatever the pitch of h is.
+inline int64_t lce_row_pitch(int64_t hidden) { return (hidden + 63) / 64 * 64; }
 
 enum LceReduction : int { kLceNone = 0, kLceMean = 1, kLceSum = 2 };
 
@@ -50,12 +54,12 @@ struct LceGrad {
   void* gw = nullptr;         // bf16 (vocab, hidden) contiguous, or null
   int64_t piece = 0;          // words at a time, a multiple of kLceTile
   void* d = nullptr;          // bf16 (padded rows, lce_piece_pitch)
-  void* scaled = nullptr;     // bf16 (padded rows, hidden), for gw
+  void* scaled = nullptr;     // bf16 (padded rows, lce_row_pitch), for gw
   int splits = 1;             // of the sum over the words in gh
-  float* acc = nullptr;       // fp32 (splits, padded rows, hidden), for gh unless lce_direct
+  float* acc = nullptr;       // fp32 (splits, padded rows, lce_row_pitch), for gh unless lce_direct
 };
 inline int64_t lce_pieces(int64_t vocab, int64_t piece) { return (vocab + piece - 1) / piece; }
-inline int64_t lce_piece_pitch(int64_t vocab, int64_t piece) { return ((vocab < piece ? vocab : piece) + 15) / 16 * 16; }
+inline int64_t lce_piece_pitch(int64_t vocab, int64_t piece) { return ((vocab < piece ? vocab : piece) + 63) / 64 * 64; }
 // gh goes straight out: its sums are whole after one launch.
 inline bool lce_direct(int64_t vocab, int64_t piece, int splits) { return vocab <= piece && splits == 1; }
 // Words at a time, and splits, when the caller leaves them to the package.

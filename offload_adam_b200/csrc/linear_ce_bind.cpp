@@ -30,7 +30,7 @@ int64_t row_stride(const Tensor& t) { return t.size(0) == 1 ? t.size(1) : t.stri
 // What backward needs of forward, in one tensor of bytes: the packed rows of h (backward needs them in
 // any case, so keeping them instead of h leaves its peak), then index, label, rest and miss of each,
 // their number with the ticket, 1 / number.
-int64_t packed_bytes(int64_t rows, int64_t hidden) { return 2 * oab::lce_padded(rows) * hidden; }
+int64_t packed_bytes(int64_t rows, int64_t hidden) { return 2 * oab::lce_padded(rows) * oab::lce_row_pitch(hidden); }
 int64_t kept_bytes(int64_t rows, int64_t hidden) { return packed_bytes(rows, hidden) + 4 * (4 * rows + 4); }
 oab::LceArgs make_args(const Tensor& w, const Tensor& labels, const Tensor& kept, int64_t ignore) {
   oab::LceArgs a;
@@ -126,8 +126,8 @@ struct LinearCE : torch::autograd::Function<LinearCE> {
     Tensor gh, gw;
     Scratch t;
     const int64_t d = t.add(2 * oab::lce_padded(rows) * oab::lce_piece_pitch(vocab, piece));
-    const int64_t acc = t.add(want_h && !oab::lce_direct(vocab, piece, x.splits) ? 4 * x.splits * oab::lce_padded(rows) * hidden : 0);
-    const int64_t scaled = t.add(want_w ? 2 * oab::lce_padded(rows) * hidden : 0);
+    const int64_t acc = t.add(want_h && !oab::lce_direct(vocab, piece, x.splits) ? 4 * x.splits * oab::lce_padded(rows) * oab::lce_row_pitch(hidden) : 0);
+    const int64_t scaled = t.add(want_w ? packed_bytes(rows, hidden) : 0);
     t.take(w);
     x.d = t.at_byte<void>(d);
     if (want_h) {
