@@ -435,6 +435,8 @@ lce_product_kernel(const __grid_constant__ GemmParams p) {
   fence_after();
   const uint32_t tmem = tmem_at;
 
+  grid_release();
+  grid_wait();
   const int n_rows = *p.count;
   Plan plan{};
   plan.make<PASS>(p, n_rows, gridDim.x >> 1);
@@ -647,6 +649,8 @@ lce_few_kernel(const __grid_constant__ GemmParams p, float* acc) {
   const uint32_t stages = (smem_addr(smem_raw) + 1023u) & ~1023u;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t full0 = smem_addr(full), empty0 = smem_addr(empty), done0 = smem_addr(done), drained0 = smem_addr(drained);
+  grid_release();
+  grid_wait();
   const int n_rows = *p.count;
   if (threadIdx.x == 0) {
     gave_up = 0;
@@ -1025,6 +1029,8 @@ lce_join_kernel(const float2* __restrict__ part, int parts, int64_t rows, const 
   __shared__ double one[kJoinRows];
   __shared__ int is_last;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  grid_release();
+  grid_wait();
   const int n = *count, of = threadIdx.x % kJoinRows, slice = threadIdx.x / kJoinRows;
   const int64_t row = (int64_t)blockIdx.x * kJoinRows + of;
   float m = -INFINITY, s = 0.f;
@@ -1102,6 +1108,7 @@ lce_join_grad_kernel(const float* __restrict__ acc, int splits, int64_t padded, 
                      const float* __restrict__ miss, const float* inv, const float* g, const float* row_g, uint16_t* gh) {
   const int64_t k = blockIdx.x;
   const int col = (blockIdx.y * 128 + threadIdx.x) * 8;
+  grid_wait();
   if (col >= hidden) return;
   if (labels[k] == ignore) *reinterpret_cast<uint4*>(gh + k * hidden + col) = make_uint4(0, 0, 0, 0);
   if (k >= *count) return;
@@ -1161,6 +1168,23 @@ bool encode(CUtensorMap* map, const void* base, int64_t inner, int64_t lines_all
             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+// Launches a kernel that begins with grid_wait: its blocks come up while the last ones of the kernel
+// before it in the stream, one of this file, still run.
+template <class... Args, class... Given>
+cudaError_t launch_behind(void (*kernel)(Args...), dim3 grid, int threads, int smem, cudaStream_t st, const Given&... given) {
+  cudaLaunchConfig_t c{};
+  c.gridDim = grid;
+  c.blockDim = dim3(threads);
+  c.dynamicSmemBytes = smem;
+  c.stream = st;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  c.attrs = &attr;
+  c.numAttrs = 1;
+  return cudaLaunchKernelEx(&c, kernel, Args(given)...);
+}
+
 // Once for each kernel and device.
 cudaError_t allow_smem(std::atomic<uint64_t>& done, const void* kernel, int bytes) {
   int device = 0;
@@ -1183,8 +1207,7 @@ cudaError_t launch_product(const GemmParams& p, int64_t tiles, cudaStream_t st) 
   if (e != cudaSuccess) return e;
   const int pairs = (int)(tiles < kNumSMs / 2 ? tiles : kNumSMs / 2);
   count_launch();
-  lce_product_kernel<PASS><<<2 * pairs, kGemmThreads, smem, st>>>(p);
-  return cudaGetLastError();
+  return launch_behind(lce_product_kernel<PASS>, dim3(2 * pairs), kGemmThreads, smem, st, p);
 }
 
 template <int PASS, int N>
@@ -1194,8 +1217,7 @@ cudaError_t launch_few_of(const GemmParams& p, float* acc, int64_t tiles, cudaSt
   const cudaError_t e = allow_smem(done, (const void*)lce_few_kernel<PASS, N>, smem);
   if (e != cudaSuccess) return e;
   count_launch();
-  lce_few_kernel<PASS, N><<<(unsigned)(tiles < kNumSMs ? tiles : kNumSMs), kFewThreads, smem, st>>>(p, acc);
-  return cudaGetLastError();
+  return launch_behind(lce_few_kernel<PASS, N>, dim3((unsigned)(tiles < kNumSMs ? tiles : kNumSMs)), kFewThreads, smem, st, p, acc);
 }
 // 16 columns keep three more stages in flight and shorten the epilogue; up to 64 rows otherwise.
 constexpr int few_columns(int64_t rows) { return rows <= 16 ? 16 : kLceFewRows; }
@@ -1272,9 +1294,8 @@ cudaError_t launch_lce_forward(const LceArgs& a, int reduction, float* part, flo
   }
   if (e != cudaSuccess) return e;
   count_launch();
-  lce_join_kernel<<<(unsigned)lce_sum_doubles(a.rows), kJoinThreads, 0, st>>>(
-      p.part, parts, a.rows, a.index, a.label, a.count, picked, a.inv, a.rest, a.miss, reduction, sums, loss);
-  return cudaGetLastError();
+  return launch_behind(lce_join_kernel, dim3((unsigned)lce_sum_doubles(a.rows)), kJoinThreads, 0, st, p.part, parts, a.rows, a.index,
+                       a.label, a.count, picked, a.inv, a.rest, a.miss, reduction, sums, loss);
 }
 
 int64_t lce_default_piece(int64_t rows, int64_t hidden, int64_t vocab) {
@@ -1373,9 +1394,9 @@ cudaError_t launch_lce_backward(const LceArgs& a, const LceGrad& g, cudaStream_t
   }
   if (g.gh != nullptr && !direct) {
     count_launch();
-    lce_join_grad_kernel<<<dim3((unsigned)a.rows, (unsigned)((a.hidden + 1023) / 1024)), 128, 0, st>>>(
-        g.acc, g.splits, p.padded, p.row_pitch, a.index, a.labels, a.ignore, a.count, (int)a.hidden, a.miss, q.inv, q.g, p.row_g, (uint16_t*)g.gh);
-    e = cudaGetLastError();
+    e = launch_behind(lce_join_grad_kernel, dim3((unsigned)a.rows, (unsigned)((a.hidden + 1023) / 1024)), 128, 0, st, g.acc, g.splits,
+                      p.padded, p.row_pitch, a.index, a.labels, a.ignore, a.count, (int)a.hidden, a.miss, q.inv, q.g, p.row_g,
+                      (uint16_t*)g.gh);
   }
   return e;
 }

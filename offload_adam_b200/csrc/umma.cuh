@@ -25,6 +25,11 @@ __device__ __forceinline__ bool elect_one() {
   return ok != 0;
 }
 
+// Until the grid that this one was launched behind is done and its writes are seen; until then
+// nothing that it reads or writes may be touched.  And: the next one may be brought up.
+__device__ __forceinline__ void grid_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void grid_release() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
 // ------------------------------------------------------------------ mbarriers
 __device__ __forceinline__ void mbar_init(uint32_t bar, uint32_t count) {
   asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count) : "memory");
