@@ -95,9 +95,11 @@ def _check(h, w, labels, g, reduction, **kw):
 
 
 # rows and words around a tile of one CTA (128) and of a pair (256), rows around the few that run
-# the narrow products (16 and 64), inner sizes around a stage (64), pieces that end with one word
+# the narrow products (16 and 64), are packed a block or a warp each (512) or in two launches (4096),
+# inner sizes around a stage (64) and a chain of sums (512)
 SIZES = [(1, 8, 1), (1, 64, 257), (2, 72, 7), (16, 264, 300), (17, 72, 129), (63, 64, 128), (64, 128, 127), (64, 1032, 5000), (65, 256, 129), (127, 264, 255),
-         (128, 8, 256), (129, 840, 513), (255, 64, 1000), (256, 256, 1024), (257, 520, 2049), (700, 136, 4099)]
+         (128, 8, 256), (129, 840, 513), (255, 64, 1000), (256, 256, 1024), (257, 520, 2049), (700, 136, 4099),
+         (512, 64, 300), (513, 72, 300), (4096, 8, 65), (4097, 16, 130), (9000, 8, 40), (130, 1032, 700), (300, 128, 5000)]
 
 
 @pytest.mark.parametrize("device", DEVICES)
@@ -107,9 +109,10 @@ def test_matches_64_bits(n, hidden, vocab, reduction, device):
     _check(*_inputs(n, hidden, vocab, device), reduction)
 
 
+# pieces that end with one word, and that leave some splits of the sum over the words nothing
 @gpu
-@pytest.mark.parametrize("piece", [1, 256, 300, 768, 4096, 1 << 20])
-@pytest.mark.parametrize("n,hidden,vocab", [(3, 64, 2561), (40, 136, 2100), (300, 200, 2560), (513, 96, 1025)])
+@pytest.mark.parametrize("piece", [1, 256, 300, 768, 2048, 4096, 1 << 62])
+@pytest.mark.parametrize("n,hidden,vocab", [(3, 64, 2561), (40, 136, 2100), (20, 64, 4097), (70, 64, 4097), (300, 200, 2560), (513, 96, 1025)])
 def test_pieces(n, hidden, vocab, piece):
     _check(*_inputs(n, hidden, vocab, "cuda"), "mean", piece=piece)
 
@@ -337,8 +340,9 @@ def test_captured_and_replayed(n):
 
 
 @pytest.mark.parametrize("device", DEVICES)
-def test_one_gradient_no_gradient_and_a_graph_used_twice(device):
-    h, w, labels, g = _inputs(70, 64, 300, device)
+@pytest.mark.parametrize("n", [20, 70])
+def test_one_gradient_no_gradient_and_a_graph_used_twice(n, device):
+    h, w, labels, g = _inputs(n, 64, 5000, device)
     both = _run(h, w, labels, g, "mean")
     for want_h, want_w in ((True, False), (False, True)):
         x, y = h.clone().requires_grad_(want_h), w.clone().requires_grad_(want_w)
