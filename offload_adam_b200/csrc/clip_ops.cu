@@ -208,13 +208,13 @@ grad_scale_kernel(const __grid_constant__ ClipTable<CAP> table, const double* __
     const int64_t end = begin + table.chunk_vecs < vecs ? begin + table.chunk_vecs : vecs;
     char* base = reinterpret_cast<char*>(e.p) + head * (32 / per);
     const uint32_t dtype = e.dtype;
-    for (int64_t v = begin + threadIdx.x; v < end; v += 4 * kThreads) {
-      V8 r[4];
+    for (int64_t v = begin + threadIdx.x; v < end; v += 2 * kThreads) {
+      V8 r[2];
 #pragma unroll
-      for (int u = 0; u < 4; ++u)
+      for (int u = 0; u < 2; ++u)
         if (v + u * kThreads < end) r[u] = ld32(base + (v + u * kThreads) * 32);
 #pragma unroll
-      for (int u = 0; u < 4; ++u)
+      for (int u = 0; u < 2; ++u)
         if (v + u * kThreads < end) st32(base + (v + u * kThreads) * 32, scaled(r[u], dtype, c));
     }
     if (begin == 0) {
@@ -259,8 +259,12 @@ cudaError_t norm_pass(const ClipTable<CAP>& t, unsigned grid, int norm, double* 
   return cudaGetLastError();
 }
 template <int CAP>
-cudaError_t scale_pass(const ClipTable<CAP>& t, unsigned grid, int norm, float max_norm, const double* partials, int n, float* out,
+cudaError_t scale_pass(const ClipTable<CAP>& t, unsigned blocks, int norm, float max_norm, const double* partials, int n, float* out,
                        int write_out, cudaStream_t st) {
+  // Two loads a thread, and twice as many blocks as fit at once where each still has eight chunks:
+  // 1.27 G bf16 values, norm and scaling, 1198 us (1272 with the blocks that fit; 1240 with four
+  // loads); 88 M values of both types 89 us and 84.
+  const unsigned grid = t.chunks >= 16u * kBlocks ? 2u * kBlocks : blocks;
   count_launch();
   if (norm == kNormL2) grad_scale_kernel<kNormL2, CAP><<<grid, kThreads, 0, st>>>(t, partials, n, max_norm, out, write_out);
   else if (norm == kNormL1) grad_scale_kernel<kNormL1, CAP><<<grid, kThreads, 0, st>>>(t, partials, n, max_norm, out, write_out);
