@@ -90,6 +90,7 @@ struct GemmParams {
   // kGrads
   const float *inv, *g;  // each may be null (1)
   int want_dh, want_dw;
+  uint16_t* gw;               // few rows; otherwise by `out`
   int narrow;            // at most 128 hidden columns: products of 128 columns
   int splits;
   int first;             // piece: its dh starts the sums
@@ -849,6 +850,146 @@ lce_few_kernel(const __grid_constant__ GemmParams p, float* acc) {
   if (warp == 1) tmem_free(tmem, S::kColumns);
 }
 
+// dW of few rows: W's size to write, and products of a single stage for each tile, 128 words by 256
+// hidden columns.  What goes out in 256 bytes of a row at a time gets 6.1 TB/s, in the 128 bytes of
+// a tiled store 5.0, whatever computes it.  So a warp stages its 32 rows and 128 columns whole, rows
+// 272 bytes apart (free of bank conflicts), and each lane copies one.  A CTA takes consecutive
+// tiles along the rows of dW: d of its words stays in shared memory and is read once, the rows of h
+// come out of L2 again and again.  32 rows, hidden 8192, 128256 words: h takes 1 MB, d 16 MB, dW
+// 2.1 GB in 454 us (4.6 TB/s); with the rows of h kept and d read again 541, in the pair kernel 503.
+constexpr int kFewDwStages = 2, kFewDwRow = 272, kFewDwStaging = 32 * kFewDwRow;
+constexpr int kFewDwSmem = kFewDwStages * 2 * kHalfBytes + kHalfBytes + kEpilogueWarps * kFewDwStaging + 1024;
+__global__ void __launch_bounds__(kGemmThreads, 1)
+lce_few_dw_kernel(const __grid_constant__ GemmParams p) {
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ uint64_t full[kFewDwStages], empty[kFewDwStages], done[2], drained[2], d_full[1], d_empty[1];
+  __shared__ uint32_t tmem_at;
+  __shared__ int gave_up;
+  const uint32_t stages = (smem_addr(smem_raw) + 1023u) & ~1023u, d_at = stages + kFewDwStages * 2 * kHalfBytes;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t full0 = smem_addr(full), empty0 = smem_addr(empty), done0 = smem_addr(done), drained0 = smem_addr(drained);
+  const uint32_t d_full0 = smem_addr(d_full), d_empty0 = smem_addr(d_empty);
+  if (threadIdx.x == 0) {
+    gave_up = 0;
+    for (int i = 0; i < kFewDwStages; ++i) {
+      mbar_init(full0 + 8 * i, 1);
+      mbar_init(empty0 + 8 * i, 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(done0 + 8 * i, 1);
+      mbar_init(drained0 + 8 * i, kEpilogueWarps / 2);
+    }
+    mbar_init(d_full0, 1);
+    mbar_init(d_empty0, 1);
+    mbar_init_fence();
+    prefetch_map(&p.a2);
+    prefetch_map(&p.b2);
+  }
+  if (warp == 1) tmem_alloc(smem_addr(&tmem_at), 512);
+  fence_before();
+  __syncthreads();
+  fence_after();
+  const uint32_t tmem = tmem_at;
+  grid_release();
+  grid_wait();
+
+  const int across = (p.hidden + kTile - 1) / kTile, total = across * ((p.words + 127) / 128);
+  const int begin = (int)((int64_t)total * blockIdx.x / gridDim.x), end = (int)((int64_t)total * (blockIdx.x + 1) / gridDim.x);
+  const int first_m = begin / across;
+  bool ok = true;
+  if (warp == 0) {
+    if (elect_one()) {
+      int m = first_m, column = begin - first_m * across;
+      for (int t = begin; t < end && ok; ++t) {
+        if (t == begin || column == 0) {
+          if (!mbar_wait(d_empty0, ((m - first_m) & 1) ^ 1)) { ok = false; break; }
+          mbar_expect_tx(d_full0, kHalfBytes);
+          tma_load(d_at, &p.a2, m * 128, 0, d_full0);
+          tma_load(d_at + kHalfBytes / 2, &p.a2, m * 128 + 64, 0, d_full0);
+        }
+        const int n = t - begin, s = n % kFewDwStages;
+        if (!mbar_wait(empty0 + 8 * s, ((n / kFewDwStages) & 1) ^ 1)) { ok = false; break; }
+        mbar_expect_tx(full0 + 8 * s, 2 * kHalfBytes);
+        for (int i = 0; i < 4; ++i)
+          tma_load(stages + (s * 4 + i) * (kHalfBytes / 2), &p.b2, column * kTile + i * 64, 0, full0 + 8 * s);
+        if (++column == across) column = 0, ++m;
+      }
+      if (!ok) {  // copies that are still under way end within microseconds
+        for (int i = 0; i < 100; ++i) __nanosleep(10000);
+      }
+    }
+    __syncwarp();
+  } else if (warp == 1) {
+    if (elect_one()) {
+      constexpr uint32_t idesc = instruction(128, kTile, true, true);
+      int m = first_m, column = begin - first_m * across;
+      for (int t = begin; t < end && ok; ++t) {
+        const int n = t - begin, s = n % kFewDwStages, acc = n & 1;
+        if ((t == begin || column == 0) && !mbar_wait(d_full0, (m - first_m) & 1)) { ok = false; break; }
+        if (!mbar_wait(drained0 + 8 * acc, ((n >> 1) & 1) ^ 1) || !mbar_wait(full0 + 8 * s, (n / kFewDwStages) & 1)) { ok = false; break; }
+        fence_after();
+        const uint64_t da = operand(d_at, kHalfBytes / 2, 1024), db = operand(stages + s * 2 * kHalfBytes, kHalfBytes / 2, 1024);
+#pragma unroll
+        for (int q = 0; q < kLceRowPad / 16; ++q) mma(tmem + acc * kTile, da + q * (2048 >> 4), db + q * (2048 >> 4), idesc, q > 0);
+        commit(empty0 + 8 * s);
+        commit(done0 + 8 * acc);
+        if (++column == across) {
+          commit(d_empty0);
+          column = 0;
+          ++m;
+        }
+      }
+    }
+    __syncwarp();
+  } else {
+    const int quarter = warp & 3, half = ((warp - 2) >> 2) & 1, group = (warp - 2) >> 3;
+    const bool none = *p.count == 0;  // d and h are not there
+    const float scale = all_scale(p);
+    const uint32_t staging = d_at + kHalfBytes + (warp - 2) * kFewDwStaging;
+    for (int t = begin + group; t < end; t += 2) {
+      const int m = t / across, column = t - m * across;
+      ok = mbar_wait(done0 + 8 * group, ((t - begin) >> 1) & 1);
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) break;
+      fence_after();
+      const uint32_t at = tmem + group * kTile + half * 128 + ((uint32_t)(quarter * 32) << 16);
+      store_wait_read();  // each lane its own row of the last tile
+      __syncwarp();
+#pragma unroll 1
+      for (int c = 0; c < 4; ++c) {
+        float v[32];
+        tmem_load32(at + c * 32, v);
+        if (c == 3) {
+          fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(drained0 + 8 * group);
+        }
+        uint32_t out[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) out[i] = none ? 0u : f32x2_to_bf16x2_rne(__fmul_rn(v[2 * i], scale), __fmul_rn(v[2 * i + 1], scale));
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          st_shared16(staging + lane * kFewDwRow + c * 64 + i * 16, out[4 * i], out[4 * i + 1], out[4 * i + 2], out[4 * i + 3]);
+      }
+      store_fence();
+      const int row = m * 128 + quarter * 32 + lane, col = column * kTile + half * 128;
+      if (row < p.words && col < p.hidden) {
+        const int values = p.hidden - col < 128 ? p.hidden - col : 128;
+        bulk_store(p.gw + (p.word0 + row) * p.hidden + col, staging + lane * kFewDwRow, values * 2);
+      }
+      store_commit();
+    }
+    store_wait();
+    __syncwarp();
+  }
+  if (!ok) gave_up = 1;
+  fence_before();
+  __syncthreads();
+  if (gave_up && threadIdx.x == 0) *reinterpret_cast<volatile int64_t*>(p.report + 1) = 1;
+  fence_after();
+  if (warp == 1) tmem_free(tmem, 512);
+}
+
 // ------------------------------------------------------------- packing of rows
 constexpr int kScanThreads = 1024;
 
@@ -954,7 +1095,7 @@ lce_pack_kernel(const PackArgs a, const int* __restrict__ index, const int* __re
 }
 
 // Both in one launch for up to kScanPackRows rows: every block looks through all labels (32 KB at
-// most, from L2) for the eight rows that it packs.  One row: 13 -> 7 us for the two.
+// most, from L2) for the eight rows that it packs. One row: 7 us, as two launches 13.
 constexpr int kScanPackRows = 4096, kScanPackBlockRows = 512;  // the latter: a block a row
 template <int THREADS>
 __global__ void __launch_bounds__(kPackThreads)
@@ -1227,6 +1368,15 @@ cudaError_t launch_few(const GemmParams& p, float* acc, int64_t tiles, cudaStrea
   return few_columns(p.rows) == 16 ? launch_few_of<PASS, 16>(p, acc, tiles, st) : launch_few_of<PASS, kLceFewRows>(p, acc, tiles, st);
 }
 
+cudaError_t launch_few_dw(const GemmParams& p, int64_t tiles, cudaStream_t st) {
+  if (tiles > (int64_t(1) << 30)) return cudaErrorInvalidValue;
+  static std::atomic<uint64_t> done{0};
+  const cudaError_t e = allow_smem(done, (const void*)lce_few_dw_kernel, kFewDwSmem);
+  if (e != cudaSuccess) return e;
+  count_launch();
+  return launch_behind(lce_few_dw_kernel, dim3((unsigned)(tiles < kNumSMs ? tiles : kNumSMs)), kGemmThreads, kFewDwSmem, st, p);
+}
+
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 int64_t tiles_of(int64_t n) { return (n + kTile - 1) / kTile; }
 
@@ -1354,6 +1504,7 @@ cudaError_t launch_lce_backward(const LceArgs& a, const LceGrad& g, cudaStream_t
   q.row_g = p.row_g;
   q.want_dh = g.gh != nullptr;
   q.want_dw = g.gw != nullptr;
+  q.gw = (uint16_t*)g.gw;
   // Half of a tile would be products with zeros (2000 rows of 64, 5000 words: 19.6 us, so 18.0).
   q.narrow = a.hidden <= kTile / 2;
   q.splits = g.splits;
@@ -1367,7 +1518,7 @@ cudaError_t launch_lce_backward(const LceArgs& a, const LceGrad& g, cudaStream_t
   if (!encode(is_few ? &p.b : &p.a, a.packed, a.hidden, p.padded, p.row_pitch, is_few ? columns : 128) ||
       !encode(is_few ? &p.a : &p.b, a.w, a.hidden, a.vocab, a.w_stride, 128) ||
       !encode(is_few ? &few.a : &q.b, a.w, a.hidden, a.vocab, a.w_stride, 64) || (q.want_dw && !encode(&q.b2, g.scaled, a.hidden, p.padded, p.row_pitch, 64)) ||
-      (q.want_dw && !encode(&q.out, g.gw, a.hidden, a.vocab, a.hidden, 32, 32)) ||
+      (q.want_dw && !is_few && !encode(&q.out, g.gw, a.hidden, a.vocab, a.hidden, 32, 32)) ||
       (q.want_dh && !direct && !encode_acc(&q.out_acc, g.acc, a.hidden, p.row_pitch, p.padded, g.splits)))
     return cudaErrorInvalidValue;
   for (int64_t i = 0; i < pieces; ++i) {
@@ -1388,6 +1539,10 @@ cudaError_t launch_lce_backward(const LceArgs& a, const LceGrad& g, cudaStream_t
       if ((e = launch_product<kLogitGrad>(p, tiles_of(a.rows) * tiles_of(p.words), st)) != cudaSuccess) return e;
     }
     p.scaled = p.gh = nullptr;  // the first piece has done it
+    if (is_few) {
+      if (q.want_dw && (e = launch_few_dw(q, (q.words + 127) / 128 * tiles_of(a.hidden), st)) != cudaSuccess) return e;
+      continue;
+    }
     const int64_t dh = q.want_dh ? tiles_of(a.rows) * tiles_of(a.hidden) * g.splits : 0;
     const int64_t dw = q.want_dw ? tiles_of(q.words) * tiles_of(a.hidden) : 0;
     if ((e = launch_product<kGrads>(q, dh + dw, st)) != cudaSuccess) return e;

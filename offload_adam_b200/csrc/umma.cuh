@@ -111,6 +111,10 @@ __device__ __forceinline__ void tma_store3(const CUtensorMap* map, uint32_t src,
                  ::"l"(map), "r"(x), "r"(y), "r"(z), "r"(src)
                  : "memory");
 }
+// `bytes`, a multiple of 16, between 16-byte aligned addresses.
+__device__ __forceinline__ void bulk_store(void* to, uint32_t src, uint32_t bytes) {
+  asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(to), "r"(src), "r"(bytes) : "memory");
+}
 __device__ __forceinline__ void store_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
 // until the sources may be written again / until the stores are done
 __device__ __forceinline__ void store_wait_read() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
