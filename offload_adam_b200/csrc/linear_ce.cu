@@ -1095,7 +1095,7 @@ lce_pack_kernel(const PackArgs a, const int* __restrict__ index, const int* __re
 }
 
 // Both in one launch for up to kScanPackRows rows: every block looks through all labels (32 KB at
-// most, from L2) for the eight rows that it packs. One row: 7 us, as two launches 13.
+// most, from L2) for the eight rows that it packs.  One row: 7 us, as two launches 13.
 constexpr int kScanPackRows = 4096, kScanPackBlockRows = 512;  // the latter: a block a row
 template <int THREADS>
 __global__ void __launch_bounds__(kPackThreads)

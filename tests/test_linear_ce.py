@@ -117,6 +117,16 @@ def test_pieces(n, hidden, vocab, piece):
     _check(*_inputs(n, hidden, vocab, "cuda"), "mean", piece=piece)
 
 
+# the head's gradient of few rows has tiles of 128 words and 256 columns, which a block takes along
+# the rows: shares that begin and end within a row of tiles, of one tile, of none; ends that are odd
+@gpu
+@pytest.mark.parametrize("ignored", [0.0, 0.6, 1.0])
+@pytest.mark.parametrize("n,hidden,vocab,piece", [(33, 1288, 9001, None), (64, 264, 20001, None), (1, 2056, 5121, None), (17, 776, 19000, 8192),
+                                                  (5, 4104, 1153, None), (64, 8, 30001, 16384), (48, 136, 18945, None)])
+def test_few_rows_and_many_words(n, hidden, vocab, piece, ignored):
+    _check(*_inputs(n, hidden, vocab, "cuda", ignored=ignored), "mean", piece=piece)
+
+
 @pytest.mark.parametrize("device", DEVICES)
 @pytest.mark.parametrize("n", [5, 70])
 def test_ignored_rows_take_no_part(n, device):
