@@ -91,7 +91,6 @@ struct GemmParams {
   const float *inv, *g;  // each may be null (1)
   int want_dh, want_dw;
   uint16_t* gw;               // few rows; otherwise by `out`
-  int narrow;            // at most 128 hidden columns: products of 128 columns
   int splits;
   int first;             // piece: its dh starts the sums
 };
@@ -109,6 +108,9 @@ struct Tile {
   int m, n;       // first row and column
   int k0, steps;  // first inner value, stages
   int split;
+  // kGrads: at most 128 hidden columns, so products of 128 columns (2000 rows of 64, 5000 words: 18.0 us
+  // for 19.6; 622 rows of 840, 32003 words, a fourth of the tiles: 72.3 for 73.4)
+  bool narrow;
 };
 
 // Tiles of a pass, and which of them a CTA pair takes.  Column tiles turn slower than up to kGroup
@@ -196,6 +198,7 @@ struct Plan {
     }
     x.m = m * kTile;
     x.n = n * kTile;
+    x.narrow = PASS == kGrads && p.hidden - x.n <= kTile / 2;
     return x;
   }
 };
@@ -453,13 +456,13 @@ lce_product_kernel(const __grid_constant__ GemmParams p) {
         const bool outer_a = PASS == kGrads && x.kind == 1, outer_b = PASS == kGrads;
         const CUtensorMap* ma = outer_a ? &p.a2 : &p.a;
         const CUtensorMap* mb = outer_a ? &p.b2 : &p.b;
-        const int am = x.m + rank * 128, bn = x.n + rank * (PASS == kGrads && p.narrow ? 64 : 128);
+        const int am = x.m + rank * 128, bn = x.n + rank * (x.narrow ? 64 : 128);
         // kLogitGrad: W's rows start at the piece; dh: so do the inner values of W
         const int b_row0 = PASS == kLogitGrad ? (int)p.word0 : 0, b_k0 = PASS == kGrads && x.kind == 0 ? (int)p.word0 : 0;
         for (int k = 0; k < x.steps; ++k, ++it) {
           const int s = it % kStages;
           if (!mbar_wait(empty0 + 8 * s, ((it / kStages) & 1) ^ 1)) { ok = false; break; }
-          if (rank == 0) mbar_expect_tx(full0 + 8 * s, PASS == kGrads && p.narrow ? 2 * kStageBytes - kHalfBytes : 2 * kStageBytes);
+          if (rank == 0) mbar_expect_tx(full0 + 8 * s, x.narrow ? 2 * kStageBytes - kHalfBytes : 2 * kStageBytes);
           const uint32_t at = stages + s * kStageBytes, bt = at + kHalfBytes, bar = lead_full0 + 8 * s;
           const int kk = x.k0 + k * kInner;
           if (outer_a) {
@@ -470,7 +473,7 @@ lce_product_kernel(const __grid_constant__ GemmParams p) {
           }
           if (outer_b) {
             tma_load_pair(bt, mb, bn, b_k0 + kk, bar);
-            if (!p.narrow) tma_load_pair(bt + kHalfBytes / 2, mb, bn + 64, b_k0 + kk, bar);
+            if (!x.narrow) tma_load_pair(bt + kHalfBytes / 2, mb, bn + 64, b_k0 + kk, bar);
           } else {
             tma_load_pair(bt, mb, kk, b_row0 + bn, bar);
           }
@@ -490,7 +493,7 @@ lce_product_kernel(const __grid_constant__ GemmParams p) {
         const Tile x = plan.at<PASS>(p, t);
         const bool outer_a = PASS == kGrads && x.kind == 1;
         constexpr bool outer_b = PASS == kGrads;
-        const uint32_t idesc = instruction(kTile, PASS == kGrads && p.narrow ? kTile / 2 : kTile, outer_a, outer_b);
+        const uint32_t idesc = instruction(kTile, x.narrow ? kTile / 2 : kTile, outer_a, outer_b);
         int k = 0;
         do {  // one chain; a tile of no stage has an empty one
           const int last = PASS == kStats && k + kChain < x.steps ? k + kChain : x.steps;
@@ -851,15 +854,16 @@ lce_few_kernel(const __grid_constant__ GemmParams p, float* acc) {
 }
 
 // dW of few rows: W's size to write, and products of a single stage for each tile, 128 words by 256
-// hidden columns.  What goes out in 256 bytes of a row at a time gets 6.1 TB/s, in the 128 bytes of
-// a tiled store 5.0, whatever computes it.  So a warp stages its 32 rows and 128 columns whole, rows
-// 272 bytes apart (free of bank conflicts), and each lane copies one.  A CTA takes consecutive
-// tiles along the rows of dW: d of its words stays in shared memory and is read once, the rows of h
-// come out of L2 again and again.  32 rows, hidden 8192, 128256 words: h takes 1 MB, d 16 MB, dW
-// 2.1 GB in 454 us (4.6 TB/s); with the rows of h kept and d read again 541, in the pair kernel 503.
-constexpr int kFewDwStages = 2, kFewDwRow = 272, kFewDwStaging = 32 * kFewDwRow;
-constexpr int kFewDwSmem = kFewDwStages * 2 * kHalfBytes + kHalfBytes + kEpilogueWarps * kFewDwStaging + 1024;
-__global__ void __launch_bounds__(kGemmThreads, 1)
+// hidden columns.  What goes out in 256 bytes of a row at a time or more gets 6.1 TB/s, in the 128
+// bytes of a tiled store 5.0, whatever computes it.  So four warps take a tile, each stages its 32 rows
+// whole, 528 bytes apart (free of bank conflicts), and each lane copies one.  A CTA takes
+// consecutive tiles along the rows of dW: d of its words stays in shared memory and is read once, the
+// rows of h come out of L2 again and again.  32 rows, hidden 8192, 128256 words (h 1 MB, d 16 MB, dW
+// 2.1 GB): 1370 us for loss and gradients, about 375 of them here; with the rows of h kept and d read
+// again, or in the pair kernel, 1460.
+constexpr int kFewDwStages = 2, kFewDwRow = 528, kFewDwStaging = 32 * kFewDwRow, kFewDwWarps = 8, kFewDwThreads = 64 + 32 * kFewDwWarps;
+constexpr int kFewDwSmem = kFewDwStages * 2 * kHalfBytes + kHalfBytes + kFewDwWarps * kFewDwStaging + 1024;
+__global__ void __launch_bounds__(kFewDwThreads, 1)
 lce_few_dw_kernel(const __grid_constant__ GemmParams p) {
   extern __shared__ uint8_t smem_raw[];
   __shared__ uint64_t full[kFewDwStages], empty[kFewDwStages], done[2], drained[2], d_full[1], d_empty[1];
@@ -877,7 +881,7 @@ lce_few_dw_kernel(const __grid_constant__ GemmParams p) {
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(done0 + 8 * i, 1);
-      mbar_init(drained0 + 8 * i, kEpilogueWarps / 2);
+      mbar_init(drained0 + 8 * i, kFewDwWarps / 2);
     }
     mbar_init(d_full0, 1);
     mbar_init(d_empty0, 1);
@@ -942,7 +946,7 @@ lce_few_dw_kernel(const __grid_constant__ GemmParams p) {
     }
     __syncwarp();
   } else {
-    const int quarter = warp & 3, half = ((warp - 2) >> 2) & 1, group = (warp - 2) >> 3;
+    const int quarter = warp & 3, group = (warp - 2) >> 2;
     const bool none = *p.count == 0;  // d and h are not there
     const float scale = all_scale(p);
     const uint32_t staging = d_at + kHalfBytes + (warp - 2) * kFewDwStaging;
@@ -952,14 +956,14 @@ lce_few_dw_kernel(const __grid_constant__ GemmParams p) {
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
       fence_after();
-      const uint32_t at = tmem + group * kTile + half * 128 + ((uint32_t)(quarter * 32) << 16);
+      const uint32_t at = tmem + group * kTile + ((uint32_t)(quarter * 32) << 16);
       store_wait_read();  // each lane its own row of the last tile
       __syncwarp();
 #pragma unroll 1
-      for (int c = 0; c < 4; ++c) {
+      for (int c = 0; c < 8; ++c) {
         float v[32];
         tmem_load32(at + c * 32, v);
-        if (c == 3) {
+        if (c == 7) {
           fence_before();
           __syncwarp();
           if (lane == 0) mbar_arrive(drained0 + 8 * group);
@@ -972,9 +976,9 @@ lce_few_dw_kernel(const __grid_constant__ GemmParams p) {
           st_shared16(staging + lane * kFewDwRow + c * 64 + i * 16, out[4 * i], out[4 * i + 1], out[4 * i + 2], out[4 * i + 3]);
       }
       store_fence();
-      const int row = m * 128 + quarter * 32 + lane, col = column * kTile + half * 128;
+      const int row = m * 128 + quarter * 32 + lane, col = column * kTile;
       if (row < p.words && col < p.hidden) {
-        const int values = p.hidden - col < 128 ? p.hidden - col : 128;
+        const int values = p.hidden - col < kTile ? p.hidden - col : kTile;
         bulk_store(p.gw + (p.word0 + row) * p.hidden + col, staging + lane * kFewDwRow, values * 2);
       }
       store_commit();
@@ -1374,7 +1378,7 @@ cudaError_t launch_few_dw(const GemmParams& p, int64_t tiles, cudaStream_t st) {
   const cudaError_t e = allow_smem(done, (const void*)lce_few_dw_kernel, kFewDwSmem);
   if (e != cudaSuccess) return e;
   count_launch();
-  return launch_behind(lce_few_dw_kernel, dim3((unsigned)(tiles < kNumSMs ? tiles : kNumSMs)), kGemmThreads, kFewDwSmem, st, p);
+  return launch_behind(lce_few_dw_kernel, dim3((unsigned)(tiles < kNumSMs ? tiles : kNumSMs)), kFewDwThreads, kFewDwSmem, st, p);
 }
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
@@ -1505,8 +1509,6 @@ cudaError_t launch_lce_backward(const LceArgs& a, const LceGrad& g, cudaStream_t
   q.want_dh = g.gh != nullptr;
   q.want_dw = g.gw != nullptr;
   q.gw = (uint16_t*)g.gw;
-  // Half of a tile would be products with zeros (2000 rows of 64, 5000 words: 19.6 us, so 18.0).
-  q.narrow = a.hidden <= kTile / 2;
   q.splits = g.splits;
   // few rows: `few` has the operands of dh, q those of dW alone
   const bool is_few = a.rows <= kLceFewRows;
