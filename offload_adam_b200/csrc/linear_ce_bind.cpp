@@ -32,7 +32,7 @@ int64_t row_stride(const Tensor& t) { return t.size(0) == 1 ? t.size(1) : t.stri
 // their number with the ticket, 1 / number.
 int64_t packed_bytes(int64_t rows, int64_t hidden) { return 2 * oab::lce_padded(rows) * oab::lce_row_pitch(hidden); }
 int64_t kept_bytes(int64_t rows, int64_t hidden) { return packed_bytes(rows, hidden) + 4 * (4 * rows + 4); }
-oab::LceArgs make_args(const Tensor& w, const Tensor& labels, const Tensor& kept, int64_t ignore) {
+oab::LceArgs make_args(const Tensor& w, const Tensor& labels, void* kept, int64_t ignore) {
   oab::LceArgs a;
   a.w = w.data_ptr();
   a.w_stride = row_stride(w);
@@ -41,8 +41,8 @@ oab::LceArgs make_args(const Tensor& w, const Tensor& labels, const Tensor& kept
   a.hidden = w.size(1);
   a.vocab = w.size(0);
   a.ignore = ignore;
-  a.packed = kept.data_ptr();
-  int* k = reinterpret_cast<int*>(static_cast<char*>(kept.data_ptr()) + packed_bytes(a.rows, a.hidden));
+  a.packed = kept;
+  int* k = reinterpret_cast<int*>(static_cast<char*>(kept) + packed_bytes(a.rows, a.hidden));
   a.index = k;
   a.label = k + a.rows;
   a.rest = reinterpret_cast<float*>(k + 2 * a.rows);
@@ -66,31 +66,33 @@ struct Scratch {
   T* at_byte(int64_t at) const { return reinterpret_cast<T*>(static_cast<char*>(memory.data_ptr()) + at); }
 };
 
+// The loss, and what backward needs of it if `keep`.
+Tensor run_forward(const Tensor& h, const Tensor& w, const Tensor& labels, int64_t reduction, int64_t ignore, Tensor* keep) {
+  c10::cuda::CUDAGuard guard(h.device());
+  oab::raise_loss_report();
+  const Tensor hc = rows_layout(h), wc = rows_layout(w);
+  const int64_t rows = h.size(0);
+  const auto f32 = h.options().dtype(at::kFloat);
+  Tensor loss = reduction == oab::kLceNone ? at::empty({rows}, f32) : at::empty({}, f32);
+  Scratch x;
+  const int64_t kept = x.add(keep != nullptr ? 0 : kept_bytes(rows, h.size(1)));
+  const int64_t part = x.add(4 * oab::lce_part_floats(rows, w.size(0))), picked = x.add(4 * rows), sums = x.add(8 * oab::lce_sum_doubles(rows));
+  x.take(h);
+  if (keep != nullptr) *keep = at::empty({kept_bytes(rows, h.size(1))}, h.options().dtype(at::kByte));
+  auto a = make_args(wc, labels, keep != nullptr ? keep->data_ptr() : x.at_byte<void>(kept), ignore);
+  a.h = hc.data_ptr();
+  a.h_stride = row_stride(hc);
+  ok(oab::launch_lce_forward(a, (int)reduction, x.at_byte<float>(part), x.at_byte<float>(picked), x.at_byte<double>(sums),
+                             loss.data_ptr<float>(), cur()),
+     "linear_cross_entropy");
+  return loss;
+}
+
 struct LinearCE : torch::autograd::Function<LinearCE> {
   static Tensor forward(AutogradContext* ctx, const Tensor& h, const Tensor& w, const Tensor& labels, int64_t reduction,
                         int64_t ignore, int64_t piece) {
-    TORCH_CHECK(h.is_cuda() && h.scalar_type() == at::kBFloat16 && h.dim() == 2 && w.scalar_type() == at::kBFloat16 && w.dim() == 2 &&
-                    w.size(1) == h.size(1) && h.size(1) % 8 == 0 && h.numel() > 0 && w.numel() > 0 && w.device() == h.device(),
-                "linear_cross_entropy: bf16 CUDA matrices of one device, rows of a multiple of 8");
-    TORCH_CHECK(labels.scalar_type() == at::kLong && labels.dim() == 1 && labels.size(0) == h.size(0) && labels.device() == h.device() &&
-                    labels.is_contiguous(), "linear_cross_entropy: one contiguous int64 label per row");
-    TORCH_CHECK(reduction >= 0 && reduction <= 2 && piece >= 0, "linear_cross_entropy: reduction or piece");
-    c10::cuda::CUDAGuard guard(h.device());
-    oab::raise_loss_report();
-    const Tensor hc = rows_layout(h), wc = rows_layout(w);
-    const int64_t rows = h.size(0);
-    const auto f32 = h.options().dtype(at::kFloat);
-    Tensor kept = at::empty({kept_bytes(rows, h.size(1))}, h.options().dtype(at::kByte));
-    Tensor loss = reduction == oab::kLceNone ? at::empty({rows}, f32) : at::empty({}, f32);
-    Scratch x;
-    const int64_t part = x.add(4 * oab::lce_part_floats(rows, w.size(0))), picked = x.add(4 * rows), sums = x.add(8 * oab::lce_sum_doubles(rows));
-    x.take(h);
-    auto a = make_args(wc, labels, kept, ignore);
-    a.h = hc.data_ptr();
-    a.h_stride = row_stride(hc);
-    ok(oab::launch_lce_forward(a, (int)reduction, x.at_byte<float>(part), x.at_byte<float>(picked), x.at_byte<double>(sums),
-                               loss.data_ptr<float>(), cur()),
-       "linear_cross_entropy");
+    Tensor kept;
+    Tensor loss = run_forward(h, w, labels, reduction, ignore, &kept);
     ctx->save_for_backward({w, labels, kept});
     ctx->saved_data["reduction"] = reduction;
     ctx->saved_data["ignore"] = ignore;
@@ -140,7 +142,7 @@ struct LinearCE : torch::autograd::Function<LinearCE> {
       x.gw = gw.data_ptr();
       x.scaled = t.at_byte<void>(scaled);
     }
-    ok(oab::launch_lce_backward(make_args(wc, lc, kept, ignore), x, cur()), "linear_cross_entropy backward");
+    ok(oab::launch_lce_backward(make_args(wc, lc, kept.data_ptr(), ignore), x, cur()), "linear_cross_entropy backward");
     if (graph) {
       const auto last = std::make_shared<torch::autograd::DelayedError>("linear_cross_entropy has no second derivative", 2);
       for (Tensor* t : {&gh, &gw})
@@ -154,15 +156,37 @@ struct LinearCE : torch::autograd::Function<LinearCE> {
   }
 };
 
+// Whether the kernels take these; the rest is the caller's, its refusals too.
+bool takes(const Tensor& h, const Tensor& w, const Tensor& labels) {
+  for (const Tensor* t : {&h, &w, &labels})
+    if (!t->defined() || !t->is_cuda() || t->layout() != at::kStrided || t->key_set().has(c10::DispatchKey::Python)) return false;
+  if (h.scalar_type() != at::kBFloat16 || w.scalar_type() != at::kBFloat16 || labels.scalar_type() != at::kLong || h.dim() < 1 || w.dim() != 2 ||
+      h.size(-1) != w.size(1) || labels.sizes() != h.sizes().slice(0, h.dim() - 1) || h.device() != w.device() || h.device() != labels.device())
+    return false;
+  const int64_t rows = labels.numel(), hidden = w.size(1), vocab = w.size(0);
+  return rows > 0 && rows <= oab::kLceMaxRows && hidden % 8 == 0 && hidden > 0 && hidden <= oab::kLceMaxHidden && vocab > 0 &&
+         vocab <= oab::kLceMaxVocab;
+}
+
+// Unless `required`, None for what the kernels do not take.
+py::object linear_ce(const Tensor& h, const Tensor& w, const Tensor& labels, int64_t reduction, int64_t ignore, int64_t piece, bool required) {
+  TORCH_CHECK(reduction >= 0 && reduction <= 2 && piece >= 0, "linear_cross_entropy: reduction or piece");
+  if (!takes(h, w, labels)) {
+    TORCH_CHECK(!required, "linear_cross_entropy: the kernels take bf16 CUDA tensors of one device, rows of a multiple of 8, an int64 label each");
+    return py::none();
+  }
+  const Tensor rows = h.dim() == 2 ? h : h.reshape({-1, h.size(-1)});
+  const Tensor each = labels.dim() == 1 && labels.is_contiguous() ? labels : labels.reshape(-1).contiguous();
+  const bool graph = at::GradMode::is_enabled() && (rows.requires_grad() || w.requires_grad());
+  Tensor loss = graph ? LinearCE::apply(rows, w, each, reduction, ignore, piece) : run_forward(rows, w, each, reduction, ignore, nullptr);
+  if (reduction == oab::kLceNone && labels.dim() != 1) loss = loss.view(labels.sizes());
+  return py::cast(loss);
+}
+
 }  // namespace
 
 void bind_linear_ce(py::module_& m) {
-  m.def("linear_ce", [](const Tensor& h, const Tensor& w, const Tensor& labels, int64_t reduction, int64_t ignore, int64_t piece) {
-    return LinearCE::apply(h, w, labels, reduction, ignore, piece);
-  });
-  m.def("linear_ce_takes", [](int64_t rows, int64_t hidden, int64_t vocab) {
-    return rows > 0 && rows <= oab::kLceMaxRows && hidden % 8 == 0 && hidden > 0 && hidden <= oab::kLceMaxHidden && vocab > 0 &&
-           vocab <= oab::kLceMaxVocab;
-  });
+  m.def("linear_ce", &linear_ce, py::arg("h"), py::arg("w"), py::arg("labels"), py::arg("reduction"), py::arg("ignore"), py::arg("piece"),
+        py::arg("required") = true);
   m.def("linear_ce_piece", &oab::lce_default_piece, py::arg("rows"), py::arg("hidden"), py::arg("vocab"));
 }

@@ -14,7 +14,7 @@ from __future__ import annotations
 import torch
 
 from .. import _ext
-from .dispatch import use_kernels
+from .dispatch import _PLAIN, eager
 
 _REDUCTIONS = {"none": 0, "mean": 1, "sum": 2}
 _PIECE = 16384  # words at a time in the operations of PyTorch
@@ -122,6 +122,12 @@ def linear_cross_entropy(h, weight, labels, reduction="mean", ignore_index=-100,
         raise ValueError(f"reduction must be one of {tuple(_REDUCTIONS)}, not {reduction!r}")
     if piece is not None and (not isinstance(piece, int) or isinstance(piece, bool) or piece < 0):
         raise ValueError(f"piece must be None or a whole number of words, not {piece!r}")
+    # the usual call is looked over in C++: short ones are bound by the host
+    if type(h) in _PLAIN and type(weight) in _PLAIN and type(labels) is torch.Tensor and h.is_cuda and eager():
+        out = _ext.load(required=True).linear_ce(h, weight, labels, _REDUCTIONS[reduction], ignore_index, piece or 0,
+                                                 False)
+        if out is not None:
+            return out
     if hasattr(weight, "_payload"):
         raise TypeError("linear_cross_entropy: the head's weight is packed; leave lm_head out of the quantization")
     if weight.dim() != 2 or h.dim() < 1 or h.shape[-1] != weight.shape[1] or weight.numel() == 0:
@@ -138,10 +144,5 @@ def linear_cross_entropy(h, weight, labels, reduction="mean", ignore_index=-100,
     shape = labels.shape
     if len(shape) != 1:
         h, labels = h.reshape(-1, h.shape[-1]), labels.reshape(-1)
-    if (use_kernels(h, weight) and type(labels) is torch.Tensor
-            and _ext.load(required=True).linear_ce_takes(*h.shape, weight.shape[0])):
-        out = _ext.load(required=True).linear_ce(h, weight, labels.contiguous(), _REDUCTIONS[reduction], ignore_index,
-                                                 piece or 0)
-    else:
-        out = _PlainLinearCE.apply(h, weight, labels, reduction, ignore_index, piece or _PIECE)
+    out = _PlainLinearCE.apply(h, weight, labels, reduction, ignore_index, piece or _PIECE)
     return out.view(shape) if reduction == "none" and len(shape) != 1 else out
