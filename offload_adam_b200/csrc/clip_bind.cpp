@@ -23,8 +23,7 @@ struct Gradients {
   std::vector<std::pair<Tensor, Tensor>> scattered;  // gradient, its copy
 
   Gradients(const std::vector<Tensor>& grads, bool write) {
-    std::vector<std::pair<Tensor, oab::ClipEntry>> all;
-    all.reserve(grads.size());
+    entries.reserve(grads.size());
     for (const Tensor& g : grads) {
       TORCH_CHECK(g.is_cuda() && g.device() == grads[0].device(), "gradients must be on one CUDA device");
       const auto t = g.scalar_type();
@@ -98,9 +97,10 @@ Tensor grad_norm(const std::vector<Tensor>& grads, int64_t norm, double max_norm
   return out;
 }
 
-// The same for the gradients of `params`; None (and nothing done) when one of them is not a plain
-// gradient of one CUDA device that the kernels take, or when there is none.
-py::object param_grad_norm(const py::list& params, int64_t norm, double max_norm, bool scale) {
+// The same for the gradients of `params`, the norm alone unless `both`; None (and nothing done) when
+// one of them is not a plain gradient of one CUDA device that the kernels take, or when there is none.
+py::object param_grad_norm(const py::list& params, int64_t norm, double max_norm, bool scale, bool both) {
+  at::NoGradGuard no_grad;
   std::vector<Tensor> grads;
   grads.reserve(params.size());
   for (const py::handle& h : params) {
@@ -114,7 +114,8 @@ py::object param_grad_norm(const py::list& params, int64_t norm, double max_norm
     grads.push_back(g);
   }
   if (grads.empty()) return py::none();
-  return py::cast(grad_norm(grads, norm, max_norm, scale));
+  const Tensor out = grad_norm(grads, norm, max_norm, scale);
+  return py::cast(both ? out : out.select(0, 1));
 }
 
 // The gradients times `coef`, one fp32 value on their device.
@@ -132,6 +133,7 @@ void grad_scale(const std::vector<Tensor>& grads, const Tensor& coef) {
 
 void bind_clip(py::module_& m) {
   m.def("grad_norm", &grad_norm, py::arg("grads"), py::arg("norm"), py::arg("max_norm"), py::arg("scale"));
-  m.def("param_grad_norm", &param_grad_norm, py::arg("params"), py::arg("norm"), py::arg("max_norm"), py::arg("scale"));
+  m.def("param_grad_norm", &param_grad_norm, py::arg("params"), py::arg("norm"), py::arg("max_norm"), py::arg("scale"),
+        py::arg("both") = true);
   m.def("grad_scale", &grad_scale, py::arg("grads"), py::arg("coef"));
 }

@@ -28,13 +28,15 @@ struct ClipTable {
   ClipEntry e[CAP];
 };
 
-__host__ __device__ __forceinline__ int per_vec(uint32_t dtype) { return dtype == kClipF32 ? 8 : 16; }
+// log2 of the values of a vector
+__host__ __device__ __forceinline__ int vec_shift(uint32_t dtype) { return dtype == kClipF32 ? 3 : 4; }
 // values in front of the first whole vector
 __host__ __device__ __forceinline__ int64_t head_of(const ClipEntry& e) {
-  const int64_t size = e.dtype == kClipF32 ? 4 : 2, over = (int64_t)(reinterpret_cast<uintptr_t>(e.p) & 31u) / size;
-  const int64_t head = over != 0 ? per_vec(e.dtype) - over : 0;
+  const int sh = vec_shift(e.dtype);
+  const int64_t over = (int64_t)((reinterpret_cast<uintptr_t>(e.p) & 31u) >> (5 - sh)), head = over != 0 ? (int64_t(1) << sh) - over : 0;
   return head < e.n ? head : e.n;
 }
+__host__ __device__ __forceinline__ int64_t vecs_of(const ClipEntry& e) { return (e.n - head_of(e)) >> vec_shift(e.dtype); }
 
 __device__ __forceinline__ float half_to_f32(uint32_t h) { return __half2float(__ushort_as_half((unsigned short)h)); }
 __device__ __forceinline__ float load_one(const ClipEntry& e, int64_t i) {
@@ -120,10 +122,11 @@ grad_norm_kernel(const __grid_constant__ ClipTable<CAP> table, double* partials)
   Sum<NORM> s;
   for (uint32_t c = blockIdx.x; c < table.chunks; c += gridDim.x) {
     const ClipEntry& e = entry_of(table, c);
-    const int64_t head = head_of(e), per = per_vec(e.dtype), vecs = (e.n - head) / per;
+    const int sh = vec_shift(e.dtype);
+    const int64_t head = head_of(e), vecs = vecs_of(e);
     const int64_t begin = (int64_t)(c - e.first_chunk) * table.chunk_vecs;
     const int64_t end = begin + table.chunk_vecs < vecs ? begin + table.chunk_vecs : vecs;
-    const char* base = reinterpret_cast<const char*>(e.p) + head * (32 / per);
+    const char* base = reinterpret_cast<const char*>(e.p) + (head << (5 - sh));
     const uint32_t dtype = e.dtype;
     for (int64_t v = begin + threadIdx.x; v < end; v += 4 * kThreads) {
       V8 r[4];
@@ -135,7 +138,7 @@ grad_norm_kernel(const __grid_constant__ ClipTable<CAP> table, double* partials)
         if (v + u * kThreads < end) take_vec<NORM>(s, r[u], dtype);
     }
     if (begin == 0) {  // what is in front of and behind the whole vectors
-      const int64_t tail = head + vecs * per;
+      const int64_t tail = head + (vecs << sh);
       if (threadIdx.x < 32 && threadIdx.x < head) s.take(load_one(e, threadIdx.x), false);
       if (threadIdx.x >= 32 && threadIdx.x < 64 && tail + threadIdx.x - 32 < e.n) s.take(load_one(e, tail + threadIdx.x - 32), false);
     }
@@ -203,10 +206,11 @@ grad_scale_kernel(const __grid_constant__ ClipTable<CAP> table, const double* __
   for (uint32_t k = blockIdx.x; k < table.chunks; k += gridDim.x) {
     const uint32_t chunk = table.chunks - 1 - k;
     const ClipEntry& e = entry_of(table, chunk);
-    const int64_t head = head_of(e), per = per_vec(e.dtype), vecs = (e.n - head) / per;
+    const int sh = vec_shift(e.dtype);
+    const int64_t head = head_of(e), vecs = vecs_of(e);
     const int64_t begin = (int64_t)(chunk - e.first_chunk) * table.chunk_vecs;
     const int64_t end = begin + table.chunk_vecs < vecs ? begin + table.chunk_vecs : vecs;
-    char* base = reinterpret_cast<char*>(e.p) + head * (32 / per);
+    char* base = reinterpret_cast<char*>(e.p) + (head << (5 - sh));
     const uint32_t dtype = e.dtype;
     for (int64_t v = begin + threadIdx.x; v < end; v += 2 * kThreads) {
       V8 r[2];
@@ -218,7 +222,7 @@ grad_scale_kernel(const __grid_constant__ ClipTable<CAP> table, const double* __
         if (v + u * kThreads < end) st32(base + (v + u * kThreads) * 32, scaled(r[u], dtype, c));
     }
     if (begin == 0) {
-      const int64_t tail = head + vecs * per;
+      const int64_t tail = head + (vecs << sh);
       if (threadIdx.x < 32 && threadIdx.x < head) scale_one(e, threadIdx.x, c);
       if (threadIdx.x >= 32 && threadIdx.x < 64 && tail + threadIdx.x - 32 < e.n) scale_one(e, tail + threadIdx.x - 32, c);
     }
@@ -232,16 +236,16 @@ unsigned fill(ClipTable<CAP>& t, const ClipEntry* entries, int count) {
   int64_t all = 0;
   for (int i = 0; i < count; ++i) {
     t.e[i] = entries[i];
-    all += (entries[i].n - head_of(entries[i])) / per_vec(entries[i].dtype);
+    all += vecs_of(entries[i]);
   }
   // 8 KB a chunk while that gives every block four at most, 64 KB beyond: 1.27 G bf16 values take
   // 392 us that way, 412 in chunks of 32 KB, 528 of 16 KB and 406 of 128 KB (clipped: 1240, 1254, 1341, 1265)
-  t.chunk_vecs = all <= int64_t(kBlocks) * 1024 ? 256 : 2048;
+  const int sh = all <= int64_t(kBlocks) * 1024 ? 8 : 11;
+  t.chunk_vecs = 1u << sh;
   int64_t chunks = 0;
   for (int i = 0; i < count; ++i) {
-    const int64_t vecs = (t.e[i].n - head_of(t.e[i])) / per_vec(t.e[i].dtype);
     t.e[i].first_chunk = (uint32_t)chunks;
-    const int64_t own = (vecs + t.chunk_vecs - 1) / t.chunk_vecs;
+    const int64_t own = (vecs_of(t.e[i]) + t.chunk_vecs - 1) >> sh;
     chunks += own < 1 ? 1 : own;
   }
   if (chunks >= (int64_t(1) << 31)) return 0;
@@ -279,15 +283,13 @@ cudaError_t each_launch(const ClipEntry* entries, int64_t count, const F& f) {
   for (int64_t at = 0; at < count; at += kClipMany) {
     const int k = (int)(count - at < kClipMany ? count - at : kClipMany);
     cudaError_t e;
-    if (k <= kClipFew) {
-      ClipTable<kClipFew> t;
-      const unsigned grid = fill(t, entries + at, k);
-      e = grid == 0 ? cudaErrorInvalidValue : f(t, grid, at);
-    } else {
-      ClipTable<kClipMany> t;
-      const unsigned grid = fill(t, entries + at, k);
-      e = grid == 0 ? cudaErrorInvalidValue : f(t, grid, at);
-    }
+    const auto take = [&](auto table) {
+      const unsigned grid = fill(table, entries + at, k);
+      return grid == 0 ? cudaErrorInvalidValue : f(table, grid, at);
+    };
+    if (k <= kClipFew) e = take(ClipTable<kClipFew>());
+    else if (k <= kClipSome) e = take(ClipTable<kClipSome>());
+    else e = take(ClipTable<kClipMany>());
     if (e != cudaSuccess) return e;
   }
   return cudaSuccess;

@@ -15,9 +15,9 @@ struct ClipEntry {
   uint32_t dtype;
   uint32_t first_chunk;  // filled in by the launch
 };
-// Tensors of a launch; the table travels as a kernel argument (the small one fits the 4 KB
-// that every launch may have, the large one the 32 KB of this architecture).
-constexpr int kClipFew = 160, kClipMany = 1300;
+// Tensors of a launch; the table travels as a kernel argument, 32 KB at most, and costs the host
+// its size: the tables are of 4, 11 and 31 KB.
+constexpr int kClipFew = 160, kClipSome = 448, kClipMany = 1300;
 
 // Doubles that the launches below need for `count` tensors: one partial per block.
 int64_t clip_partials(int64_t count);

@@ -67,25 +67,30 @@ def _norm_code(norm_type):
     return code
 
 
-def _run(parameters, norm_type, max_norm, scale):
-    """``{coefficient, norm}``, or None without a gradient."""
+def _run(parameters, norm_type, max_norm, scale, both=False):
+    """The norm, or with ``both`` ``{coefficient, norm}``; None without a gradient."""
     code = _norm_code(norm_type)
-    parameters = [parameters] if isinstance(parameters, torch.Tensor) else list(parameters)
+    if isinstance(parameters, torch.Tensor):
+        parameters = [parameters]
+    elif type(parameters) is not list:
+        parameters = list(parameters)
     # hundreds of small tensors are bound by what the host does for each of them: the usual case
-    # is looked over in C++ (291 tensors: 163 us a call without, 43 with it)
-    if torch.cuda.is_available() and eager():
-        out = _ext.load(required=True).param_grad_norm(parameters, code, max_norm, scale)
+    # is looked over in C++ (291 tensors: 163 us a call without, 28 with it)
+    if parameters and getattr(parameters[0], "is_cuda", False) and eager():
+        out = _ext.load(required=True).param_grad_norm(parameters, code, max_norm, scale, both)
         if out is not None:
             return out
     grads = _gradients(parameters)
     if not grads:
         return None
-    if _kernels(grads):
-        return _ext.load(required=True).grad_norm(grads, code, max_norm, scale)
-    return _plain(grads, float(norm_type), max_norm, scale)
+    with torch.no_grad():
+        if _kernels(grads):
+            out = _ext.load(required=True).grad_norm(grads, code, max_norm, scale)
+        else:
+            out = _plain(grads, float(norm_type), max_norm, scale)
+        return out if both else out[1]
 
 
-@torch.no_grad()
 def grad_norm(parameters, norm_type=2.0):
     """Norm of all gradients of ``parameters`` (a tensor or an iterable) as if they were one
     vector: an fp32 scalar on their device, without a synchronisation.
@@ -95,10 +100,9 @@ def grad_norm(parameters, norm_type=2.0):
     The sum is kept in fp64 and has the same bits in every run.
     """
     out = _run(parameters, norm_type, 0.0, False)
-    return torch.zeros(()) if out is None else out[1]
+    return torch.zeros(()) if out is None else out
 
 
-@torch.no_grad()
 def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=False, foreach=None):
     """Scales all gradients of ``parameters`` in place so that their norm (see
     :func:`grad_norm`) is at most ``max_norm``; returns the norm before.
@@ -111,24 +115,25 @@ def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=Fals
     max_norm = check_max_norm(max_norm)
     if not error_if_nonfinite:
         out = _run(parameters, norm_type, max_norm, True)
-        return torch.zeros(()) if out is None else out[1]
+        return torch.zeros(()) if out is None else out
     parameters = [parameters] if isinstance(parameters, torch.Tensor) else list(parameters)
-    out = _run(parameters, norm_type, max_norm, False)
+    out = _run(parameters, norm_type, max_norm, False, True)
     if out is None:
         return torch.zeros(())
     if not math.isfinite(out[1].item()):
         raise RuntimeError(f"the norm of order {norm_type} of the gradients is not finite; they are not clipped")
     grads = _gradients(parameters)
-    if _kernels(grads):
-        _ext.load(required=True).grad_scale(grads, out)
-    else:
-        _plain(grads, float(norm_type), max_norm, True)
-    return out[1]
+    with torch.no_grad():
+        if _kernels(grads):
+            _ext.load(required=True).grad_scale(grads, out)
+        else:
+            _plain(grads, float(norm_type), max_norm, True)
+        return out[1]
 
 
 @torch.no_grad()
 def clip_coefficient(parameters, max_norm):
     """``(min(1, max_norm / (norm + 1e-6)), norm)`` of the L2 norm, as device scalars; for a
     step that applies the coefficient itself.  ``(None, None)`` without a gradient."""
-    out = _run(parameters, 2.0, float(max_norm), False)
+    out = _run(parameters, 2.0, float(max_norm), False, True)
     return (None, None) if out is None else (out[:1], out[1])

@@ -84,6 +84,23 @@ def test_tables_of_every_size(sizes):
     _check_clip(params, 0.5 * _exact_norm(params, 2.0), 2.0)
 
 
+@gpu
+@pytest.mark.parametrize("count", [160, 448, 449, 1300])
+def test_tables_that_are_just_full(count):
+    params = _params([5, 33, 20000] * (count // 3) + [9] * (count % 3), (BF16, F32, F16), "cuda", shift=1)
+    _check_clip(params, 0.5 * _exact_norm(params, 1.0), 1.0)
+
+
+@gpu
+def test_parameters_of_any_container_and_order():
+    a = _params(SIZES, (BF16, F32), "cuda")
+    none, meta = torch.nn.Parameter(torch.zeros(3)), torch.nn.Parameter(torch.zeros(3, device="meta"))
+    want = grad_norm(a)
+    for each in (tuple(a), iter(a), [none] + a, [meta] + a + [none], a[::-1], dict(enumerate(a)).values()):
+        assert torch.equal(grad_norm(each), want)
+    assert torch.equal(grad_norm(a[1]), grad_norm([a[1]]))
+
+
 @pytest.mark.parametrize("device", DEVICES)
 def test_views_of_one_bucket_leave_their_neighbours(device):
     flat = torch.randn(5000, generator=torch.Generator().manual_seed(1)).to(BF16).to(device)
