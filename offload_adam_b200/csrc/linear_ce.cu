@@ -19,7 +19,8 @@
 // chains of 32 additions (512 terms; 256 for few rows) that the epilogue adds up.
 //
 // Forward: one product whose epilogue keeps, per row and 128 words, the maximum and the sum of
-// exponentials (8 bytes for 256 bytes of bf16 logits), and a small kernel that joins them.
+// exponentials (8 bytes for 256 bytes of bf16 logits), and a small kernel that joins them (of a few
+// rows the last block of the product).
 // Backward, for each piece of the vocabulary: the product again, whose epilogue writes the
 // gradient of the piece's logits in bf16, and one launch for both products that read it; dh is
 // summed over the pieces in fp32 and rounded once.
@@ -611,6 +612,73 @@ lce_product_kernel(const __grid_constant__ GemmParams p) {
   if (warp == 1) tmem_free_pair(tmem, 512);
 }
 
+// ------------------------------------------------------------ joining the sums
+struct JoinArgs {
+  const float *picked, *inv;
+  float *rest, *miss;
+  int* count;
+  int reduction, parts;
+  float* loss;  // null, of lce_few_kernel: a launch of its own joins
+};
+__device__ __forceinline__ void join(float& m, float& s, float m2, float s2) {
+  const float mn = fmaxf(m, m2), sh = finite_shift(mn);
+  s = __fadd_rn(__fmul_rn(s, expf(__fsub_rn(m, sh))), __fmul_rn(s2, expf(__fsub_rn(m2, sh))));
+  m = mn;
+}
+constexpr int kJoinLoads = 8;  // partials that a thread loads at a time
+// A row's partials are always joined in the same order, so its loss does not depend on the rows beside it:
+// slice i of kJoinSlices has every kJoinSlices-th partial from i on, and a warp joins the slices.
+// A thread's K of the slices, 32 apart.
+constexpr int kJoinSlices = 64;
+template <int K>
+__device__ __forceinline__ void join_slices(const float2* __restrict__ part, int64_t rows, int64_t row, int slice, int parts, float (&m)[K],
+                                            float (&s)[K]) {
+  for (int i = slice; i < parts; i += kJoinSlices * kJoinLoads) {
+    float2 x[K][kJoinLoads];
+#pragma unroll
+    for (int k = 0; k < K; ++k)
+#pragma unroll
+      for (int u = 0; u < kJoinLoads; ++u) {
+        const int at = i + k * 32 + u * kJoinSlices;
+        x[k][u] = at < parts ? __ldcg(part + (int64_t)at * rows + row) : make_float2(-INFINITY, 0.f);
+      }
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      float mn = m[k];
+#pragma unroll
+      for (int u = 0; u < kJoinLoads; ++u) mn = fmaxf(mn, x[k][u].x);
+      const float sh = finite_shift(mn);
+      s[k] = __fmul_rn(s[k], expf(__fsub_rn(m[k], sh)));
+#pragma unroll
+      for (int u = 0; u < kJoinLoads; ++u) s[k] = __fadd_rn(s[k], __fmul_rn(x[k][u].y, expf(__fsub_rn(x[k][u].x, sh))));
+      m[k] = mn;
+    }
+  }
+}
+// m, s: of slices `lane` and `lane + 32`; lane 0 gets the row's.
+__device__ __forceinline__ void join_warp(float& m, float& s, float m2, float s2) {
+  join(m, s, m2, s2);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    m2 = __shfl_xor_sync(0xffffffffu, m, o);
+    s2 = __shfl_xor_sync(0xffffffffu, s, o);
+    join(m, s, m2, s2);
+  }
+}
+// The loss of packed row `at` from the maximum and the sum of its other words; what backward needs.
+__device__ __forceinline__ double finish_row(const JoinArgs& j, int64_t at, const int* index, const int* label, float m, float s) {
+  const double z = j.picked[at], top = m, rest = s;
+  double loss_of;
+  // an infinite logit of the label's own has no loss, as in PyTorch
+  if (label[at] < 0 || z == INFINITY) loss_of = NAN;
+  else if (z >= top) loss_of = log1p(rest * exp(top - z));
+  else loss_of = top - z + log(rest + exp(z - top));
+  j.rest[at] = m == -INFINITY ? 0.f : (float)(top + log(rest));  // exp(-inf - rest) is 0, too, where all others are
+  j.miss[at] = (float)-expm1(-loss_of);
+  if (j.reduction == kLceNone) j.loss[index[at]] = (float)loss_of;
+  return loss_of;
+}
+
 // ---------------------------------------------------------- product, few rows
 // Up to kLceFewRows rows the products read W once and little else.  A pair's tile of 256 rows would
 // spend most of its products on rows that are not there: one row of 128256 words took 166 us of
@@ -619,6 +687,10 @@ lce_product_kernel(const __grid_constant__ GemmParams p) {
 // columns: lanes of tensor memory are words, columns are rows.  A stage is 18 or 24 KB, 16 of
 // them W, so that 12 or 9 stages keep more of W on its way.
 constexpr int kFewThreads = 64 + 128;
+// The statistics' last block joins their sums itself, which saves a launch, where its four warps need
+// two turns of 512 partials at most (32000 words of 1024, the loss alone, 8 rows: 28.6 us with the
+// launch, so 23.5; 16 rows, four turns: 28.8 and 29.8).
+constexpr bool few_join(int64_t rows, int64_t parts) { return (rows + 3) / 4 * ((parts + 511) / 512) <= 2; }
 template <int N>
 struct FewShape {
   static constexpr int kStage = kHalfBytes + N * 128, kCount = (220 * 1024) / kStage, kSmem = kCount * kStage + 1024;
@@ -639,7 +711,7 @@ __device__ __forceinline__ void tmem_load_rows(uint32_t at, float (&v)[N]) {
 
 template <int PASS, int N>
 __global__ void __launch_bounds__(kFewThreads, 1)
-lce_few_kernel(const __grid_constant__ GemmParams p, float* acc) {
+lce_few_kernel(const __grid_constant__ GemmParams p, float* acc, const JoinArgs j) {
   using S = FewShape<N>;
   extern __shared__ uint8_t smem_raw[];
   __shared__ uint64_t full[S::kCount], empty[S::kCount], done[S::kAccs], drained[S::kAccs];
@@ -650,6 +722,7 @@ lce_few_kernel(const __grid_constant__ GemmParams p, float* acc) {
   __shared__ float rest_of[N], scale_of[N];
   __shared__ int row_of[N];
   __shared__ float2 warp_part[4][N];
+  __shared__ double row_loss[PASS == kStats ? N : 1];
   const uint32_t stages = (smem_addr(smem_raw) + 1023u) & ~1023u;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t full0 = smem_addr(full), empty0 = smem_addr(empty), done0 = smem_addr(done), drained0 = smem_addr(drained);
@@ -842,6 +915,31 @@ lce_few_kernel(const __grid_constant__ GemmParams p, float* acc) {
           const float x = steps != 0 ? v[r] : 0.f;
           to[(int64_t)r * p.row_pitch] = p.first ? x : __fadd_rn(to[(int64_t)r * p.row_pitch], x);
         }
+      }
+    }
+  }
+  if (PASS == kStats && j.loss != nullptr && warp >= 2 && ok) {
+    // The block that is the last to come here joins the sums of all of them.
+    const int t = threadIdx.x - 64;
+    __threadfence();
+    asm volatile("bar.sync 1, 128;" ::: "memory");
+    if (t == 0) stop = atomicAdd(j.count + 1, 1) == (int)gridDim.x - 1;
+    asm volatile("bar.sync 1, 128;" ::: "memory");
+    if (stop) {
+      __threadfence();
+      for (int r = t >> 5; r < n_rows; r += 4) {
+        float m[2] = {-INFINITY, -INFINITY}, s[2] = {0.f, 0.f};
+        join_slices(p.part, p.rows, r, lane, j.parts, m, s);
+        join_warp(m[0], s[0], m[1], s[1]);
+        if (lane == 0) warp_part[0][r] = make_float2(m[0], s[0]);
+      }
+      asm volatile("bar.sync 1, 128;" ::: "memory");
+      if (t < n_rows) row_loss[t] = finish_row(j, t, p.index, p.label, warp_part[0][t].x, warp_part[0][t].y);
+      asm volatile("bar.sync 1, 128;" ::: "memory");
+      if (t == 0 && j.reduction != kLceNone) {
+        double sum = 0.0;
+        for (int i = 0; i < n_rows; ++i) sum += row_loss[i];
+        *j.loss = (float)(j.reduction == kLceMean ? sum * (double)*j.inv : sum);
       }
     }
   }
@@ -1156,83 +1254,43 @@ lce_scan_pack_kernel(const PackArgs a, const int64_t* __restrict__ labels, int r
   pack_row<THREADS>(a, first + own, n, source[own], source_label[own]);
 }
 
-// ------------------------------------------------------------ joining the sums
 // A block has 8 rows (the partials of 4 are one 32-byte sector) and 64 slices of the words; a thread
 // loads eight partials at a time.  One row of 128256 words: 1002 partials, 20 us with one load at a
 // time in 32 slices.
-constexpr int kJoinRows = 8, kJoinSlices = 64, kJoinThreads = kJoinRows * kJoinSlices, kJoinLoads = 8;
-__device__ __forceinline__ void join(float& m, float& s, float m2, float s2) {
-  const float mn = fmaxf(m, m2), sh = finite_shift(mn);
-  s = __fadd_rn(__fmul_rn(s, expf(__fsub_rn(m, sh))), __fmul_rn(s2, expf(__fsub_rn(m2, sh))));
-  m = mn;
-}
+constexpr int kJoinRows = 8, kJoinThreads = kJoinRows * kJoinSlices;
 __global__ void __launch_bounds__(kJoinThreads)
-lce_join_kernel(const float2* __restrict__ part, int parts, int64_t rows, const int* __restrict__ index,
-                const int* __restrict__ label, int* count, const float* __restrict__ picked, const float* __restrict__ inv,
-                float* rest_out, float* miss, int reduction, double* sums, float* loss) {
+lce_join_kernel(const float2* __restrict__ part, int64_t rows, const int* __restrict__ index, const int* __restrict__ label,
+                const JoinArgs j, double* sums) {
   __shared__ float sm[kJoinSlices][kJoinRows], ss[kJoinSlices][kJoinRows];
   __shared__ double one[kJoinRows];
   __shared__ int is_last;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   grid_release();
   grid_wait();
-  const int n = *count, of = threadIdx.x % kJoinRows, slice = threadIdx.x / kJoinRows;
+  const int n = *j.count, of = threadIdx.x % kJoinRows, slice = threadIdx.x / kJoinRows;
   const int64_t row = (int64_t)blockIdx.x * kJoinRows + of;
-  float m = -INFINITY, s = 0.f;
-  if (row < n) {
-    for (int i = slice; i < parts; i += kJoinSlices * kJoinLoads) {
-      float2 x[kJoinLoads];
-      float mn = m;
-#pragma unroll
-      for (int u = 0; u < kJoinLoads; ++u) {
-        const int at = i + u * kJoinSlices;
-        x[u] = at < parts ? part[(int64_t)at * rows + row] : make_float2(-INFINITY, 0.f);
-      }
-#pragma unroll
-      for (int u = 0; u < kJoinLoads; ++u) mn = fmaxf(mn, x[u].x);
-      const float sh = finite_shift(mn);
-      s = __fmul_rn(s, expf(__fsub_rn(m, sh)));
-#pragma unroll
-      for (int u = 0; u < kJoinLoads; ++u) s = __fadd_rn(s, __fmul_rn(x[u].y, expf(__fsub_rn(x[u].x, sh))));
-      m = mn;
-    }
-  }
-  sm[slice][of] = m;
-  ss[slice][of] = s;
+  float mine[1] = {-INFINITY}, sum[1] = {0.f};
+  if (row < n) join_slices(part, rows, row, slice, j.parts, mine, sum);
+  sm[slice][of] = mine[0];
+  ss[slice][of] = sum[0];
   __syncthreads();
   if (warp < kJoinRows) {  // warp w finishes the block's row w
-    m = sm[lane][warp];
-    s = ss[lane][warp];
-    join(m, s, sm[lane + 32][warp], ss[lane + 32][warp]);
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-      const float m2 = __shfl_xor_sync(0xffffffffu, m, o), s2 = __shfl_xor_sync(0xffffffffu, s, o);
-      join(m, s, m2, s2);
-    }
+    float m = sm[lane][warp], s = ss[lane][warp];
+    join_warp(m, s, sm[lane + 32][warp], ss[lane + 32][warp]);
     const int64_t at = (int64_t)blockIdx.x * kJoinRows + warp;
     if (lane == 0) {
-      double loss_of = 0.0;
-      if (at < n) {
-        const double z = picked[at], top = m, rest = s;
-        // an infinite logit of the label's own has no loss, as in PyTorch
-        if (label[at] < 0 || z == INFINITY) loss_of = NAN;
-        else if (z >= top) loss_of = log1p(rest * exp(top - z));
-        else loss_of = top - z + log(rest + exp(z - top));
-        rest_out[at] = m == -INFINITY ? 0.f : (float)(top + log(rest));  // exp(-inf - rest) is 0, too, where all others are
-        miss[at] = (float)-expm1(-loss_of);
-        if (reduction == kLceNone) loss[index[at]] = (float)loss_of;
-      }
+      const double loss_of = at < n ? finish_row(j, at, index, label, m, s) : 0.0;
       one[warp] = loss_of;
     }
   }
-  if (reduction == kLceNone) return;
+  if (j.reduction == kLceNone) return;
   __syncthreads();
   if (threadIdx.x == 0) {  // the same order whatever the blocks' order
     double t = 0.0;
     for (int i = 0; i < kJoinRows; ++i) t += one[i];
     sums[blockIdx.x] = t;
     __threadfence();
-    is_last = atomicAdd(count + 1, 1) == (int)gridDim.x - 1;
+    is_last = atomicAdd(j.count + 1, 1) == (int)gridDim.x - 1;
   }
   __syncthreads();
   if (is_last && warp == 0) {
@@ -1241,7 +1299,7 @@ lce_join_kernel(const float2* __restrict__ part, int parts, int64_t rows, const 
     for (int i = lane; i < (int)gridDim.x; i += 32) t += __ldcg(sums + i);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
-    if (lane == 0) *loss = (float)(reduction == kLceMean ? t * (double)*inv : t);
+    if (lane == 0) *j.loss = (float)(j.reduction == kLceMean ? t * (double)*j.inv : t);
   }
 }
 
@@ -1356,20 +1414,20 @@ cudaError_t launch_product(const GemmParams& p, int64_t tiles, cudaStream_t st) 
 }
 
 template <int PASS, int N>
-cudaError_t launch_few_of(const GemmParams& p, float* acc, int64_t tiles, cudaStream_t st) {
+cudaError_t launch_few_of(const GemmParams& p, float* acc, const JoinArgs& j, int64_t tiles, cudaStream_t st) {
   constexpr int smem = FewShape<N>::kSmem;
   static std::atomic<uint64_t> done{0};
   const cudaError_t e = allow_smem(done, (const void*)lce_few_kernel<PASS, N>, smem);
   if (e != cudaSuccess) return e;
   count_launch();
-  return launch_behind(lce_few_kernel<PASS, N>, dim3((unsigned)(tiles < kNumSMs ? tiles : kNumSMs)), kFewThreads, smem, st, p, acc);
+  return launch_behind(lce_few_kernel<PASS, N>, dim3((unsigned)(tiles < kNumSMs ? tiles : kNumSMs)), kFewThreads, smem, st, p, acc, j);
 }
 // 16 columns keep three more stages in flight and shorten the epilogue; up to 64 rows otherwise.
 constexpr int few_columns(int64_t rows) { return rows <= 16 ? 16 : kLceFewRows; }
 template <int PASS>
-cudaError_t launch_few(const GemmParams& p, float* acc, int64_t tiles, cudaStream_t st) {
+cudaError_t launch_few(const GemmParams& p, float* acc, const JoinArgs& j, int64_t tiles, cudaStream_t st) {
   if (tiles > (int64_t(1) << 30)) return cudaErrorInvalidValue;
-  return few_columns(p.rows) == 16 ? launch_few_of<PASS, 16>(p, acc, tiles, st) : launch_few_of<PASS, kLceFewRows>(p, acc, tiles, st);
+  return few_columns(p.rows) == 16 ? launch_few_of<PASS, 16>(p, acc, j, tiles, st) : launch_few_of<PASS, kLceFewRows>(p, acc, j, tiles, st);
 }
 
 cudaError_t launch_few_dw(const GemmParams& p, int64_t tiles, cudaStream_t st) {
@@ -1434,13 +1492,17 @@ cudaError_t launch_lce_forward(const LceArgs& a, int reduction, float* part, flo
   common_params(p, a);
   p.words = (int)a.vocab;
   p.part = reinterpret_cast<float2*>(part);
-  int parts = (int)(2 * tiles_of(a.vocab));
-  if (a.rows <= kLceFewRows) {
+  const bool few = a.rows <= kLceFewRows;
+  p.index = a.index;
+  JoinArgs j{picked, a.inv, a.rest, a.miss, a.count, reduction, (int)(few ? (a.vocab + 127) / 128 : 2 * tiles_of(a.vocab)), loss};
+  if (few) {
     if (!encode(&p.a, a.w, a.hidden, a.vocab, a.w_stride, 128) ||
         !encode(&p.b, a.packed, a.hidden, p.padded, p.row_pitch, few_columns(a.rows)))
       return cudaErrorInvalidValue;
-    parts = (int)((a.vocab + 127) / 128);
-    e = launch_few<kStats>(p, nullptr, parts, st);
+    const bool own = few_join(a.rows, j.parts);
+    JoinArgs none{};
+    e = launch_few<kStats>(p, nullptr, own ? j : none, j.parts, st);
+    if (e != cudaSuccess || own) return e;
   } else {
     if (!encode(&p.a, a.packed, a.hidden, p.padded, p.row_pitch, 128) || !encode(&p.b, a.w, a.hidden, a.vocab, a.w_stride, 128))
       return cudaErrorInvalidValue;
@@ -1448,8 +1510,8 @@ cudaError_t launch_lce_forward(const LceArgs& a, int reduction, float* part, flo
   }
   if (e != cudaSuccess) return e;
   count_launch();
-  return launch_behind(lce_join_kernel, dim3((unsigned)lce_sum_doubles(a.rows)), kJoinThreads, 0, st, p.part, parts, a.rows, a.index,
-                       a.label, a.count, picked, a.inv, a.rest, a.miss, reduction, sums, loss);
+  return launch_behind(lce_join_kernel, dim3((unsigned)lce_sum_doubles(a.rows)), kJoinThreads, 0, st, p.part, a.rows, a.index, a.label, j,
+                       sums);
 }
 
 int64_t lce_default_piece(int64_t rows, int64_t hidden, int64_t vocab) {
@@ -1533,8 +1595,8 @@ cudaError_t launch_lce_backward(const LceArgs& a, const LceGrad& g, cudaStream_t
       few.words = q.words;
       few.first = q.first;
       if (!encode(&few.b, g.d, q.words, p.padded, pitch, columns)) return cudaErrorInvalidValue;
-      if ((e = launch_few<kLogitGrad>(p, nullptr, (p.words + 127) / 128, st)) != cudaSuccess) return e;
-      if (few.want_dh && (e = launch_few<kGrads>(few, g.acc, (a.hidden + 127) / 128 * g.splits, st)) != cudaSuccess) return e;
+      if ((e = launch_few<kLogitGrad>(p, nullptr, JoinArgs{}, (p.words + 127) / 128, st)) != cudaSuccess) return e;
+      if (few.want_dh && (e = launch_few<kGrads>(few, g.acc, JoinArgs{}, (a.hidden + 127) / 128 * g.splits, st)) != cudaSuccess) return e;
     } else {
       if (!encode(&p.out, g.d, q.words, p.padded, pitch, 32, 32) || !encode(&q.a, g.d, q.words, p.padded, pitch, 128))
         return cudaErrorInvalidValue;

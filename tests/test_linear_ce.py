@@ -235,6 +235,26 @@ def test_layouts_in_place_and_copied(n):
     assert torch.equal(each[0], linear_cross_entropy(h, w, labels, reduction="none"))
 
 
+# one launch joins the sums of up to 8 rows (4 beyond 65536 words), another one those of more
+@gpu
+@pytest.mark.parametrize("reduction", ["mean", "sum", "none"])
+@pytest.mark.parametrize("n,vocab", [(1, 131072), (1, 131073), (4, 65537), (5, 65537), (8, 65536), (9, 65536), (8, 65537), (3, 100)])
+def test_rows_have_the_same_loss_in_any_company(n, vocab, reduction):
+    h, w, labels, _ = _inputs(n + 30, 16, vocab, "cuda", ignored=0.0)
+    all_rows = linear_cross_entropy(h, w, labels, reduction="none")
+    some = labels.clone()
+    some[n:] = -100
+    some[0] = -100
+    for x, y, want in ((h[:n], labels[:n], all_rows[:n]), (h[:n], some[:n], torch.where(some[:n] < 0, 0.0, all_rows[:n]))):
+        got = linear_cross_entropy(x, w, y, reduction=reduction)
+        rows = int((y >= 0).sum())
+        if reduction == "none":
+            assert torch.equal(got, want)
+        else:  # summed in fp64 and rounded once; the mean takes 1 / rows in fp32
+            exact = want.double().sum() / (max(1, rows) if reduction == "mean" else 1)
+            assert abs(got.double() - exact) <= exact * (2.0 ** -23 + 2.0 ** -24)
+
+
 @gpu
 @pytest.mark.parametrize("n", [5, 100])
 def test_logits_of_any_size(n):
