@@ -56,14 +56,28 @@ __device__ __forceinline__ bool mbar_try(uint32_t bar, uint32_t parity) {
       : "memory");
   return done != 0;
 }
-// A wait ends: false after kWaitTries tries.  One try takes at least tens of nanoseconds (the
-// hardware suspends it for up to microseconds), so the limit is far above any wait of a kernel
-// that makes progress and still well below a second or two.
-constexpr int kWaitTries = 1 << 22;
-__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity) {
-  for (int i = 0; i < kWaitTries; ++i)
+// A wait ends: false after two seconds, looked at every kWaitLook tries, or after kWaitTries.  The
+// longest tile that the sizes allow (2^24 rows into one tile of a head's gradient) takes a tenth of
+// a second.
+constexpr uint32_t kWaitLook = 1u << 14, kWaitTries = 1u << 28;
+constexpr uint64_t kWaitNanoseconds = 2000000000ull;
+__device__ __forceinline__ uint64_t nanoseconds() {
+  uint64_t t;
+  asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
+  return t;
+}
+__device__ __forceinline__ bool mbar_wait_long(uint32_t bar, uint32_t parity) {
+  const uint64_t begin = nanoseconds();
+  for (uint32_t i = 0; i < kWaitTries; ++i) {
     if (mbar_try(bar, parity)) return true;
+    if (i % kWaitLook == kWaitLook - 1 && nanoseconds() - begin > kWaitNanoseconds) return false;
+  }
   return false;
+}
+__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity) {
+  for (int i = 0; i < 64; ++i)
+    if (mbar_try(bar, parity)) return true;
+  return mbar_wait_long(bar, parity);
 }
 // The address of the same shared variable in CTA `rank` of the cluster.
 __device__ __forceinline__ uint32_t map_to_rank(uint32_t addr, uint32_t rank) {
