@@ -369,6 +369,41 @@ def test_captured_and_replayed(n):
         assert torch.equal(a, b)
 
 
+@gpu
+@pytest.mark.parametrize("reduction", ["mean", "none"])
+@pytest.mark.parametrize("n", [3, 8])
+def test_scores_of_few_rows_replayed_and_side_by_side(n, reduction):
+    """Without a graph, in one launch for the product and its sums: captured twice, replayed with other
+    labels, the two replays at the same time on two streams."""
+    jobs = [_inputs(n, 72, 5000, "cuda", ignored=0.3, seed=s) for s in range(2)]
+
+    def score(job):
+        with torch.no_grad():
+            return linear_cross_entropy(*job[:3], reduction=reduction)
+
+    streams, graphs, outs = [torch.cuda.Stream() for _ in jobs], [], []
+    for job, stream in zip(jobs, streams):
+        stream.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(stream):
+            score(job)
+            graphs.append(torch.cuda.CUDAGraph())
+            with torch.cuda.graph(graphs[-1], stream=stream):
+                outs.append(score(job))
+    for k in range(4):
+        torch.cuda.synchronize()
+        for job in jobs:
+            job[2].copy_(job[2].roll(1))
+        want = [score(job) for job in jobs]
+        torch.cuda.synchronize()
+        for _ in range(20):
+            for graph, stream in zip(graphs, streams):
+                with torch.cuda.stream(stream):
+                    graph.replay()
+        torch.cuda.synchronize()
+        for out, ref in zip(outs, want):
+            assert torch.equal(out, ref)
+
+
 @pytest.mark.parametrize("device", DEVICES)
 @pytest.mark.parametrize("n", [20, 70])
 def test_one_gradient_no_gradient_and_a_graph_used_twice(n, device):
