@@ -26,11 +26,6 @@ class _PlainLinearCE(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, h, weight, labels, reduction, ignore_index, piece):
-        with torch.autocast(h.device.type, enabled=False):
-            return _PlainLinearCE._forward(ctx, h, weight, labels, reduction, ignore_index, piece)
-
-    @staticmethod
-    def _forward(ctx, h, weight, labels, reduction, ignore_index, piece):
         wide = torch.float64 if h.dtype == torch.float64 else torch.float32
         valid = labels != ignore_index
         rows = valid.nonzero(as_tuple=True)[0]
@@ -136,7 +131,9 @@ def linear_cross_entropy(h, weight, labels, reduction="mean", ignore_index=-100,
         raise ValueError(f"linear_cross_entropy: int64 labels of shape {tuple(h.shape[:-1])} are needed, not "
                          f"{labels.dtype} of {tuple(labels.shape)}")
     if torch.is_autocast_enabled(h.device.type):
-        h, weight = (t.to(torch.get_autocast_dtype(h.device.type)) for t in (h, weight))
+        dtype = torch.get_autocast_dtype(h.device.type)
+        with torch.autocast(h.device.type, enabled=False):  # nothing inside is to be cast again
+            return linear_cross_entropy(h.to(dtype), weight.to(dtype), labels, reduction, ignore_index, piece)
     if not h.is_floating_point() or h.dtype != weight.dtype:
         raise ValueError(f"linear_cross_entropy: hidden states of {h.dtype} and a head of {weight.dtype}")
     if not (h.device == weight.device == labels.device):

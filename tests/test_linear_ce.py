@@ -500,6 +500,22 @@ def test_refusals_on_the_gpu():
     _check(h, w, labels, g, "mean")
 
 
+@gpu
+def test_kernels_run_under_autocast():
+    h, w, labels, g = _inputs(100, 64, 3000, "cuda")
+    want = _run(h, w, labels, g, "mean")
+    x, y = h.float().requires_grad_(True), w.float().requires_grad_(True)
+    C = _ext.load(required=True)
+    before = C.launch_count()
+    with torch.autocast("cuda", torch.bfloat16):
+        loss = linear_cross_entropy(x, y, labels)
+    assert C.launch_count() > before
+    loss.backward(g[0])
+    assert torch.equal(loss.detach(), want[0]) and torch.equal(x.grad, want[1].float()) and torch.equal(y.grad, want[2].float())
+    with torch.autocast("cuda", torch.bfloat16), pytest.raises(ValueError, match="one device"):
+        linear_cross_entropy(x, y, labels.cpu())
+
+
 @pytest.mark.parametrize("device", DEVICES)
 def test_under_autocast(device):
     h, w, labels, g = _inputs(40, 64, 300, device)
