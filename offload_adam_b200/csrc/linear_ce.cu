@@ -300,7 +300,7 @@ __device__ __forceinline__ void prepare_rows(const GemmParams& p, int n_rows, in
 
 template <class Release>
 __device__ __forceinline__ void logit_grad_tile(const GemmParams& p, const Tile& x, uint32_t tmem, int row, int half, uint32_t staging,
-                                                int lane, const RowValues& values, const Release& release) {
+                                                int lane, const RowValues& values, bool counts, const Release& release) {
   const int lab = values.label >= 0 ? (int)(values.label - p.word0) : -1;
   const float rest = values.rest;
 #pragma unroll 1
@@ -316,6 +316,12 @@ __device__ __forceinline__ void logit_grad_tile(const GemmParams& p, const Tile&
 #pragma unroll
       for (int i = 0; i < 32; ++i)
         if (i == hit) v[i] = -1.f;
+    }
+    // the zero rows behind the last one, which pad the inner dimension of dW: where a word of W holds an
+    // infinity their logits are NaN
+    if (!counts) {
+#pragma unroll
+      for (int i = 0; i < 32; ++i) v[i] = 0.f;
     }
     stage_bf16(staging, lane, v);
     if (lane == 0) {
@@ -596,7 +602,7 @@ lce_product_kernel(const __grid_constant__ GemmParams p) {
         }
         if (row < n_rows) p.part[(int64_t)(x.n / 128 + half) * p.rows + row] = join2(both[0], both[1]);
       }
-      if (PASS == kLogitGrad) logit_grad_tile(p, x, at, row, half, staging, lane, values, release);
+      if (PASS == kLogitGrad) logit_grad_tile(p, x, at, row, half, staging, lane, values, row < n_rows, release);
       if (PASS == kGrads && x.kind == 0) dh_tile(p, x, at, row, n_rows, half, scale, staging, lane, release);
       if (PASS == kGrads && x.kind == 1) dw_tile(p, x, at, row, half, scale, staging, lane, release);
     }
