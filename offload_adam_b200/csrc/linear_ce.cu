@@ -11,9 +11,11 @@
 // statistics leave that word out; and with their m and s
 //     loss_i = log(1 + s exp(m - z_label)),    1 - p_label = 1 - exp(-loss_i)
 // in fp64.  The gradient of the logits is held apart from its size: with q_i = 1 - p_label,
-//     d_ij = q_i g_i (exp(z_ij - rest_i) - [j = label_i]),    rest_i = log sum_{j != label} exp z_ij
+//     d_ij = q_i g_i (exp(z_ij - m_i) / s_i - [j = label_i]),    over the other words, as above
 // so the label's entry, which most of a row's gradient hangs on, is -1 exactly in bf16; q_i g_i is
 // applied to the fp32 sums of dh, and to the rows of h that go into dW (bf16, rounded once more).
+// m and log s stay two numbers: their sum would lose the latter beside logits of 1e9, or of a mask's
+// lowest value, and each word of such a row would have the whole of it.
 // tcgen05 cuts off what it adds to an accumulator, towards zero each time: logits of 4096 terms came
 // out 1e-5 too small, the losses of unsure rows 2.5e-5 off.  So the statistics take their logits in
 // chains of 32 additions (512 terms; 256 for few rows) that the epilogue adds up.
@@ -77,7 +79,7 @@ struct GemmParams {
   // kStats
   float2* part;
   // kLogitGrad
-  const float* rest;
+  const float *top, *rest;
   const float *miss, *row_g;  // the latter by row, or null
   const int* index;
   const uint16_t* packed;
@@ -96,12 +98,16 @@ struct GemmParams {
   int first;             // piece: its dh starts the sums
 };
 
-// off by about (|x| + 4) 2^-24 of its value
-__device__ __forceinline__ float exp_of(float x) {
+// exp_of is off by about (|x| + 4) 2^-24 of its value
+__device__ __forceinline__ float exp2_of(float x) {
   float r;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(__fmul_rn(x, 1.4426950408889634f)));
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
   return r;
 }
+constexpr float kLog2E = 1.4426950408889634f;
+__device__ __forceinline__ float exp_of(float x) { return exp2_of(__fmul_rn(x, kLog2E)); }
+// the softmax of a logit over the words that are not the label; `rest` in base 2
+__device__ __forceinline__ float share_of(float z, float top, float rest) { return exp2_of(__fmaf_rn(__fsub_rn(z, top), kLog2E, -rest)); }
 __device__ __forceinline__ float finite_shift(float m) { return m == -INFINITY ? 0.f : m; }
 
 struct Tile {
@@ -214,14 +220,17 @@ struct Plan {
 
 struct RowValues {  // of the packed row that a thread has in a tile
   int label;
-  float rest;
+  float top, rest;
 };
 template <int PASS>
 __device__ __forceinline__ RowValues row_values(const GemmParams& p, int row, int n_rows) {
-  RowValues r{-1, INFINITY};
+  RowValues r{-1, 0.f, INFINITY};
   if (PASS != kGrads && row < n_rows) {
     r.label = p.label[row];
-    if (PASS == kLogitGrad) r.rest = p.rest[row];
+    if (PASS == kLogitGrad) {
+      r.top = p.top[row];
+      r.rest = p.rest[row];
+    }
   }
   return r;
 }
@@ -302,7 +311,7 @@ template <class Release>
 __device__ __forceinline__ void logit_grad_tile(const GemmParams& p, const Tile& x, uint32_t tmem, int row, int half, uint32_t staging,
                                                 int lane, const RowValues& values, bool counts, const Release& release) {
   const int lab = values.label >= 0 ? (int)(values.label - p.word0) : -1;
-  const float rest = values.rest;
+  const float top = values.top, rest = values.rest;
 #pragma unroll 1
   for (int c = 0; c < 4; ++c) {
     float v[32];
@@ -310,7 +319,7 @@ __device__ __forceinline__ void logit_grad_tile(const GemmParams& p, const Tile&
     if (c == 3) release();
     const int col = x.n + half * 128 + c * 32;
 #pragma unroll
-    for (int i = 0; i < 32; ++i) v[i] = exp_of(__fsub_rn(v[i], rest));
+    for (int i = 0; i < 32; ++i) v[i] = share_of(v[i], top, rest);
     const int hit = lab - col;
     if (lab >= 0 && hit >= 0 && hit < 32) {
 #pragma unroll
@@ -621,7 +630,7 @@ lce_product_kernel(const __grid_constant__ GemmParams p) {
 // ------------------------------------------------------------ joining the sums
 struct JoinArgs {
   const float *picked, *inv;
-  float *rest, *miss;
+  float *top, *rest, *miss;
   int* count;
   int reduction, parts;
   float* loss;  // null, of lce_few_kernel: a launch of its own joins
@@ -679,7 +688,8 @@ __device__ __forceinline__ double finish_row(const JoinArgs& j, int64_t at, cons
   if (label[at] < 0 || z == INFINITY) loss_of = NAN;
   else if (z >= top) loss_of = log1p(rest * exp(top - z));
   else loss_of = top - z + log(rest + exp(z - top));
-  j.rest[at] = m == -INFINITY ? 0.f : (float)(top + log(rest));  // exp(-inf - rest) is 0, too, where all others are
+  j.top[at] = finite_shift(m);  // all others -inf: exp(-inf - 0) is 0
+  j.rest[at] = m == -INFINITY ? 0.f : (float)log2(rest);
   j.miss[at] = (float)-expm1(-loss_of);
   if (j.reduction == kLceNone) j.loss[index[at]] = (float)loss_of;
   return loss_of;
@@ -725,7 +735,7 @@ lce_few_kernel(const __grid_constant__ GemmParams p, float* acc, const JoinArgs 
   __shared__ int gave_up;
   __shared__ volatile int stop;  // of the epilogue warps
   __shared__ int label_of[N];
-  __shared__ float rest_of[N], scale_of[N];
+  __shared__ float top_of[N], rest_of[N], scale_of[N];
   __shared__ int row_of[N];
   __shared__ float2 warp_part[4][N];
   __shared__ double row_loss[PASS == kStats ? N : 1];
@@ -753,7 +763,10 @@ lce_few_kernel(const __grid_constant__ GemmParams p, float* acc, const JoinArgs 
   if (PASS != kGrads && threadIdx.x < N) {
     const int r = threadIdx.x;
     label_of[r] = r < n_rows ? p.label[r] : -1;
-    if (PASS == kLogitGrad) rest_of[r] = r < n_rows ? p.rest[r] : INFINITY;
+    if (PASS == kLogitGrad) {
+      top_of[r] = r < n_rows ? p.top[r] : 0.f;
+      rest_of[r] = r < n_rows ? p.rest[r] : INFINITY;
+    }
   }
   if (PASS == kGrads && p.gh != nullptr && threadIdx.x < n_rows) {
     const int r = threadIdx.x;
@@ -901,7 +914,7 @@ lce_few_kernel(const __grid_constant__ GemmParams p, float* acc, const JoinArgs 
         if (at < p.words) {
 #pragma unroll
           for (int r = 0; r < N; ++r) {
-            float d = label_of[r] == word ? -1.f : exp_of(__fsub_rn(v[r], rest_of[r]));
+            float d = label_of[r] == word ? -1.f : share_of(v[r], top_of[r], rest_of[r]);
             if (r >= n_rows) d = 0.f;  // the rows that pad the inner dimension of dW
             p.d[(int64_t)r * p.pitch + at] = (uint16_t)f32_to_bf16_rne_bits(d);
           }
@@ -1500,7 +1513,7 @@ cudaError_t launch_lce_forward(const LceArgs& a, int reduction, float* part, flo
   p.part = reinterpret_cast<float2*>(part);
   const bool few = a.rows <= kLceFewRows;
   p.index = a.index;
-  JoinArgs j{picked, a.inv, a.rest, a.miss, a.count, reduction, (int)(few ? (a.vocab + 127) / 128 : 2 * tiles_of(a.vocab)), loss};
+  JoinArgs j{picked, a.inv, a.top, a.rest, a.miss, a.count, reduction, (int)(few ? (a.vocab + 127) / 128 : 2 * tiles_of(a.vocab)), loss};
   if (few) {
     if (!encode(&p.a, a.w, a.hidden, a.vocab, a.w_stride, 128) ||
         !encode(&p.b, a.packed, a.hidden, p.padded, p.row_pitch, few_columns(a.rows)))
@@ -1557,6 +1570,7 @@ cudaError_t launch_lce_backward(const LceArgs& a, const LceGrad& g, cudaStream_t
   const int64_t pieces = lce_pieces(a.vocab, g.piece), pitch = lce_piece_pitch(a.vocab, g.piece);
   GemmParams p{};
   common_params(p, a);
+  p.top = a.top;
   p.rest = a.rest;
   p.miss = a.miss;
   p.row_g = g.reduction == kLceNone ? g.g : nullptr;

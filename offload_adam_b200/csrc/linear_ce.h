@@ -25,7 +25,8 @@ struct LceArgs {
   int* label = nullptr;              // (rows,) label of the packed row, -1: outside the vocabulary
   int* count = nullptr;              // [0] packed rows, [1] ticket
   float* inv = nullptr;              // 1 / max(1, packed rows)
-  float* rest = nullptr;             // (rows,) log-sum-exp of the packed row without its label
+  float* top = nullptr;              // (rows,) largest logit of the packed row without its label, 0 where that is -inf
+  float* rest = nullptr;             // (rows,) log2 of the sum of exp(logit - top) over the same words
   float* miss = nullptr;             // (rows,) 1 - probability of its label
   void* packed = nullptr;            // bf16 (rows padded, lce_row_pitch)
   int64_t* report = nullptr;         // host memory: [0] a label past the vocabulary, [1] a wait that gave up, [2] a negative label

@@ -28,10 +28,10 @@ Tensor rows_layout(const Tensor& t) {
 int64_t row_stride(const Tensor& t) { return t.size(0) == 1 ? t.size(1) : t.stride(0); }
 
 // What backward needs of forward, in one tensor of bytes: the packed rows of h (backward needs them in
-// any case, so keeping them instead of h leaves its peak), then index, label, rest and miss of each,
+// any case, so keeping them instead of h leaves its peak), then index, label, top, rest and miss of each,
 // their number with the ticket, 1 / number.
 int64_t packed_bytes(int64_t rows, int64_t hidden) { return 2 * oab::lce_padded(rows) * oab::lce_row_pitch(hidden); }
-int64_t kept_bytes(int64_t rows, int64_t hidden) { return packed_bytes(rows, hidden) + 4 * (4 * rows + 4); }
+int64_t kept_bytes(int64_t rows, int64_t hidden) { return packed_bytes(rows, hidden) + 4 * (5 * rows + 4); }
 oab::LceArgs make_args(const Tensor& w, const Tensor& labels, void* kept, int64_t ignore) {
   oab::LceArgs a;
   a.w = w.data_ptr();
@@ -45,10 +45,11 @@ oab::LceArgs make_args(const Tensor& w, const Tensor& labels, void* kept, int64_
   int* k = reinterpret_cast<int*>(static_cast<char*>(kept) + packed_bytes(a.rows, a.hidden));
   a.index = k;
   a.label = k + a.rows;
-  a.rest = reinterpret_cast<float*>(k + 2 * a.rows);
-  a.miss = reinterpret_cast<float*>(k + 3 * a.rows);
-  a.count = k + 4 * a.rows;
-  a.inv = reinterpret_cast<float*>(k + 4 * a.rows + 2);
+  a.top = reinterpret_cast<float*>(k + 2 * a.rows);
+  a.rest = reinterpret_cast<float*>(k + 3 * a.rows);
+  a.miss = reinterpret_cast<float*>(k + 4 * a.rows);
+  a.count = k + 5 * a.rows;
+  a.inv = reinterpret_cast<float*>(k + 5 * a.rows + 2);
   a.report = oab::loss_report();
   return a;
 }

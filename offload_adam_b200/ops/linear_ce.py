@@ -45,11 +45,12 @@ class _PlainLinearCE(torch.autograd.Function):
             here = (lab >= s) & (lab < s + w.shape[0])
             at = (lab - s).clamp(0, w.shape[0] - 1)
             picked = torch.where(here, z.gather(1, at[:, None])[:, 0], picked)
-        lse = top + total.log()
-        ctx.save_for_backward(h, weight, labels, lse)
+        # two numbers: their sum would lose the logarithm beside large logits
+        rest = total.log()
+        ctx.save_for_backward(h, weight, labels, top, rest)
         ctx.args = reduction, ignore_index, piece
         losses = torch.zeros(labels.shape, dtype=wide, device=h.device)
-        losses[rows] = lse - picked
+        losses[rows] = (top - picked) + rest
         if reduction == "none":
             return losses
         return losses.sum() / (max(1, len(rows)) if reduction == "mean" else 1)
@@ -62,17 +63,17 @@ class _PlainLinearCE(torch.autograd.Function):
 
     @staticmethod
     def _backward(ctx, g):
-        h, weight, labels, lse = ctx.saved_tensors
+        h, weight, labels, top, rest = ctx.saved_tensors
         reduction, ignore_index, piece = ctx.args
         rows = (labels != ignore_index).nonzero(as_tuple=True)[0]
-        lab, x = labels[rows], h[rows].to(lse.dtype)
+        lab, x = labels[rows], h[rows].to(top.dtype)
         scale = g[rows] if reduction == "none" else g / (max(1, len(rows)) if reduction == "mean" else 1)
-        scale = scale.to(lse.dtype).expand(len(rows))[:, None]
+        scale = scale.to(top.dtype).expand(len(rows))[:, None]
         gx = torch.zeros_like(x) if ctx.needs_input_grad[0] else None
         gw = torch.empty_like(weight) if ctx.needs_input_grad[1] else None
         for s in range(0, weight.shape[0], piece):
-            w = weight[s:s + piece].to(lse.dtype)
-            d = (x @ w.T - lse[:, None]).exp()
+            w = weight[s:s + piece].to(top.dtype)
+            d = (x @ w.T - top[:, None] - rest[:, None]).exp()
             here = ((lab >= s) & (lab < s + w.shape[0])).nonzero(as_tuple=True)[0]
             d[here, lab[here] - s] -= 1
             d *= scale

@@ -44,3 +44,50 @@ def test_a_word_of_minus_infinity(n, device):
     # d, the rows of h times 1 - p and the result round to bf16 (2^-8 each)
     off = (3 * 2.0 ** -8 + 2.0 ** -13) * (d.abs().T @ h[rows].double().abs())
     assert ((gw.double() - want).abs() <= off).all()
+
+
+def _far(n, vocab, device, shift):
+    """Logits that differ by at most 8, all of them `shift` away from 0, both exact in bf16 products:
+    the hidden state's first value is 1 and carries the shift."""
+    gen = torch.Generator().manual_seed(n + vocab)
+    h = torch.zeros(n, 64)
+    h[:, 0] = 1.0
+    h[:, 1:9] = torch.randint(0, 2, (n, 8), generator=gen).float()
+    w = torch.zeros(vocab, 64)
+    w[:, 0] = shift
+    if abs(shift) < 1e30:  # beside the lowest value there is no room for any difference
+        w[:, 1:9] = torch.randint(0, 2, (vocab, 8), generator=gen).float()
+    labels = torch.randint(0, vocab, (n,), generator=gen)
+    labels[2::5] = -100
+    return h.to(BF16).to(device), w.to(BF16).to(device), labels.to(device)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("shift", [0.0, -2.0 ** 20, 2.0 ** 20, torch.finfo(BF16).min, torch.finfo(BF16).max])
+@pytest.mark.parametrize("n,vocab", [(5, 600), (20, 601), (100, 600), (300, 1025)])
+def test_logits_far_from_zero(n, vocab, shift, device):
+    """Only the differences of a row's logits matter, also where their logarithm's sum is lost beside
+    the logits, as for a row whose words are all masked with the type's lowest value."""
+    h, w, labels = _far(n, vocab, device, shift)
+    h.requires_grad_(True)
+    w.requires_grad_(True)
+    loss = linear_cross_entropy(h, w, labels, reduction="none")
+    gh, gw = torch.autograd.grad(loss.sum(), (h, w))
+    rows = (labels != -100).nonzero(as_tuple=True)[0]
+    x, y = h.detach().double()[rows], w.detach().double()
+    z = x[:, 1:] @ y[:, 1:].T  # without the shift, the same in every logit
+    logp = torch.log_softmax(z, 1)
+    at = torch.arange(len(rows), device=device)
+    exact = -logp[at, labels[rows]]
+    # every logit is exact; the losses are those of sums of exponentials, (|x| + 4) 2^-24 off each and
+    # 2^-24 with each of fewer than 1025 additions at most
+    assert ((loss[rows].double() - exact).abs() <= 2.0 ** -13 * (1 + exact)).all()
+    assert (loss[labels == -100] == 0).all() and (gh[labels == -100] == 0).all()
+    d = logp.exp()
+    d[at, labels[rows]] -= 1
+    want_h, want_w = d @ y, d.T @ x
+    # d, the rows of h times 1 - p and the results round to bf16, 2^-8 each; sums of up to 1025
+    # products in fp32 add 2^-13
+    assert ((gw.double() - want_w).abs() <= (3 * 2.0 ** -8 + 2.0 ** -12) * (d.abs().T @ x.abs()) + 1e-30).all()
+    off = (2 * 2.0 ** -8 + 2.0 ** -12) * (d.abs() @ y.abs())
+    assert ((gh[rows].double() - want_h).abs() <= off + 1e-30).all()
