@@ -18,7 +18,10 @@
 // lowest value, and each word of such a row would have the whole of it.
 // tcgen05 cuts off what it adds to an accumulator, towards zero each time: logits of 4096 terms came
 // out 1e-5 too small, the losses of unsure rows 2.5e-5 off.  So the statistics take their logits in
-// chains of 32 additions (512 terms; 256 for few rows) that the epilogue adds up.
+// chains of 32 additions (512 terms; 256 for few rows) that the epilogue adds up.  Sums of terms of one
+// sign lose about 1e-7 of their value with each addition of 16 terms (dW of ones over 2^20 rows: 0.7 %,
+// over 2^22: 2.3 %), so an accumulator takes kLceSumTerms of them at most, 4e-4, and dW of more rows is
+// summed in fp32 in memory, a launch for every kLceSumTerms rows.
 //
 // Forward: one product whose epilogue keeps, per row and 128 words, the maximum and the sum of
 // exponentials (8 bytes for 256 bytes of bf16 logits), and a small kernel that joins them (of a few
@@ -66,7 +69,7 @@ enum Pass { kStats = 0, kLogitGrad = 1, kGrads = 2 };
 struct GemmParams {
   CUtensorMap a, b;    // kStats, kLogitGrad: packed rows and W.  kGrads: d and W, for dh
   CUtensorMap a2, b2;  // kGrads: d and packed rows, for dW
-  CUtensorMap out;     // kLogitGrad: d.  kGrads: dW
+  CUtensorMap out;     // kLogitGrad: d.  kGrads: dW, or with wacc its fp32 sums
   CUtensorMap out_acc; // kGrads: the fp32 sums of dh, by split
   const int* count;
   int64_t rows;        // capacity of the per-row arrays
@@ -94,6 +97,8 @@ struct GemmParams {
   const float *inv, *g;  // each may be null (1)
   int want_dh, want_dw;
   uint16_t* gw;               // few rows; otherwise by `out`
+  int row0;                   // first packed row of the sums of dW
+  int wacc;                   // dW goes to fp32 sums; those of row0 = 0 start them
   int splits;
   int first;             // piece: its dh starts the sums
 };
@@ -137,7 +142,8 @@ struct Plan {
       dh_tiles = p.want_dh ? per_split * p.splits : 0;
       total = dh_tiles + wt * ht;
       k_steps = (p.words + kInner - 1) / kInner;
-      row_steps = (n_rows + kInner - 1) / kInner;
+      const int left = n_rows - p.row0, own = left < 0 ? 0 : left < kLceSumTerms ? left : kLceSumTerms;
+      row_steps = (own + kInner - 1) / kInner;
       // The tiles of dh are long (a sum over the words) and come first, those of dW (a sum over the
       // rows) fill up.  Pairs that a last, partial round of dh leaves idle take as many tiles
       // of dW as such a tile is long before the others join in.  4096 rows, hidden 4096, 32768
@@ -196,6 +202,7 @@ struct Plan {
         x.steps = hi - lo;
       } else {
         x.kind = 1;
+        x.k0 = p.row0;
         place(t - dh_tiles, wt, ht, m, n);
         x.steps = row_steps;
       }
@@ -360,6 +367,21 @@ __device__ __forceinline__ float row_scale(const GemmParams& p, int k, float sca
   return p.row_g != nullptr ? __fmul_rn(scale, p.row_g[p.index[k]]) : scale;
 }
 
+// 16 columns as fp32 on their way to sums in memory.
+__device__ __forceinline__ void stage_sums(uint32_t staging, int lane, const Tile& x, float (&v)[16]) {
+  if (x.steps == 0) {  // nothing was summed
+#pragma unroll
+    for (int i = 0; i < 16; ++i) v[i] = 0.f;
+  }
+  stage_begin(lane);
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    stage_part(staging, lane, i, __float_as_uint(v[4 * i]), __float_as_uint(v[4 * i + 1]), __float_as_uint(v[4 * i + 2]),
+               __float_as_uint(v[4 * i + 3]));
+  store_fence();
+  __syncwarp();
+}
+
 template <class Release>
 __device__ __forceinline__ void dh_tile(const GemmParams& p, const Tile& x, uint32_t tmem, int row, int n_rows, int half, float scale,
                                         uint32_t staging, int lane, const Release& release) {
@@ -379,17 +401,7 @@ __device__ __forceinline__ void dh_tile(const GemmParams& p, const Tile& x, uint
       if (out != nullptr && col + 8 < p.hidden) store_bf16x8(out + col + 8, v + 8, scale);
       continue;
     }
-    if (x.steps == 0) {  // a last piece of fewer stages than splits: nothing was summed
-#pragma unroll
-      for (int i = 0; i < 16; ++i) v[i] = 0.f;
-    }
-    stage_begin(lane);
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      stage_part(staging, lane, i, __float_as_uint(v[4 * i]), __float_as_uint(v[4 * i + 1]), __float_as_uint(v[4 * i + 2]),
-                 __float_as_uint(v[4 * i + 3]));
-    store_fence();
-    __syncwarp();
+    stage_sums(staging, lane, x, v);  // no stage: a last piece of fewer stages than splits
     if (lane == 0) {
       if (col < p.hidden && row < n_rows) tma_store3(&p.out_acc, staging, col, row, x.split, !p.first);
       store_commit();
@@ -400,6 +412,21 @@ __device__ __forceinline__ void dh_tile(const GemmParams& p, const Tile& x, uint
 template <class Release>
 __device__ __forceinline__ void dw_tile(const GemmParams& p, const Tile& x, uint32_t tmem, int row, int half, float scale,
                                         uint32_t staging, int lane, const Release& release) {
+  if (p.wacc) {
+#pragma unroll 1
+    for (int c = 0; c < 8; ++c) {
+      float v[16];
+      tmem_load16(tmem + c * 16, v);
+      if (c == 7) release();
+      const int col = x.n + half * 128 + c * 16;
+      stage_sums(staging, lane, x, v);
+      if (lane == 0) {
+        if (col < p.hidden && row < p.words) tma_store3(&p.out, staging, col, row, 0, p.row0 != 0);
+        store_commit();
+      }
+    }
+    return;
+  }
 #pragma unroll 1
   for (int c = 0; c < 4; ++c) {
     float v[32];
@@ -1347,6 +1374,23 @@ lce_join_grad_kernel(const float* __restrict__ acc, int splits, int64_t padded, 
   store_bf16x8(gh + (int64_t)index[k] * hidden + col, v, scale);
 }
 
+// ------------------------------------------------------- dW of many rows, rounded
+// One piece, from its fp32 sums.
+__global__ void __launch_bounds__(128)
+lce_round_head_kernel(const float* __restrict__ acc, int64_t pitch, int hidden, const float* inv, const float* g, uint16_t* gw) {
+  const int64_t word = blockIdx.x;
+  const int col = (blockIdx.y * 128 + threadIdx.x) * 8;
+  grid_wait();
+  if (col >= hidden) return;
+  float scale = inv != nullptr ? *inv : 1.f;
+  if (g != nullptr) scale = __fmul_rn(scale, *g);
+  const V8 x = ld32(acc + word * pitch + col);
+  float v[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v[i] = __uint_as_float(x.w[i]);
+  store_bf16x8(gw + word * hidden + col, v, scale);
+}
+
 // ------------------------------------------------------------------- launching
 PFN_cuTensorMapEncodeTiled_v12000 encoder() {
   static const PFN_cuTensorMapEncodeTiled_v12000 fn = [] {
@@ -1368,12 +1412,13 @@ cudaError_t make_context_current() {
   return e != cudaSuccess ? e : cudaSetDevice(device);
 }
 
-// The fp32 sums of dh as (hidden, rows, splits) in boxes of 16 columns and 32 rows.
-bool encode_acc(CUtensorMap* map, float* base, int64_t hidden, int64_t pitch, int64_t padded, int splits) {
+// The fp32 sums of dh as (hidden, rows, splits), of dW as (hidden, words, 1), in boxes of 16 columns and
+// 32 lines.
+bool encode_acc(CUtensorMap* map, float* base, int64_t hidden, int64_t pitch, int64_t lines, int splits) {
   const auto fn = encoder();
   if (fn == nullptr) return false;
-  const cuuint64_t dims[3] = {(cuuint64_t)hidden, (cuuint64_t)padded, (cuuint64_t)splits};
-  const cuuint64_t strides[2] = {(cuuint64_t)pitch * 4, (cuuint64_t)pitch * 4 * (cuuint64_t)padded};
+  const cuuint64_t dims[3] = {(cuuint64_t)hidden, (cuuint64_t)lines, (cuuint64_t)splits};
+  const cuuint64_t strides[2] = {(cuuint64_t)pitch * 4, (cuuint64_t)pitch * 4 * (cuuint64_t)lines};
   const cuuint32_t box[3] = {16, 32, 1}, steps[3] = {1, 1, 1};
   return fn(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 3, base, dims, strides, box, steps, CU_TENSOR_MAP_INTERLEAVE_NONE,
             CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
@@ -1564,7 +1609,8 @@ int lce_splits(int64_t rows, int64_t hidden, int64_t vocab, int64_t piece) {
 cudaError_t launch_lce_backward(const LceArgs& a, const LceGrad& g, cudaStream_t st) {
   if (!args_ok(a) || g.piece <= 0 || g.piece % kTile != 0 || g.splits < 1 || g.g == nullptr) return cudaErrorInvalidValue;
   if (g.gh == nullptr && g.gw == nullptr) return cudaSuccess;
-  if (g.d == nullptr || (g.gh != nullptr && g.acc == nullptr && !lce_direct(a.vocab, g.piece, g.splits)) || (g.gw != nullptr && g.scaled == nullptr)) return cudaErrorInvalidValue;
+  if (g.d == nullptr || (g.gh != nullptr && g.acc == nullptr && !lce_direct(a.vocab, g.piece, g.splits)) || (g.gw != nullptr && g.scaled == nullptr) ||
+      (g.gw != nullptr && g.wacc == nullptr && lce_row_groups(a.rows) > 1)) return cudaErrorInvalidValue;
   cudaError_t e = make_context_current();
   if (e != cudaSuccess) return e;
   const int64_t pieces = lce_pieces(a.vocab, g.piece), pitch = lce_piece_pitch(a.vocab, g.piece);
@@ -1591,6 +1637,8 @@ cudaError_t launch_lce_backward(const LceArgs& a, const LceGrad& g, cudaStream_t
   q.want_dh = g.gh != nullptr;
   q.want_dw = g.gw != nullptr;
   q.gw = (uint16_t*)g.gw;
+  const int groups = q.want_dw ? (int)lce_row_groups(a.rows) : 1;
+  q.wacc = groups > 1;
   q.splits = g.splits;
   // few rows: `few` has the operands of dh, q those of dW alone
   const bool is_few = a.rows <= kLceFewRows;
@@ -1602,7 +1650,7 @@ cudaError_t launch_lce_backward(const LceArgs& a, const LceGrad& g, cudaStream_t
   if (!encode(is_few ? &p.b : &p.a, a.packed, a.hidden, p.padded, p.row_pitch, is_few ? columns : 128) ||
       !encode(is_few ? &p.a : &p.b, a.w, a.hidden, a.vocab, a.w_stride, 128) ||
       !encode(is_few ? &few.a : &q.b, a.w, a.hidden, a.vocab, a.w_stride, 64) || (q.want_dw && !encode(&q.b2, g.scaled, a.hidden, p.padded, p.row_pitch, 64)) ||
-      (q.want_dw && !is_few && !encode(&q.out, g.gw, a.hidden, a.vocab, a.hidden, 32, 32)) ||
+      (q.want_dw && !is_few && !q.wacc && !encode(&q.out, g.gw, a.hidden, a.vocab, a.hidden, 32, 32)) ||
       (q.want_dh && !direct && !encode_acc(&q.out_acc, g.acc, a.hidden, p.row_pitch, p.padded, g.splits)))
     return cudaErrorInvalidValue;
   for (int64_t i = 0; i < pieces; ++i) {
@@ -1627,9 +1675,20 @@ cudaError_t launch_lce_backward(const LceArgs& a, const LceGrad& g, cudaStream_t
       if (q.want_dw && (e = launch_few_dw(q, (q.words + 127) / 128 * tiles_of(a.hidden), st)) != cudaSuccess) return e;
       continue;
     }
-    const int64_t dh = q.want_dh ? tiles_of(a.rows) * tiles_of(a.hidden) * g.splits : 0;
+    const int64_t dh = g.gh != nullptr ? tiles_of(a.rows) * tiles_of(a.hidden) * g.splits : 0;
     const int64_t dw = q.want_dw ? tiles_of(q.words) * tiles_of(a.hidden) : 0;
-    if ((e = launch_product<kGrads>(q, dh + dw, st)) != cudaSuccess) return e;
+    if (q.wacc && !encode_acc(&q.out, g.wacc, a.hidden, p.row_pitch, q.words, 1)) return cudaErrorInvalidValue;
+    for (int k = 0; k < groups; ++k) {  // the first one takes dh, too
+      q.row0 = k * kLceSumTerms;
+      q.want_dh = k == 0 && g.gh != nullptr;
+      if ((e = launch_product<kGrads>(q, (k == 0 ? dh : 0) + dw, st)) != cudaSuccess) return e;
+    }
+    if (q.wacc) {
+      count_launch();
+      e = launch_behind(lce_round_head_kernel, dim3((unsigned)q.words, (unsigned)((a.hidden + 1023) / 1024)), 128, 0, st, g.wacc, p.row_pitch,
+                        (int)a.hidden, q.inv, q.g, (uint16_t*)g.gw + q.word0 * a.hidden);
+      if (e != cudaSuccess) return e;
+    }
   }
   if (g.gh != nullptr && !direct) {
     count_launch();

@@ -8,6 +8,7 @@ namespace oab {
 constexpr int kLceTile = 256;     // rows and columns of an output tile; a piece of the vocabulary is a multiple
 constexpr int kLceFewRows = 64;   // up to here the rows are the narrow side of the products
 constexpr int kLceRowPad = 64;    // the packed rows are padded with zeros to a multiple of this
+constexpr int kLceSumTerms = 65536;  // that an accumulator of the tensor cores sums
 // Sizes that the kernels take.
 constexpr int64_t kLceMaxRows = int64_t(1) << 24, kLceMaxHidden = int64_t(1) << 18, kLceMaxVocab = int64_t(1) << 26;
 
@@ -58,7 +59,10 @@ struct LceGrad {
   void* scaled = nullptr;     // bf16 (padded rows, lce_row_pitch), for gw
   int splits = 1;             // of the sum over the words in gh
   float* acc = nullptr;       // fp32 (splits, padded rows, lce_row_pitch), for gh unless lce_direct
+  float* wacc = nullptr;      // fp32 (words of a piece, lce_row_pitch), for gw of several row groups
 };
+// Launches whose sums make up one gw.
+inline int64_t lce_row_groups(int64_t rows) { return (rows + kLceSumTerms - 1) / kLceSumTerms; }
 inline int64_t lce_pieces(int64_t vocab, int64_t piece) { return (vocab + piece - 1) / piece; }
 inline int64_t lce_piece_pitch(int64_t vocab, int64_t piece) { return ((vocab < piece ? vocab : piece) + 63) / 64 * 64; }
 // gh goes straight out: its sums are whole after one launch.

@@ -131,6 +131,7 @@ struct LinearCE : torch::autograd::Function<LinearCE> {
     const int64_t d = t.add(2 * oab::lce_padded(rows) * oab::lce_piece_pitch(vocab, piece));
     const int64_t acc = t.add(want_h && !oab::lce_direct(vocab, piece, x.splits) ? 4 * x.splits * oab::lce_padded(rows) * oab::lce_row_pitch(hidden) : 0);
     const int64_t scaled = t.add(want_w ? packed_bytes(rows, hidden) : 0);
+    const int64_t wacc = t.add(want_w && oab::lce_row_groups(rows) > 1 ? 4 * std::min(piece, vocab) * oab::lce_row_pitch(hidden) : 0);
     t.take(w);
     x.d = t.at_byte<void>(d);
     if (want_h) {
@@ -142,6 +143,7 @@ struct LinearCE : torch::autograd::Function<LinearCE> {
       gw = at::empty({vocab, hidden}, w.options());
       x.gw = gw.data_ptr();
       x.scaled = t.at_byte<void>(scaled);
+      x.wacc = t.at_byte<float>(wacc);
     }
     ok(oab::launch_lce_backward(make_args(wc, lc, kept.data_ptr(), ignore), x, cur()), "linear_cross_entropy backward");
     if (graph) {

@@ -108,7 +108,8 @@ def linear_cross_entropy(h, weight, labels, reduction="mean", ignore_index=-100,
     2^26 words) run the kernels (``csrc/linear_ce.cu``); everything else runs operations of PyTorch
     piece by piece.  Beside the gradients the kernels take a copy of the rows that count, until
     backward, ``rows * vocab / 16`` bytes in forward, and in backward one piece, a second copy of
-    the rows and the fp32 sums of the hidden states' gradient.
+    the rows and the fp32 sums of the hidden states' gradient (beyond 65536 rows also of one piece of the
+    head's).
 
     A label outside the vocabulary is an ``IndexError``.  The kernels see it when they run: the
     loss of that call is NaN, and the next call that looks (its backward, or the next loss)

@@ -91,3 +91,62 @@ def test_logits_far_from_zero(n, vocab, shift, device):
     assert ((gw.double() - want_w).abs() <= (3 * 2.0 ** -8 + 2.0 ** -12) * (d.abs().T @ x.abs()) + 1e-30).all()
     off = (2 * 2.0 ** -8 + 2.0 ** -12) * (d.abs() @ y.abs())
     assert ((gh[rows].double() - want_h).abs() <= off + 1e-30).all()
+
+
+def _even(n, vocab, device, seed=0):
+    """Words that are all as likely but word 0, the label of every row, which is next to impossible: the
+    gradient of the logits is 1 / (vocab - 1), exact for a power of two, and -1 at the label."""
+    gen = torch.Generator(device=device).manual_seed(seed)
+    h = torch.randint(64, 193, (n, 64), generator=gen, device=device).float() / 128
+    h[:, 0] = 1.0
+    w = torch.zeros(vocab, 64, device=device)
+    w[0, 0] = -128.0
+    return h.to(BF16), w.to(BF16), torch.zeros(n, dtype=torch.int64, device=device)
+
+
+@gpu
+@pytest.mark.parametrize("reduction", ["sum", "none"])
+@pytest.mark.parametrize("n", [65535, 65536, 65537, 131073, 200000, (1 << 20) + 37])
+def test_head_gradient_over_many_rows(n, reduction):
+    h, w, labels = _even(n, 65, "cuda", seed=n)
+    labels[5::7] = -100
+    w.requires_grad_(True)
+    g = torch.randint(0, 2, (n,), device="cuda").float() + 1 if reduction == "none" else torch.full((), 0.5, device="cuda")
+    gw, = torch.autograd.grad(linear_cross_entropy(h, w, labels, reduction=reduction), w, g)
+    rows = labels != -100
+    total = (h[rows].double() * (g[rows][:, None].double() if reduction == "none" else g.double())).sum(0)
+    want = torch.cat([-total[None], total.expand(64, 64) / 64])
+    # d and the rows that count are exact in bf16; each of 4096 additions is off by 2^-23 of the sum at
+    # most, and sums of 65536 rows add up in fp32; the result rounds to bf16
+    assert ((gw.double() - want).abs() <= (2.0 ** -8 + 2.0 ** -11) * want.abs()).all()
+
+
+@gpu
+def test_gradients_of_more_rows_than_an_accumulator_sums():
+    """Random rows in two groups, in pieces, with the gradient of the hidden states: against 64 bits, and
+    the same bits again."""
+    n, hidden, vocab = 70000, 72, 700
+    gen = torch.Generator(device="cuda").manual_seed(1)
+    h = torch.randn(n, hidden, device="cuda", generator=gen).to(BF16).requires_grad_(True)
+    w = (torch.randn(vocab, hidden, device="cuda", generator=gen) / math.sqrt(hidden)).to(BF16).requires_grad_(True)
+    for count in (n, 65536, 66000, 300, 0):  # rows that count: the second group has many, few or none
+        labels = torch.randint(0, vocab, (n,), device="cuda", generator=gen)
+        labels[torch.randperm(n, device="cuda", generator=gen)[count:]] = -100
+        rows = labels != -100
+        x, y = h.detach().double()[rows], w.detach().double()
+        z = x @ y.T
+        d = z.softmax(1)
+        d[torch.arange(len(x), device="cuda"), labels[rows]] -= 1
+        want_h, want_w = d @ y / max(1, count), d.T @ x / max(1, count)
+        tol_w = d.abs().T @ x.abs() / max(1, count) * (3 * 2.0 ** -8 + 2.0 ** -11)
+        tol_h = d.abs() @ y.abs() / max(1, count) * (2 * 2.0 ** -8 + 2.0 ** -11)
+        first = None
+        for piece in (None, 256):
+            gh, gw = torch.autograd.grad(linear_cross_entropy(h, w, labels, piece=piece), (h, w))
+            assert ((gw.double() - want_w).abs() <= tol_w).all()
+            assert ((gh[rows].double() - want_h).abs() <= tol_h).all()
+            assert (gh[~rows] == 0).all()
+            again = torch.autograd.grad(linear_cross_entropy(h, w, labels, piece=piece), (h, w))
+            assert torch.equal(gh, again[0]) and torch.equal(gw, again[1])
+            first = gw if first is None else first
+            assert torch.equal(gw, first)  # pieces change nothing of the head's gradient
