@@ -20,8 +20,9 @@
 // out 1e-5 too small, the losses of unsure rows 2.5e-5 off.  So the statistics take their logits in
 // chains of 32 additions (512 terms; 256 for few rows) that the epilogue adds up.  Sums of terms of one
 // sign lose about 1e-7 of their value with each addition of 16 terms (dW of ones over 2^20 rows: 0.7 %,
-// over 2^22: 2.3 %), so an accumulator takes kLceSumTerms of them at most, 4e-4, and dW of more rows is
-// summed in fp32 in memory, a launch for every kLceSumTerms rows.
+// over 2^22: 2.3 %), so an accumulator takes kLceSumTerms of them at most, 4e-4: dW of more rows is
+// summed in fp32 in memory, a launch for every kLceSumTerms rows, and dh of more words in splits (in
+// chains for few rows).
 //
 // Forward: one product whose epilogue keeps, per row and 128 words, the maximum and the sum of
 // exponentials (8 bytes for 256 bytes of bf16 logits), and a small kernel that joins them (of a few
@@ -742,6 +743,8 @@ struct FewShape {
 // Stages of a chain of the statistics.  One row of 128256 words x 4096: 174 us without chains, 179 with
 // four stages, 186 with two; the loss of a confident row up to 25, 1.0 and 0.8e-6 off 64 bits.
 constexpr int kFewChain = 4;
+// Of the gradients; only dh has as many.
+constexpr int kFewSumChain = kLceSumTerms / kInner;
 template <int N>
 __device__ __forceinline__ void tmem_load_rows(uint32_t at, float (&v)[N]) {
   if constexpr (N == 16) {
@@ -756,6 +759,7 @@ template <int PASS, int N>
 __global__ void __launch_bounds__(kFewThreads, 1)
 lce_few_kernel(const __grid_constant__ GemmParams p, float* acc, const JoinArgs j) {
   using S = FewShape<N>;
+  constexpr int kLength = PASS == kStats ? kFewChain : kFewSumChain;  // stages of a chain
   extern __shared__ uint8_t smem_raw[];
   __shared__ uint64_t full[S::kCount], empty[S::kCount], done[S::kAccs], drained[S::kAccs];
   __shared__ uint32_t tmem_at;
@@ -853,7 +857,7 @@ lce_few_kernel(const __grid_constant__ GemmParams p, float* acc, const JoinArgs 
         const int steps = share(t, first);
         int k = 0;
         do {  // one chain; a tile of no stage has an empty one
-          const int last = PASS == kStats && k + kFewChain < steps ? k + kFewChain : steps;
+          const int last = k + kLength < steps ? k + kLength : steps;
           const uint32_t buf = chains % S::kAccs, d = tmem + buf * N;
           if (!mbar_wait(drained0 + 8 * buf, ((chains / S::kAccs) & 1) ^ 1)) { ok = false; break; }
           fence_after();
@@ -884,7 +888,7 @@ lce_few_kernel(const __grid_constant__ GemmParams p, float* acc, const JoinArgs 
     if (PASS == kLogitGrad) prepare_rows(p, n_rows, blockIdx.x * 4 + warp - 2, gridDim.x * 4);
     for (int t = blockIdx.x; t < total; t += gridDim.x) {
       int first;
-      const int steps = share(t, first), m = t % across * 128, length = PASS == kStats ? kFewChain : steps;
+      const int steps = share(t, first), m = t % across * 128;
       float v[N];
       int k = 0;
       do {
@@ -905,7 +909,7 @@ lce_few_kernel(const __grid_constant__ GemmParams p, float* acc, const JoinArgs 
         __syncwarp();
         if (lane == 0) mbar_arrive(drained0 + 8 * buf);
         ++chains;
-        k += length;
+        k += kLength;
       } while (k < steps);
       if (PASS != kStats && !ok) break;
       const int at = m + quarter * 32 + lane;  // this lane's word of the piece, or hidden column
@@ -1581,11 +1585,12 @@ cudaError_t launch_lce_forward(const LceArgs& a, int reduction, float* part, flo
 int64_t lce_default_piece(int64_t rows, int64_t hidden, int64_t vocab) {
   const int64_t words = (int64_t(256) << 20) / (2 * lce_padded(rows)) / kTile * kTile;
   const int64_t all = tiles_of(vocab) * kTile;
-  return words < kTile ? kTile : words < all ? words : all;
+  const int64_t most = words < all ? words : all;
+  return most < kTile ? kTile : most < kLceMaxPiece ? most : kLceMaxPiece;
 }
 
 int lce_splits(int64_t rows, int64_t hidden, int64_t vocab, int64_t piece) {
-  const int64_t steps = (piece < vocab ? piece : vocab) / kInner;
+  const int64_t words = piece < vocab ? piece : vocab, steps = words / kInner;
   if (vocab <= piece && steps <= 32) return 1;  // up to 9 us; a launch to join the splits is longer
   if (rows <= kLceFewRows) {
     // the number that leaves the fewest SMs idle in the last round; each split is as much again
@@ -1603,11 +1608,12 @@ int lce_splits(int64_t rows, int64_t hidden, int64_t vocab, int64_t piece) {
   const int64_t tiles = tiles_of(rows) * tiles_of(hidden);
   int64_t s = kNumSMs / 2 / tiles;
   if (s > steps / 8) s = steps / 8;
-  return s < 1 ? 1 : (int)s;
+  const int64_t least = (words + kLceSumTerms - 1) / kLceSumTerms;  // 16 at most
+  return (int)(s < least ? least : s);
 }
 
 cudaError_t launch_lce_backward(const LceArgs& a, const LceGrad& g, cudaStream_t st) {
-  if (!args_ok(a) || g.piece <= 0 || g.piece % kTile != 0 || g.splits < 1 || g.g == nullptr) return cudaErrorInvalidValue;
+  if (!args_ok(a) || g.piece <= 0 || g.piece % kTile != 0 || g.piece > kLceMaxPiece || g.splits < 1 || g.g == nullptr) return cudaErrorInvalidValue;
   if (g.gh == nullptr && g.gw == nullptr) return cudaSuccess;
   if (g.d == nullptr || (g.gh != nullptr && g.acc == nullptr && !lce_direct(a.vocab, g.piece, g.splits)) || (g.gw != nullptr && g.scaled == nullptr) ||
       (g.gw != nullptr && g.wacc == nullptr && lce_row_groups(a.rows) > 1)) return cudaErrorInvalidValue;

@@ -11,6 +11,7 @@ constexpr int kLceRowPad = 64;    // the packed rows are padded with zeros to a 
 constexpr int kLceSumTerms = 65536;  // that an accumulator of the tensor cores sums
 // Sizes that the kernels take.
 constexpr int64_t kLceMaxRows = int64_t(1) << 24, kLceMaxHidden = int64_t(1) << 18, kLceMaxVocab = int64_t(1) << 26;
+constexpr int64_t kLceMaxPiece = int64_t(1) << 20;  // words at a time
 
 // Operands and workspaces of one loss.  `rows` are the rows of h; the kernels work on those whose
 // label counts, packed in order: how many there are is known on the device only.

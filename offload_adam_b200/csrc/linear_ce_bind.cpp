@@ -119,7 +119,7 @@ struct LinearCE : torch::autograd::Function<LinearCE> {
     const Tensor gc = g.to(at::kFloat).contiguous();
     const int64_t rows = labels.size(0), hidden = w.size(1), vocab = w.size(0);
     int64_t piece = ctx->saved_data["piece"].toInt();
-    piece = std::min(piece, vocab);
+    piece = std::min({piece, vocab, oab::kLceMaxPiece});
     piece = piece > 0 ? (piece + oab::kLceTile - 1) / oab::kLceTile * oab::kLceTile : oab::lce_default_piece(rows, hidden, vocab);
     oab::LceGrad x;
     x.reduction = (int)reduction;

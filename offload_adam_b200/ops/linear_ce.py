@@ -101,7 +101,8 @@ def linear_cross_entropy(h, weight, labels, reduction="mean", ignore_index=-100,
         ignore_index: rows with this label take no part: whatever ``h`` holds there, they
             contribute nothing and their gradient is zero.
         piece: words of the vocabulary whose gradient backward holds at a time; rounded up
-            to a multiple of 256 where the kernels run.  ``None`` or 0: as many as take 256 MB.
+            to a multiple of 256 where the kernels run, 2^20 at most there.  ``None`` or 0: as many as take
+            256 MB.
 
     The result is fp32 (fp64 for fp64 inputs) and differentiable once with respect to ``h`` and
     ``weight``.  Plain bf16 CUDA tensors whose ``hidden`` is a multiple of 8 (2^18 at most; 2^24 rows,

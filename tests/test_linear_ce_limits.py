@@ -150,3 +150,30 @@ def test_gradients_of_more_rows_than_an_accumulator_sums():
             assert torch.equal(gh, again[0]) and torch.equal(gw, again[1])
             first = gw if first is None else first
             assert torch.equal(gw, first)  # pieces change nothing of the head's gradient
+
+
+@gpu
+@pytest.mark.parametrize("n,hidden,vocab,piece", [
+    (4, 64, (1 << 20) + 1, None), (60, 4736, (1 << 18) + 1, None),  # few rows
+    (2432, 1024, (1 << 20) + 1, 1 << 20), (2432, 1024, (1 << 18) + 1, 1 << 62),  # more tiles than pairs of SMs
+    (300, 64, (1 << 21) + 1, 1 << 62)])  # more than one piece holds
+def test_gradient_of_hidden_states_over_many_words(n, hidden, vocab, piece):
+    """Every word but the label is as likely, so that a row's gradient is the mean of the words."""
+    gen = torch.Generator(device="cuda").manual_seed(vocab)
+    w = torch.randint(64, 193, (vocab, hidden), generator=gen, device="cuda", dtype=torch.int16).to(BF16).div_(128)
+    w[:, 0] = 0.0
+    w[0] = 0.0
+    w[0, 0] = -128.0
+    h = torch.zeros(n, hidden, device="cuda", dtype=BF16)
+    h[:, 0] = 1.0
+    h.requires_grad_(True)
+    labels = torch.zeros(n, dtype=torch.int64, device="cuda")
+    gh, = torch.autograd.grad(linear_cross_entropy(h, w, labels, reduction="sum", piece=piece), h)
+    total = torch.zeros(hidden, dtype=torch.float64, device="cuda")
+    for s in range(1, vocab, 1 << 16):
+        total += w[s:s + (1 << 16)].sum(0, dtype=torch.float64)
+    want = total / (vocab - 1)
+    want[0] = 128.0
+    # 1 / (vocab - 1) is exact in bf16; 4096 additions are off by 2^-23 of the sum each at most, and up to 32
+    # such sums add up in fp32; the result rounds to bf16
+    assert ((gh.double() - want).abs() <= (2.0 ** -8 + 2.0 ** -11) * want).all()
