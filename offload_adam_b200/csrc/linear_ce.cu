@@ -18,7 +18,9 @@
 // lowest value, and each word of such a row would have the whole of it.
 // tcgen05 cuts off what it adds to an accumulator, towards zero each time: logits of 4096 terms came
 // out 1e-5 too small, the losses of unsure rows 2.5e-5 off.  So the statistics take their logits in
-// chains of 32 additions (512 terms; 256 for few rows) that the epilogue adds up.  Sums of terms of one
+// chains of 32 additions (512 terms; 256 for few rows) that the epilogue adds up, and the logits that
+// backward forms again in chains of 8192 terms (a logit of 32 is 1e-3 off at most; of 2^18 terms in one
+// chain it was 0.05).  Sums of terms of one
 // sign lose about 1e-7 of their value with each addition of 16 terms (dW of ones over 2^20 rows: 0.7 %,
 // over 2^22: 2.3 %), so an accumulator takes kLceSumTerms of them at most, 4e-4: dW of more rows is
 // summed in fp32 in memory, a launch for every kLceSumTerms rows, and dh of more words in splits (in
@@ -62,7 +64,7 @@ constexpr int kEpilogueWarps = 16;       // eight for each accumulator
 constexpr int kStagingBytes = 32 * 64;   // of an epilogue warp: 32 lines of 64 bytes on their way out
 constexpr int smem_of(bool staging) { return kStages * kStageBytes + (staging ? kEpilogueWarps * kStagingBytes : 0) + 1024; }  // starts on 1024 bytes
 constexpr int kGemmThreads = 64 + 32 * kEpilogueWarps;
-constexpr int kChain = 8;   // stages of a chain of the statistics
+constexpr int kChain = 8, kGradChain = 128;  // stages of a chain of the statistics, of the logits for backward
 constexpr int kGroup = 16;  // row tiles that share a column tile in turn: 4096 rows of h stay in L2
 
 enum Pass { kStats = 0, kLogitGrad = 1, kGrads = 2 };
@@ -223,8 +225,8 @@ struct Plan {
 // tile, and every other tile of its pair.  A warp is a chain of latencies (the accumulator is
 // done, its load, a fence, the way out), so there are eight for each accumulator, and the accumulator
 // is given back (`release`) with the last load from it, before anything is computed from that.
-// Of the statistics likewise, unless the sums come in several chains: then all sixteen take 64 columns
-// of every tile.  (4096 rows of 128, 32000 words: 55 us by halves, 78 all together.)
+// Of the statistics likewise; and of both, unless the sums come in several chains: then all sixteen take
+// 64 columns of every tile.  (4096 rows of 128, 32000 words: 55 us by halves, 78 all together.)
 
 struct RowValues {  // of the packed row that a thread has in a tile
   int label;
@@ -315,36 +317,41 @@ __device__ __forceinline__ void prepare_rows(const GemmParams& p, int n_rows, in
   }
 }
 
+// 32 of a row's logits become their gradient, and go out.
+__device__ __forceinline__ void logit_grad_part(const GemmParams& p, float (&v)[32], int col, int row, uint32_t staging, int lane,
+                                                const RowValues& values, bool counts) {
+  const int lab = values.label >= 0 ? (int)(values.label - p.word0) : -1;
+  const float top = values.top, rest = values.rest;
+#pragma unroll
+  for (int i = 0; i < 32; ++i) v[i] = share_of(v[i], top, rest);
+  const int hit = lab - col;
+  if (lab >= 0 && hit >= 0 && hit < 32) {
+#pragma unroll
+    for (int i = 0; i < 32; ++i)
+      if (i == hit) v[i] = -1.f;
+  }
+  // the zero rows behind the last one, which pad the inner dimension of dW: where a word of W holds an
+  // infinity their logits are NaN
+  if (!counts) {
+#pragma unroll
+    for (int i = 0; i < 32; ++i) v[i] = 0.f;
+  }
+  stage_bf16(staging, lane, v);
+  if (lane == 0) {
+    if (col < p.words && row < p.padded) tma_store(&p.out, staging, col, row);
+    store_commit();
+  }
+}
+
 template <class Release>
 __device__ __forceinline__ void logit_grad_tile(const GemmParams& p, const Tile& x, uint32_t tmem, int row, int half, uint32_t staging,
                                                 int lane, const RowValues& values, bool counts, const Release& release) {
-  const int lab = values.label >= 0 ? (int)(values.label - p.word0) : -1;
-  const float top = values.top, rest = values.rest;
 #pragma unroll 1
   for (int c = 0; c < 4; ++c) {
     float v[32];
     tmem_load32(tmem + c * 32, v);
     if (c == 3) release();
-    const int col = x.n + half * 128 + c * 32;
-#pragma unroll
-    for (int i = 0; i < 32; ++i) v[i] = share_of(v[i], top, rest);
-    const int hit = lab - col;
-    if (lab >= 0 && hit >= 0 && hit < 32) {
-#pragma unroll
-      for (int i = 0; i < 32; ++i)
-        if (i == hit) v[i] = -1.f;
-    }
-    // the zero rows behind the last one, which pad the inner dimension of dW: where a word of W holds an
-    // infinity their logits are NaN
-    if (!counts) {
-#pragma unroll
-      for (int i = 0; i < 32; ++i) v[i] = 0.f;
-    }
-    stage_bf16(staging, lane, v);
-    if (lane == 0) {
-      if (col < p.words && row < p.padded) tma_store(&p.out, staging, col, row);
-      store_commit();
-    }
+    logit_grad_part(p, v, x.n + half * 128 + c * 32, row, staging, lane, values, counts);
   }
 }
 
@@ -446,20 +453,22 @@ __device__ __forceinline__ void dw_tile(const GemmParams& p, const Tile& x, uint
 }
 
 // --------------------------------------------------------------------- product
-template <int PASS>
+// LONG: the gradient of logits of several chains; an instance of its own, as the sums take registers
+template <int PASS, bool LONG>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmThreads, 1)
 lce_product_kernel(const __grid_constant__ GemmParams p) {
   extern __shared__ uint8_t smem_raw[];
   __shared__ uint64_t full[kStages], empty[kStages], done[2], drained[2];
   __shared__ uint32_t tmem_at;
   __shared__ int gave_up;
-  __shared__ float2 row_part[PASS == kStats ? 2 : 1][4][PASS == kStats ? 128 : 1];  // by turn, columns and row
+  __shared__ float2 row_part[2][4][PASS == kStats ? 128 : 1];  // by turn, columns and row
   __shared__ volatile int stop[8][2];  // of two epilogue warps of the same 32 rows, by turn
   const uint32_t stages = (smem_addr(smem_raw) + 1023u) & ~1023u;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = cluster_rank();
   const uint32_t full0 = smem_addr(full), empty0 = smem_addr(empty), done0 = smem_addr(done), drained0 = smem_addr(drained);
-  const bool chained = p.hidden > kChain * kInner;  // the statistics' sums
+  constexpr int kLength = PASS == kStats ? kChain : kGradChain;  // stages of a chain; kGrads has one a tile
+  const bool chained = PASS == kStats ? p.hidden > kLength * kInner : LONG;
 
   if (threadIdx.x == 0) {
     gave_up = 0;
@@ -470,7 +479,7 @@ lce_product_kernel(const __grid_constant__ GemmParams p) {
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(done0 + 8 * i, 1);
-      mbar_init(drained0 + 8 * i, PASS == kStats && chained ? 2 * kEpilogueWarps : kEpilogueWarps);  // of both CTAs
+      mbar_init(drained0 + 8 * i, chained ? 2 * kEpilogueWarps : kEpilogueWarps);  // of both CTAs
     }
     mbar_init_fence();
     prefetch_map(&p.a);
@@ -540,7 +549,7 @@ lce_product_kernel(const __grid_constant__ GemmParams p) {
         const uint32_t idesc = instruction(kTile, x.narrow ? kTile / 2 : kTile, outer_a, outer_b);
         int k = 0;
         do {  // one chain; a tile of no stage has an empty one
-          const int last = PASS == kStats && k + kChain < x.steps ? k + kChain : x.steps;
+          const int last = PASS != kGrads && k + kLength < x.steps ? k + kLength : x.steps;
           const uint32_t acc = chains & 1, d = tmem + acc * kTile;
           if (!mbar_wait(drained0 + 8 * acc, ((chains >> 1) & 1) ^ 1)) { ok = false; break; }
           fence_after();
@@ -566,8 +575,10 @@ lce_product_kernel(const __grid_constant__ GemmParams p) {
       }
     }
     __syncwarp();
-  } else if (PASS == kStats && chained) {
+  } else if ((PASS == kStats || LONG) && chained) {
     // warps 2 to 17: four rows of 32, four of 64 columns; the sums of a tile stay in registers
+    const uint32_t staging = stages + kStages * kStageBytes + (warp - 2) * kStagingBytes;
+    if (PASS == kLogitGrad) prepare_rows(p, n_rows, blockIdx.x * kEpilogueWarps + warp - 2, gridDim.x * kEpilogueWarps);
     const int quarter = warp & 3, part = (warp - 2) >> 2, in_cta = quarter * 32 + lane, mates = quarter + (part >> 1) * 4;
     const uint32_t lead_drained0 = map_to_rank(drained0, 0);
     int chains = 0;
@@ -576,7 +587,7 @@ lce_product_kernel(const __grid_constant__ GemmParams p) {
       const int row = x.m + (int)rank * 128 + in_cta, turn = mine & 1;
       const RowValues values = row_values<PASS>(p, row, n_rows);  // on their way while the products run
       float v[64];
-      for (int k = 0; k < x.steps && ok; k += kChain, ++chains) {
+      for (int k = 0; k < x.steps && ok; k += kLength, ++chains) {
         const uint32_t acc = chains & 1, at = tmem + acc * kTile + part * 64 + ((uint32_t)(quarter * 32) << 16);
         ok = mbar_wait(done0 + 8 * acc, (chains >> 1) & 1);
         ok = __all_sync(0xffffffffu, ok);
@@ -597,6 +608,12 @@ lce_product_kernel(const __grid_constant__ GemmParams p) {
         __syncwarp();
         if (lane == 0) mbar_arrive_cluster(lead_drained0 + 8 * acc);
       }
+      if (PASS == kLogitGrad) {
+        if (!ok) break;
+        logit_grad_part(p, reinterpret_cast<float(&)[32]>(v[0]), x.n + part * 64, row, staging, lane, values, row < n_rows);
+        logit_grad_part(p, reinterpret_cast<float(&)[32]>(v[32]), x.n + part * 64 + 32, row, staging, lane, values, row < n_rows);
+        continue;
+      }
       // The two warps of these rows and 128 columns join.  One that gave up comes here, too, and both
       // leave: what belongs to a turn is written again two turns later, when they have met once more.
       if (ok) row_part[turn][part][in_cta] = stats_of(v, x.n + part * 64, p.words, values.label);
@@ -607,6 +624,8 @@ lce_product_kernel(const __grid_constant__ GemmParams p) {
       if ((part & 1) == 0 && row < n_rows)
         p.part[(int64_t)(x.n / 128 + (part >> 1)) * p.rows + row] = join2(row_part[turn][part][in_cta], row_part[turn][part + 1][in_cta]);
     }
+    if (PASS != kStats && lane == 0) store_wait();
+    __syncwarp();
   } else {
     const int quarter = warp & 3, half = ((warp - 2) >> 2) & 1, group = (warp - 2) >> 3;
     const uint32_t lead_drained0 = map_to_rank(drained0, 0);
@@ -743,7 +762,7 @@ struct FewShape {
 // Stages of a chain of the statistics.  One row of 128256 words x 4096: 174 us without chains, 179 with
 // four stages, 186 with two; the loss of a confident row up to 25, 1.0 and 0.8e-6 off 64 bits.
 constexpr int kFewChain = 4;
-// Of the gradients; only dh has as many.
+// Of dh; the logits for backward have theirs of kGradChain.
 constexpr int kFewSumChain = kLceSumTerms / kInner;
 template <int N>
 __device__ __forceinline__ void tmem_load_rows(uint32_t at, float (&v)[N]) {
@@ -759,7 +778,7 @@ template <int PASS, int N>
 __global__ void __launch_bounds__(kFewThreads, 1)
 lce_few_kernel(const __grid_constant__ GemmParams p, float* acc, const JoinArgs j) {
   using S = FewShape<N>;
-  constexpr int kLength = PASS == kStats ? kFewChain : kFewSumChain;  // stages of a chain
+  constexpr int kLength = PASS == kStats ? kFewChain : PASS == kLogitGrad ? kGradChain : kFewSumChain;  // stages of a chain
   extern __shared__ uint8_t smem_raw[];
   __shared__ uint64_t full[S::kCount], empty[S::kCount], done[S::kAccs], drained[S::kAccs];
   __shared__ uint32_t tmem_at;
@@ -1468,17 +1487,17 @@ cudaError_t allow_smem(std::atomic<uint64_t>& done, const void* kernel, int byte
   return e;
 }
 
-template <int PASS>
+template <int PASS, bool LONG = false>
 cudaError_t launch_product(const GemmParams& p, int64_t tiles, cudaStream_t st) {
   if (tiles <= 0) return cudaSuccess;
   if (tiles > (int64_t(1) << 30)) return cudaErrorInvalidValue;
   constexpr int smem = smem_of(PASS != kStats);
   static std::atomic<uint64_t> done{0};
-  const cudaError_t e = allow_smem(done, (const void*)lce_product_kernel<PASS>, smem);
+  const cudaError_t e = allow_smem(done, (const void*)lce_product_kernel<PASS, LONG>, smem);
   if (e != cudaSuccess) return e;
   const int pairs = (int)(tiles < kNumSMs / 2 ? tiles : kNumSMs / 2);
   count_launch();
-  return launch_behind(lce_product_kernel<PASS>, dim3(2 * pairs), kGemmThreads, smem, st, p);
+  return launch_behind(lce_product_kernel<PASS, LONG>, dim3(2 * pairs), kGemmThreads, smem, st, p);
 }
 
 template <int PASS, int N>
@@ -1674,7 +1693,9 @@ cudaError_t launch_lce_backward(const LceArgs& a, const LceGrad& g, cudaStream_t
     } else {
       if (!encode(&p.out, g.d, q.words, p.padded, pitch, 32, 32) || !encode(&q.a, g.d, q.words, p.padded, pitch, 128))
         return cudaErrorInvalidValue;
-      if ((e = launch_product<kLogitGrad>(p, tiles_of(a.rows) * tiles_of(p.words), st)) != cudaSuccess) return e;
+      const int64_t tiles = tiles_of(a.rows) * tiles_of(p.words);
+      e = a.hidden > kGradChain * kInner ? launch_product<kLogitGrad, true>(p, tiles, st) : launch_product<kLogitGrad>(p, tiles, st);
+      if (e != cudaSuccess) return e;
     }
     p.scaled = p.gh = nullptr;  // the first piece has done it
     if (is_few) {

@@ -177,3 +177,54 @@ def test_gradient_of_hidden_states_over_many_words(n, hidden, vocab, piece):
     # 1 / (vocab - 1) is exact in bf16; 4096 additions are off by 2^-23 of the sum each at most, and up to 32
     # such sums add up in fp32; the result rounds to bf16
     assert ((gh.double() - want).abs() <= (2.0 ** -8 + 2.0 ** -11) * want).all()
+
+
+@gpu
+@pytest.mark.parametrize("n,hidden", [(20, 8192), (20, 8200), (300, 8192), (300, 8200), (300, 16384), (130, 16456), (20, 1 << 17), (130, 1 << 17),
+                                      (50, 1 << 18), (300, 1 << 18)])
+def test_logits_of_many_terms(n, hidden):
+    """Logits of 32 that are sums of terms of one sign, the same for every word but the label."""
+    gen = torch.Generator(device="cuda").manual_seed(hidden)
+    vocab = 257
+    h = torch.randint(64, 193, (n, hidden), generator=gen, device="cuda").float() / 128
+    h = (h / h.mean(1, keepdim=True)).to(BF16)
+    w = torch.full((vocab, hidden), 32.0 / hidden, device="cuda", dtype=BF16)
+    w[0] = 0.0
+    labels = torch.zeros(n, dtype=torch.int64, device="cuda")
+    labels[1::3] = -100
+    h.requires_grad_(True)
+    w.requires_grad_(True)
+    loss = linear_cross_entropy(h, w, labels, reduction="none")
+    gh, gw = torch.autograd.grad(loss.sum(), (h, w))
+    rows = labels == 0
+    z = h.detach().double()[rows].sum(1) * w[1, 0].item()
+    assert ((loss[rows].double() - (z + math.log(vocab - 1))).abs() <= 2.0 ** -12).all()
+    total = h.detach().double()[rows].sum(0)
+    # 1 - p is 1 to 2^-37.  A chain of 8192 terms is 512 additions, each off by 2^-23 of 32 at most: 2^-9
+    # in a logit; up to 32 chains add up in fp32, 2^-13; d and the result round to bf16
+    for got, want in ((gw[0], -total), (gw[1:], total / (vocab - 1))):
+        assert ((got.double() - want).abs() <= (2 * 2.0 ** -8 + 2.0 ** -9 + 2.0 ** -12) * want.abs()).all()
+    want = (w[1:].detach().double().sum(0) / (vocab - 1)).expand(int(rows.sum()), hidden)
+    assert ((gh[rows].double() - want).abs() <= (2 * 2.0 ** -8 + 2.0 ** -9 + 2.0 ** -12) * want.abs()).all()
+    assert (gh[~rows] == 0).all()
+
+
+@gpu
+@pytest.mark.parametrize("n,hidden,vocab", [(20, 8264, 700), (300, 8264, 1025), (700, 12288, 4099)])
+def test_random_logits_of_many_terms(n, hidden, vocab):
+    gen = torch.Generator(device="cuda").manual_seed(n)
+    h = torch.randn(n, hidden, device="cuda", generator=gen).to(BF16).requires_grad_(True)
+    w = (torch.randn(vocab, hidden, device="cuda", generator=gen) / math.sqrt(hidden)).to(BF16).requires_grad_(True)
+    labels = torch.randint(0, vocab, (n,), device="cuda", generator=gen)
+    labels[::5] = -100
+    rows = labels != -100
+    x, y = h.detach().double()[rows], w.detach().double()
+    d = (x @ y.T).softmax(1)
+    p = d.clone()
+    d[torch.arange(len(x), device="cuda"), labels[rows]] -= 1
+    for piece in (None, 256):
+        gh, gw = torch.autograd.grad(linear_cross_entropy(h, w, labels, reduction="sum", piece=piece), (h, w))
+        # logits below 6, 512 additions in a chain: 2^-23 * 512 * 6 < 2^-11 in each
+        off = (d.abs() * 2.0 ** -8 + p * 2.0 ** -10)
+        assert ((gh[rows].double() - d @ y).abs() <= off @ y.abs() + (2.0 ** -8 + 2.0 ** -12) * (d.abs() @ y.abs())).all()
+        assert ((gw.double() - d.T @ x).abs() <= off.T @ x.abs() + (2 * 2.0 ** -8 + 2.0 ** -12) * (d.abs().T @ x.abs())).all()
