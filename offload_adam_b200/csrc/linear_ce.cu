@@ -81,6 +81,8 @@ struct GemmParams {
   int64_t word0;       // first word of the piece
   int words;           // and how many
   int64_t* report;
+  int* lost;           // set by a launch that gave up a wait: the results of all that follows are NaN
+  uint64_t wait_limit;
   const int* label;
   // kStats
   float2* part;
@@ -364,11 +366,12 @@ __device__ __forceinline__ void store_bf16x8(uint16_t* at, const float* v, float
   *reinterpret_cast<uint4*>(at) = o;
 }
 // What all rows of dh, and dW, are multiplied by.
-__device__ __forceinline__ float all_scale(const GemmParams& p) {
-  float scale = 1.f;
-  if (p.inv != nullptr) scale = *p.inv;
-  return p.g != nullptr ? __fmul_rn(scale, *p.g) : scale;
+__device__ __forceinline__ float all_scale(const float* inv, const float* g, const int* lost) {
+  float scale = *lost != 0 ? NAN : 1.f;
+  if (inv != nullptr) scale = __fmul_rn(scale, *inv);
+  return g != nullptr ? __fmul_rn(scale, *g) : scale;
 }
+__device__ __forceinline__ float all_scale(const GemmParams& p) { return all_scale(p.inv, p.g, p.lost); }
 // What packed row k of dh is multiplied by, beside the scale of all rows.
 __device__ __forceinline__ float row_scale(const GemmParams& p, int k, float scale) {
   scale = __fmul_rn(scale, p.miss[k]);
@@ -452,6 +455,26 @@ __device__ __forceinline__ void dw_tile(const GemmParams& p, const Tile& x, uint
   }
 }
 
+// At the end of a block that gave up a wait.  Its own tiles of the gradients were not all written, so it
+// makes NaN of all that the launch writes of `dw` and, where its rows go straight out, of `dh`; other
+// blocks may write theirs over that.
+__device__ __forceinline__ void give_up(const GemmParams& p, int n_rows, bool dh, bool dw) {
+  if (threadIdx.x == 0) {
+    *reinterpret_cast<volatile int64_t*>(p.report + 1) = 1;
+    *reinterpret_cast<volatile int*>(p.lost) = 1;
+  }
+  const int vecs = p.hidden >> 3;
+  const uint4 nan = make_uint4(0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u);
+  if (dh)
+    for (int k = 0; k < n_rows; ++k)
+      for (int v = threadIdx.x; v < vecs; v += blockDim.x) reinterpret_cast<uint4*>(p.gh + (int64_t)p.index[k] * p.hidden)[v] = nan;
+  if (dw) {
+    uint4* to = reinterpret_cast<uint4*>(p.gw + p.word0 * p.hidden);
+    for (int64_t v = threadIdx.x; v < (int64_t)p.words * vecs; v += blockDim.x) to[v] = nan;
+  }
+  __syncthreads();  // what follows is for whole warps
+}
+
 // --------------------------------------------------------------------- product
 // LONG: the gradient of logits of several chains; an instance of its own, as the sums take registers
 template <int PASS, bool LONG>
@@ -514,7 +537,7 @@ lce_product_kernel(const __grid_constant__ GemmParams p) {
         const int b_row0 = PASS == kLogitGrad ? (int)p.word0 : 0, b_k0 = PASS == kGrads && x.kind == 0 ? (int)p.word0 : 0;
         for (int k = 0; k < x.steps; ++k, ++it) {
           const int s = it % kStages;
-          if (!mbar_wait(empty0 + 8 * s, ((it / kStages) & 1) ^ 1)) { ok = false; break; }
+          if (!mbar_wait(empty0 + 8 * s, ((it / kStages) & 1) ^ 1, p.wait_limit)) { ok = false; break; }
           if (rank == 0) mbar_expect_tx(full0 + 8 * s, x.narrow ? 2 * kStageBytes - kHalfBytes : 2 * kStageBytes);
           const uint32_t at = stages + s * kStageBytes, bt = at + kHalfBytes, bar = lead_full0 + 8 * s;
           const int kk = x.k0 + k * kInner;
@@ -533,7 +556,7 @@ lce_product_kernel(const __grid_constant__ GemmParams p) {
         }
       }
       // every stage is released before this CTA may go: the last arrivals come from the partner
-      for (int i = 0; i < kStages && ok; ++i, ++it) ok = mbar_wait(empty0 + 8 * (it % kStages), ((it / kStages) & 1) ^ 1);
+      for (int i = 0; i < kStages && ok; ++i, ++it) ok = mbar_wait(empty0 + 8 * (it % kStages), ((it / kStages) & 1) ^ 1, p.wait_limit);
       if (!ok) {  // copies that are still under way end within microseconds
         for (int i = 0; i < 100; ++i) __nanosleep(10000);
       }
@@ -551,11 +574,11 @@ lce_product_kernel(const __grid_constant__ GemmParams p) {
         do {  // one chain; a tile of no stage has an empty one
           const int last = PASS != kGrads && k + kLength < x.steps ? k + kLength : x.steps;
           const uint32_t acc = chains & 1, d = tmem + acc * kTile;
-          if (!mbar_wait(drained0 + 8 * acc, ((chains >> 1) & 1) ^ 1)) { ok = false; break; }
+          if (!mbar_wait(drained0 + 8 * acc, ((chains >> 1) & 1) ^ 1, p.wait_limit)) { ok = false; break; }
           fence_after();
           for (bool begun = false; k < last; ++k, ++it) {
             const int s = it % kStages;
-            if (!mbar_wait(full0 + 8 * s, (it / kStages) & 1)) { ok = false; break; }
+            if (!mbar_wait(full0 + 8 * s, (it / kStages) & 1, p.wait_limit)) { ok = false; break; }
             fence_after();
             const uint32_t at = stages + s * kStageBytes, bt = at + kHalfBytes;
             const uint64_t da = outer_a ? operand(at, kHalfBytes / 2, 1024) : operand(at, 16, 1024);
@@ -569,6 +592,7 @@ lce_product_kernel(const __grid_constant__ GemmParams p) {
             }
             commit_pair(empty0 + 8 * s);
           }
+          if (!ok) break;
           commit_pair(done0 + 8 * acc);
           ++chains;
         } while (ok && k < x.steps);
@@ -589,7 +613,7 @@ lce_product_kernel(const __grid_constant__ GemmParams p) {
       float v[64];
       for (int k = 0; k < x.steps && ok; k += kLength, ++chains) {
         const uint32_t acc = chains & 1, at = tmem + acc * kTile + part * 64 + ((uint32_t)(quarter * 32) << 16);
-        ok = mbar_wait(done0 + 8 * acc, (chains >> 1) & 1);
+        ok = mbar_wait(done0 + 8 * acc, (chains >> 1) & 1, p.wait_limit);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
         fence_after();
@@ -637,7 +661,7 @@ lce_product_kernel(const __grid_constant__ GemmParams p) {
       const uint32_t acc = group;
       const int row = x.m + (int)rank * 128 + quarter * 32 + lane;
       const RowValues values = row_values<PASS>(p, row, n_rows);  // on their way while the products run
-      ok = mbar_wait(done0 + 8 * acc, (mine >> 1) & 1);
+      ok = mbar_wait(done0 + 8 * acc, (mine >> 1) & 1, p.wait_limit);
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
       fence_after();
@@ -668,7 +692,7 @@ lce_product_kernel(const __grid_constant__ GemmParams p) {
   if (!ok) gave_up = 1;
   fence_before();
   __syncthreads();
-  if (gave_up && threadIdx.x == 0) *reinterpret_cast<volatile int64_t*>(p.report + 1) = 1;
+  if (gave_up) give_up(p, n_rows, PASS == kGrads && p.want_dh && p.gh != nullptr, PASS == kGrads && p.want_dw && !p.wacc);
   cluster_sync();
   fence_after();
   if (warp == 1) tmem_free_pair(tmem, 512);
@@ -679,6 +703,7 @@ struct JoinArgs {
   const float *picked, *inv;
   float *top, *rest, *miss;
   int* count;
+  const int* lost;
   int reduction, parts;
   float* loss;  // null, of lce_few_kernel: a launch of its own joins
 };
@@ -732,7 +757,7 @@ __device__ __forceinline__ double finish_row(const JoinArgs& j, int64_t at, cons
   const double z = j.picked[at], top = m, rest = s;
   double loss_of;
   // an infinite logit of the label's own has no loss, as in PyTorch
-  if (label[at] < 0 || z == INFINITY) loss_of = NAN;
+  if (label[at] < 0 || z == INFINITY || __ldcg(j.lost) != 0) loss_of = NAN;
   else if (z >= top) loss_of = log1p(rest * exp(top - z));
   else loss_of = top - z + log(rest + exp(z - top));
   j.top[at] = finite_shift(m);  // all others -inf: exp(-inf - 0) is 0
@@ -850,7 +875,7 @@ lce_few_kernel(const __grid_constant__ GemmParams p, float* acc, const JoinArgs 
         const int steps = share(t, first), m = t % across * 128;
         for (int k = 0; k < steps; ++k, ++it) {
           const int s = it % S::kCount, kk = (first + k) * kInner;
-          if (!mbar_wait(empty0 + 8 * s, ((it / S::kCount) & 1) ^ 1)) { ok = false; break; }
+          if (!mbar_wait(empty0 + 8 * s, ((it / S::kCount) & 1) ^ 1, p.wait_limit)) { ok = false; break; }
           const uint32_t at = stages + s * S::kStage, bar = full0 + 8 * s;
           mbar_expect_tx(bar, S::kStage);
           if (PASS == kGrads) {
@@ -878,11 +903,11 @@ lce_few_kernel(const __grid_constant__ GemmParams p, float* acc, const JoinArgs 
         do {  // one chain; a tile of no stage has an empty one
           const int last = k + kLength < steps ? k + kLength : steps;
           const uint32_t buf = chains % S::kAccs, d = tmem + buf * N;
-          if (!mbar_wait(drained0 + 8 * buf, ((chains / S::kAccs) & 1) ^ 1)) { ok = false; break; }
+          if (!mbar_wait(drained0 + 8 * buf, ((chains / S::kAccs) & 1) ^ 1, p.wait_limit)) { ok = false; break; }
           fence_after();
           for (bool begun = false; k < last; ++k, ++it) {
             const int s = it % S::kCount;
-            if (!mbar_wait(full0 + 8 * s, (it / S::kCount) & 1)) { ok = false; break; }
+            if (!mbar_wait(full0 + 8 * s, (it / S::kCount) & 1, p.wait_limit)) { ok = false; break; }
             fence_after();
             const uint32_t at = stages + s * S::kStage;
             const uint64_t da = PASS == kGrads ? operand(at, kHalfBytes / 2, 1024) : operand(at, 16, 1024);
@@ -895,6 +920,7 @@ lce_few_kernel(const __grid_constant__ GemmParams p, float* acc, const JoinArgs 
             }
             commit(empty0 + 8 * s);
           }
+          if (!ok) break;
           commit(done0 + 8 * buf);
           ++chains;
         } while (ok && k < steps);
@@ -912,7 +938,7 @@ lce_few_kernel(const __grid_constant__ GemmParams p, float* acc, const JoinArgs 
       int k = 0;
       do {
         const uint32_t buf = chains % S::kAccs, from = tmem + buf * N + ((uint32_t)(quarter * 32) << 16);
-        ok = mbar_wait(done0 + 8 * buf, (chains / S::kAccs) & 1);
+        ok = mbar_wait(done0 + 8 * buf, (chains / S::kAccs) & 1, p.wait_limit);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
         fence_after();
@@ -987,9 +1013,10 @@ lce_few_kernel(const __grid_constant__ GemmParams p, float* acc, const JoinArgs 
       }
     }
   }
-  if (PASS == kStats && j.loss != nullptr && warp >= 2 && ok) {
+  if (PASS == kStats && j.loss != nullptr && warp >= 2) {
     // The block that is the last to come here joins the sums of all of them.
     const int t = threadIdx.x - 64;
+    if (!ok && t == 0) *reinterpret_cast<volatile int*>(p.lost) = 1;
     __threadfence();
     asm volatile("bar.sync 1, 128;" ::: "memory");
     if (t == 0) stop = atomicAdd(j.count + 1, 1) == (int)gridDim.x - 1;
@@ -1015,7 +1042,7 @@ lce_few_kernel(const __grid_constant__ GemmParams p, float* acc, const JoinArgs 
   if (!ok) gave_up = 1;
   fence_before();
   __syncthreads();
-  if (gave_up && threadIdx.x == 0) *reinterpret_cast<volatile int64_t*>(p.report + 1) = 1;
+  if (gave_up) give_up(p, n_rows, PASS == kGrads && p.gh != nullptr, false);
   fence_after();
   if (warp == 1) tmem_free(tmem, S::kColumns);
 }
@@ -1073,13 +1100,13 @@ lce_few_dw_kernel(const __grid_constant__ GemmParams p) {
       int m = first_m, column = begin - first_m * across;
       for (int t = begin; t < end && ok; ++t) {
         if (t == begin || column == 0) {
-          if (!mbar_wait(d_empty0, ((m - first_m) & 1) ^ 1)) { ok = false; break; }
+          if (!mbar_wait(d_empty0, ((m - first_m) & 1) ^ 1, p.wait_limit)) { ok = false; break; }
           mbar_expect_tx(d_full0, kHalfBytes);
           tma_load(d_at, &p.a2, m * 128, 0, d_full0);
           tma_load(d_at + kHalfBytes / 2, &p.a2, m * 128 + 64, 0, d_full0);
         }
         const int n = t - begin, s = n % kFewDwStages;
-        if (!mbar_wait(empty0 + 8 * s, ((n / kFewDwStages) & 1) ^ 1)) { ok = false; break; }
+        if (!mbar_wait(empty0 + 8 * s, ((n / kFewDwStages) & 1) ^ 1, p.wait_limit)) { ok = false; break; }
         mbar_expect_tx(full0 + 8 * s, 2 * kHalfBytes);
         for (int i = 0; i < 4; ++i)
           tma_load(stages + (s * 4 + i) * (kHalfBytes / 2), &p.b2, column * kTile + i * 64, 0, full0 + 8 * s);
@@ -1096,8 +1123,8 @@ lce_few_dw_kernel(const __grid_constant__ GemmParams p) {
       int m = first_m, column = begin - first_m * across;
       for (int t = begin; t < end && ok; ++t) {
         const int n = t - begin, s = n % kFewDwStages, acc = n & 1;
-        if ((t == begin || column == 0) && !mbar_wait(d_full0, (m - first_m) & 1)) { ok = false; break; }
-        if (!mbar_wait(drained0 + 8 * acc, ((n >> 1) & 1) ^ 1) || !mbar_wait(full0 + 8 * s, (n / kFewDwStages) & 1)) { ok = false; break; }
+        if ((t == begin || column == 0) && !mbar_wait(d_full0, (m - first_m) & 1, p.wait_limit)) { ok = false; break; }
+        if (!mbar_wait(drained0 + 8 * acc, ((n >> 1) & 1) ^ 1, p.wait_limit) || !mbar_wait(full0 + 8 * s, (n / kFewDwStages) & 1, p.wait_limit)) { ok = false; break; }
         fence_after();
         const uint64_t da = operand(d_at, kHalfBytes / 2, 1024), db = operand(stages + s * 2 * kHalfBytes, kHalfBytes / 2, 1024);
 #pragma unroll
@@ -1119,7 +1146,7 @@ lce_few_dw_kernel(const __grid_constant__ GemmParams p) {
     const uint32_t staging = d_at + kHalfBytes + (warp - 2) * kFewDwStaging;
     for (int t = begin + group; t < end; t += 2) {
       const int m = t / across, column = t - m * across;
-      ok = mbar_wait(done0 + 8 * group, ((t - begin) >> 1) & 1);
+      ok = mbar_wait(done0 + 8 * group, ((t - begin) >> 1) & 1, p.wait_limit);
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
       fence_after();
@@ -1156,7 +1183,7 @@ lce_few_dw_kernel(const __grid_constant__ GemmParams p) {
   if (!ok) gave_up = 1;
   fence_before();
   __syncthreads();
-  if (gave_up && threadIdx.x == 0) *reinterpret_cast<volatile int64_t*>(p.report + 1) = 1;
+  if (gave_up) give_up(p, 0, false, true);
   fence_after();
   if (warp == 1) tmem_free(tmem, 512);
 }
@@ -1165,10 +1192,10 @@ lce_few_dw_kernel(const __grid_constant__ GemmParams p) {
 constexpr int kScanThreads = 1024;
 
 // index[k] = row of the k-th label that counts, label[k] = that label (-1: outside the vocabulary),
-// count[0] = how many, count[1] = 0, inv; row_loss of ignored rows = 0.
+// count[0] = how many, count[1] = 0, inv, lost = 0; row_loss of ignored rows = 0.
 __global__ void __launch_bounds__(kScanThreads)
 lce_scan_kernel(const int64_t* __restrict__ labels, int64_t rows, int64_t vocab, int64_t ignore, int* index, int* label,
-                int* count, float* inv, float* row_loss, volatile int64_t* bad) {
+                int* count, float* inv, int* lost, float* row_loss, volatile int64_t* bad) {
   __shared__ int warps[kScanThreads / 32 + 1];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   int base = 0;
@@ -1205,7 +1232,7 @@ lce_scan_kernel(const int64_t* __restrict__ labels, int64_t rows, int64_t vocab,
   }
   if (threadIdx.x == 0) {
     count[0] = base;
-    count[1] = 0;
+    count[1] = *lost = 0;
     *inv = __fdiv_rn(1.f, (float)(base < 1 ? 1 : base));
   }
 }
@@ -1271,7 +1298,7 @@ constexpr int kScanPackRows = 4096, kScanPackBlockRows = 512;  // the latter: a 
 template <int THREADS>
 __global__ void __launch_bounds__(kPackThreads)
 lce_scan_pack_kernel(const PackArgs a, const int64_t* __restrict__ labels, int rows, int64_t vocab, int64_t ignore, int* index,
-                     int* label, int* count, float* inv, float* row_loss, volatile int64_t* bad) {
+                     int* label, int* count, float* inv, int* lost, float* row_loss, volatile int64_t* bad) {
   constexpr int kOwn = kPackThreads / THREADS, kEach = (THREADS == 32 ? kScanPackRows : kScanPackBlockRows) / kPackThreads;
   __shared__ int warps[kPackThreads / 32], source[kOwn], source_label[kOwn];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, first = blockIdx.x * kOwn;
@@ -1315,7 +1342,7 @@ lce_scan_pack_kernel(const PackArgs a, const int64_t* __restrict__ labels, int r
   }
   if (blockIdx.x == 0 && threadIdx.x == 0) {
     count[0] = n;
-    count[1] = 0;
+    count[1] = *lost = 0;
     *inv = __fdiv_rn(1.f, (float)(n < 1 ? 1 : n));
   }
   __syncthreads();
@@ -1377,14 +1404,15 @@ lce_join_kernel(const float2* __restrict__ part, int64_t rows, const int* __rest
 __global__ void __launch_bounds__(128)
 lce_join_grad_kernel(const float* __restrict__ acc, int splits, int64_t padded, int64_t pitch, const int* __restrict__ index,
                      const int64_t* __restrict__ labels, int64_t ignore, const int* __restrict__ count, int hidden,
-                     const float* __restrict__ miss, const float* inv, const float* g, const float* row_g, uint16_t* gh) {
+                     const float* __restrict__ miss, const float* inv, const float* g, const int* lost, const float* row_g,
+                     uint16_t* gh) {
   const int64_t k = blockIdx.x;
   const int col = (blockIdx.y * 128 + threadIdx.x) * 8;
   grid_wait();
   if (col >= hidden) return;
   if (labels[k] == ignore) *reinterpret_cast<uint4*>(gh + k * hidden + col) = make_uint4(0, 0, 0, 0);
   if (k >= *count) return;
-  float scale = miss[k];
+  float scale = *lost != 0 ? NAN : miss[k];
   if (inv != nullptr) scale = __fmul_rn(scale, *inv);
   if (g != nullptr) scale = __fmul_rn(scale, *g);
   if (row_g != nullptr) scale = __fmul_rn(scale, row_g[index[k]]);
@@ -1400,13 +1428,13 @@ lce_join_grad_kernel(const float* __restrict__ acc, int splits, int64_t padded, 
 // ------------------------------------------------------- dW of many rows, rounded
 // One piece, from its fp32 sums.
 __global__ void __launch_bounds__(128)
-lce_round_head_kernel(const float* __restrict__ acc, int64_t pitch, int hidden, const float* inv, const float* g, uint16_t* gw) {
+lce_round_head_kernel(const float* __restrict__ acc, int64_t pitch, int hidden, const float* inv, const float* g, const int* lost,
+                      uint16_t* gw) {
   const int64_t word = blockIdx.x;
   const int col = (blockIdx.y * 128 + threadIdx.x) * 8;
   grid_wait();
   if (col >= hidden) return;
-  float scale = inv != nullptr ? *inv : 1.f;
-  if (g != nullptr) scale = __fmul_rn(scale, *g);
+  const float scale = all_scale(inv, g, lost);
   const V8 x = ld32(acc + word * pitch + col);
   float v[8];
 #pragma unroll
@@ -1536,6 +1564,9 @@ bool args_ok(const LceArgs& a) {
          a.w_stride < (int64_t(1) << 36);
 }
 
+// Nanoseconds.  The longest tile that the sizes allow takes milliseconds.
+std::atomic<uint64_t> wait_limit{2000000000ull};
+
 void common_params(GemmParams& p, const LceArgs& a) {
   p.count = a.count;
   p.rows = a.rows;
@@ -1543,10 +1574,14 @@ void common_params(GemmParams& p, const LceArgs& a) {
   p.hidden = (int)a.hidden;
   p.row_pitch = lce_row_pitch(a.hidden);
   p.report = a.report;
+  p.lost = a.lost;
+  p.wait_limit = wait_limit.load(std::memory_order_relaxed);
   p.label = a.label;
 }
 
 }  // namespace
+
+uint64_t lce_wait_limit(uint64_t nanoseconds) { return wait_limit.exchange(nanoseconds); }
 
 int64_t lce_part_floats(int64_t rows, int64_t vocab) {
   return 2 * rows * (rows <= kLceFewRows ? (vocab + 127) / 128 : 2 * tiles_of(vocab));
@@ -1562,14 +1597,14 @@ cudaError_t launch_lce_forward(const LceArgs& a, int reduction, float* part, flo
   if (a.rows <= kScanPackBlockRows) {
     count_launch();
     lce_scan_pack_kernel<kPackThreads><<<(unsigned)lce_padded(a.rows), kPackThreads, 0, st>>>(
-        k, a.labels, (int)a.rows, a.vocab, a.ignore, a.index, a.label, a.count, a.inv, row_loss, a.report);
+        k, a.labels, (int)a.rows, a.vocab, a.ignore, a.index, a.label, a.count, a.inv, a.lost, row_loss, a.report);
   } else if (a.rows <= kScanPackRows) {
     count_launch();
     lce_scan_pack_kernel<32><<<blocks, kPackThreads, 0, st>>>(k, a.labels, (int)a.rows, a.vocab, a.ignore, a.index, a.label, a.count,
-                                                              a.inv, row_loss, a.report);
+                                                              a.inv, a.lost, row_loss, a.report);
   } else {
     count_launch(2);
-    lce_scan_kernel<<<1, kScanThreads, 0, st>>>(a.labels, a.rows, a.vocab, a.ignore, a.index, a.label, a.count, a.inv, row_loss,
+    lce_scan_kernel<<<1, kScanThreads, 0, st>>>(a.labels, a.rows, a.vocab, a.ignore, a.index, a.label, a.count, a.inv, a.lost, row_loss,
                                                 a.report);
     lce_pack_kernel<<<blocks, kPackThreads, 0, st>>>(k, a.index, a.label, a.count);
   }
@@ -1581,7 +1616,7 @@ cudaError_t launch_lce_forward(const LceArgs& a, int reduction, float* part, flo
   p.part = reinterpret_cast<float2*>(part);
   const bool few = a.rows <= kLceFewRows;
   p.index = a.index;
-  JoinArgs j{picked, a.inv, a.top, a.rest, a.miss, a.count, reduction, (int)(few ? (a.vocab + 127) / 128 : 2 * tiles_of(a.vocab)), loss};
+  JoinArgs j{picked, a.inv, a.top, a.rest, a.miss, a.count, a.lost, reduction, (int)(few ? (a.vocab + 127) / 128 : 2 * tiles_of(a.vocab)), loss};
   if (few) {
     if (!encode(&p.a, a.w, a.hidden, a.vocab, a.w_stride, 128) ||
         !encode(&p.b, a.packed, a.hidden, p.padded, p.row_pitch, few_columns(a.rows)))
@@ -1713,14 +1748,14 @@ cudaError_t launch_lce_backward(const LceArgs& a, const LceGrad& g, cudaStream_t
     if (q.wacc) {
       count_launch();
       e = launch_behind(lce_round_head_kernel, dim3((unsigned)q.words, (unsigned)((a.hidden + 1023) / 1024)), 128, 0, st, g.wacc, p.row_pitch,
-                        (int)a.hidden, q.inv, q.g, (uint16_t*)g.gw + q.word0 * a.hidden);
+                        (int)a.hidden, q.inv, q.g, a.lost, (uint16_t*)g.gw + q.word0 * a.hidden);
       if (e != cudaSuccess) return e;
     }
   }
   if (g.gh != nullptr && !direct) {
     count_launch();
     e = launch_behind(lce_join_grad_kernel, dim3((unsigned)a.rows, (unsigned)((a.hidden + 1023) / 1024)), 128, 0, st, g.acc, g.splits,
-                      p.padded, p.row_pitch, a.index, a.labels, a.ignore, a.count, (int)a.hidden, a.miss, q.inv, q.g, p.row_g,
+                      p.padded, p.row_pitch, a.index, a.labels, a.ignore, a.count, (int)a.hidden, a.miss, q.inv, q.g, a.lost, p.row_g,
                       (uint16_t*)g.gh);
   }
   return e;

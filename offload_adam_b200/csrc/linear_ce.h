@@ -27,6 +27,7 @@ struct LceArgs {
   int* label = nullptr;              // (rows,) label of the packed row, -1: outside the vocabulary
   int* count = nullptr;              // [0] packed rows, [1] ticket
   float* inv = nullptr;              // 1 / max(1, packed rows)
+  int* lost = nullptr;               // not 0: a kernel gave up a wait, the loss and gradients are NaN
   float* top = nullptr;              // (rows,) largest logit of the packed row without its label, 0 where that is -inf
   float* rest = nullptr;             // (rows,) log2 of the sum of exp(logit - top) over the same words
   float* miss = nullptr;             // (rows,) 1 - probability of its label
@@ -42,6 +43,10 @@ inline int64_t lce_padded(int64_t rows) { return (rows + kLceRowPad - 1) / kLceR
 inline int64_t lce_row_pitch(int64_t hidden) { return (hidden + 63) / 64 * 64; }
 
 enum LceReduction : int { kLceNone = 0, kLceMean = 1, kLceSum = 2 };
+
+// How long a wait of the kernels for their own pipeline may take from now on; what it was.  0: none waits,
+// every launch gives up.
+uint64_t lce_wait_limit(uint64_t nanoseconds);
 
 // Floats of `part` and doubles of `sums` that the forward pass needs.
 int64_t lce_part_floats(int64_t rows, int64_t vocab);

@@ -29,7 +29,7 @@ int64_t row_stride(const Tensor& t) { return t.size(0) == 1 ? t.size(1) : t.stri
 
 // What backward needs of forward, in one tensor of bytes: the packed rows of h (backward needs them in
 // any case, so keeping them instead of h leaves its peak), then index, label, top, rest and miss of each,
-// their number with the ticket, 1 / number.
+// their number with the ticket, 1 / number, and whether a wait was given up.
 int64_t packed_bytes(int64_t rows, int64_t hidden) { return 2 * oab::lce_padded(rows) * oab::lce_row_pitch(hidden); }
 int64_t kept_bytes(int64_t rows, int64_t hidden) { return packed_bytes(rows, hidden) + 4 * (5 * rows + 4); }
 oab::LceArgs make_args(const Tensor& w, const Tensor& labels, void* kept, int64_t ignore) {
@@ -50,6 +50,7 @@ oab::LceArgs make_args(const Tensor& w, const Tensor& labels, void* kept, int64_
   a.miss = reinterpret_cast<float*>(k + 4 * a.rows);
   a.count = k + 5 * a.rows;
   a.inv = reinterpret_cast<float*>(k + 5 * a.rows + 2);
+  a.lost = k + 5 * a.rows + 3;
   a.report = oab::loss_report();
   return a;
 }
@@ -191,5 +192,6 @@ py::object linear_ce(const Tensor& h, const Tensor& w, const Tensor& labels, int
 void bind_linear_ce(py::module_& m) {
   m.def("linear_ce", &linear_ce, py::arg("h"), py::arg("w"), py::arg("labels"), py::arg("reduction"), py::arg("ignore"), py::arg("piece"),
         py::arg("required") = true);
+  m.def("linear_ce_wait_limit", &oab::lce_wait_limit, py::arg("nanoseconds"));
   m.def("linear_ce_piece", &oab::lce_default_piece, py::arg("rows"), py::arg("hidden"), py::arg("vocab"));
 }

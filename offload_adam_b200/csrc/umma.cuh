@@ -56,28 +56,27 @@ __device__ __forceinline__ bool mbar_try(uint32_t bar, uint32_t parity) {
       : "memory");
   return done != 0;
 }
-// A wait ends: false after two seconds, looked at every kWaitLook tries, or after kWaitTries.  The
-// longest tile that the sizes allow (2^24 rows into one tile of a head's gradient) takes a tenth of
-// a second.
+// A wait ends: false after `limit` nanoseconds, looked at every kWaitLook tries, or after kWaitTries; with a
+// limit of 0 without a look.
 constexpr uint32_t kWaitLook = 1u << 14, kWaitTries = 1u << 28;
-constexpr uint64_t kWaitNanoseconds = 2000000000ull;
 __device__ __forceinline__ uint64_t nanoseconds() {
   uint64_t t;
   asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
   return t;
 }
-__device__ __forceinline__ bool mbar_wait_long(uint32_t bar, uint32_t parity) {
+__device__ __forceinline__ bool mbar_wait_long(uint32_t bar, uint32_t parity, uint64_t limit) {
   const uint64_t begin = nanoseconds();
   for (uint32_t i = 0; i < kWaitTries; ++i) {
     if (mbar_try(bar, parity)) return true;
-    if (i % kWaitLook == kWaitLook - 1 && nanoseconds() - begin > kWaitNanoseconds) return false;
+    if (i % kWaitLook == kWaitLook - 1 && nanoseconds() - begin > limit) return false;
   }
   return false;
 }
-__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity) {
+__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, uint64_t limit) {
+  if (limit == 0) return false;
   for (int i = 0; i < 64; ++i)
     if (mbar_try(bar, parity)) return true;
-  return mbar_wait_long(bar, parity);
+  return mbar_wait_long(bar, parity, limit);
 }
 // The address of the same shared variable in CTA `rank` of the cluster.
 __device__ __forceinline__ uint32_t map_to_rank(uint32_t addr, uint32_t rank) {

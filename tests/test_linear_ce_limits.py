@@ -6,6 +6,7 @@ import math
 import pytest
 import torch
 
+from offload_adam_b200 import _ext
 from offload_adam_b200.ops.linear_ce import linear_cross_entropy
 
 gpu = pytest.mark.gpu
@@ -228,3 +229,72 @@ def test_random_logits_of_many_terms(n, hidden, vocab):
         off = (d.abs() * 2.0 ** -8 + p * 2.0 ** -10)
         assert ((gh[rows].double() - d @ y).abs() <= off @ y.abs() + (2.0 ** -8 + 2.0 ** -12) * (d.abs() @ y.abs())).all()
         assert ((gw.double() - d.T @ x).abs() <= off.T @ x.abs() + (2 * 2.0 ** -8 + 2.0 ** -12) * (d.abs().T @ x.abs())).all()
+
+
+# every kind of launch: few rows whose last block joins, or a launch behind it; sums in one chain or
+# several; rows that go straight out, splits, pieces, groups of rows
+@gpu
+@pytest.mark.parametrize("reduction", ["mean", "none"])
+@pytest.mark.parametrize("n,hidden,vocab,piece", [
+    (5, 64, 300, None), (40, 72, 3000, None), (8, 136, 9001, 1024), (100, 64, 300, None), (100, 1032, 700, None), (300, 520, 5000, None),
+    (300, 264, 5000, 1024), (100, 8264, 300, None), (66000, 64, 300, None)])
+def test_a_wait_that_gives_up(n, hidden, vocab, piece, reduction):
+    """A pipeline that waits in vain ends its launch: the results of that call are NaN, the next call that
+    looks raises, and everything after it is as before."""
+    C = _ext.load(required=True)
+    gen = torch.Generator(device="cuda").manual_seed(n)
+    h = torch.randn(n, hidden, device="cuda", generator=gen).to(BF16).requires_grad_(True)
+    w = (torch.randn(vocab, hidden, device="cuda", generator=gen) / math.sqrt(hidden)).to(BF16).requires_grad_(True)
+    labels = torch.randint(0, vocab, (n,), device="cuda", generator=gen)
+    labels[::4] = -100
+    rows = labels != -100
+    g = torch.ones(n if reduction == "none" else (), device="cuda")
+
+    def forward():
+        return linear_cross_entropy(h, w, labels, reduction=reduction, piece=piece)
+
+    def grads(loss):
+        return torch.autograd.grad(loss, (h, w), g, retain_graph=True)
+
+    def in_vain(f, *args):
+        before = C.linear_ce_wait_limit(0)
+        try:
+            out = f(*args)
+        finally:
+            C.linear_ce_wait_limit(before)
+        torch.cuda.synchronize()
+        return out
+
+    def all_nan(loss):
+        return loss.isnan().all() if reduction == "mean" else loss[rows].isnan().all() and (loss[~rows] == 0).all()
+
+    def gradients_nan(gh, gw):
+        return gw.isnan().all() and gh[rows].isnan().all() and (gh[~rows] == 0).all()
+
+    good = forward()
+    want = grads(good)
+    with torch.no_grad():
+        assert all_nan(in_vain(forward))
+        with pytest.raises(RuntimeError, match="gave up waiting"):
+            forward()
+        assert torch.equal(forward(), good)
+    lost = in_vain(forward)
+    assert all_nan(lost)
+    with pytest.raises(RuntimeError, match="gave up waiting"):
+        grads(lost)
+    assert gradients_nan(*grads(lost))
+    again = forward()
+    assert torch.equal(again, good)
+    assert gradients_nan(*in_vain(grads, again))
+    with pytest.raises(RuntimeError, match="gave up waiting"):
+        forward()
+    again = forward()
+    assert torch.equal(again, good)
+    for a, b in zip(grads(again), want):
+        assert torch.equal(a, b)
+    for one in (0, 1):  # one gradient alone
+        again = forward()
+        alone, = in_vain(torch.autograd.grad, again, (h, w)[one], g)
+        assert alone[rows].isnan().all() if one == 0 else alone.isnan().all()
+        with pytest.raises(RuntimeError, match="gave up waiting"):
+            forward()
