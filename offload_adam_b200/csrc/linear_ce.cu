@@ -755,13 +755,14 @@ __device__ __forceinline__ void join_warp(float& m, float& s, float m2, float s2
 // The loss of packed row `at` from the maximum and the sum of its other words; what backward needs.
 __device__ __forceinline__ double finish_row(const JoinArgs& j, int64_t at, const int* index, const int* label, float m, float s) {
   const double z = j.picked[at], top = m, rest = s;
+  const bool known = label[at] >= 0, lost = __ldcg(j.lost) != 0;  // loaded together
   double loss_of;
   // an infinite logit of the label's own has no loss, as in PyTorch
-  if (label[at] < 0 || z == INFINITY || __ldcg(j.lost) != 0) loss_of = NAN;
+  if (!known | lost | (z == INFINITY)) loss_of = NAN;
   else if (z >= top) loss_of = log1p(rest * exp(top - z));
   else loss_of = top - z + log(rest + exp(z - top));
   j.top[at] = finite_shift(m);  // all others -inf: exp(-inf - 0) is 0
-  j.rest[at] = m == -INFINITY ? 0.f : (float)log2(rest);
+  j.rest[at] = m == -INFINITY ? 0.f : log2f(s);
   j.miss[at] = (float)-expm1(-loss_of);
   if (j.reduction == kLceNone) j.loss[index[at]] = (float)loss_of;
   return loss_of;
@@ -1412,7 +1413,8 @@ lce_join_grad_kernel(const float* __restrict__ acc, int splits, int64_t padded, 
   if (col >= hidden) return;
   if (labels[k] == ignore) *reinterpret_cast<uint4*>(gh + k * hidden + col) = make_uint4(0, 0, 0, 0);
   if (k >= *count) return;
-  float scale = *lost != 0 ? NAN : miss[k];
+  float scale = miss[k];
+  if (*lost != 0) scale = NAN;
   if (inv != nullptr) scale = __fmul_rn(scale, *inv);
   if (g != nullptr) scale = __fmul_rn(scale, *g);
   if (row_g != nullptr) scale = __fmul_rn(scale, row_g[index[k]]);
