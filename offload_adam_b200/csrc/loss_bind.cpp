@@ -130,11 +130,11 @@ void oab::raise_loss_report() {
     __atomic_store_n(at + 1, int64_t(0), __ATOMIC_RELAXED);
     TORCH_CHECK(false, "a kernel of an earlier cross-entropy gave up waiting for its own pipeline; its results are not valid");
   }
-  int64_t label = -1;
-  if (__atomic_load_n(at, __ATOMIC_RELAXED) >= 0) label = __atomic_exchange_n(at, int64_t(-1), __ATOMIC_RELAXED);
-  else if (__atomic_load_n(at + 2, __ATOMIC_RELAXED) != 0) label = __atomic_exchange_n(at + 2, int64_t(0), __ATOMIC_RELAXED);
-  else return;
-  TORCH_CHECK_INDEX(false, "label ", std::to_string(label), " of an earlier cross-entropy is outside its vocabulary; that loss is NaN");
+  if (__atomic_load_n(at, __ATOMIC_RELAXED) < 0 && __atomic_load_n(at + 2, __ATOMIC_RELAXED) == 0) return;
+  // one call may have left one of either kind: both are taken, or the call after the next would raise, too
+  const int64_t above = __atomic_exchange_n(at, int64_t(-1), __ATOMIC_RELAXED), below = __atomic_exchange_n(at + 2, int64_t(0), __ATOMIC_RELAXED);
+  const int64_t label = above >= 0 ? above : below;
+  TORCH_CHECK_INDEX(above < 0 && below == 0, "label ", std::to_string(label), " of an earlier cross-entropy is outside its vocabulary; that loss is NaN");
 }
 
 void bind_loss(py::module_& m) {

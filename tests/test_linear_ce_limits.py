@@ -298,3 +298,19 @@ def test_a_wait_that_gives_up(n, hidden, vocab, piece, reduction):
         assert alone[rows].isnan().all() if one == 0 else alone.isnan().all()
         with pytest.raises(RuntimeError, match="gave up waiting"):
             forward()
+
+
+@gpu
+@pytest.mark.parametrize("n", [20, 300, 5000])
+def test_two_labels_outside_the_vocabulary_raise_once(n):
+    gen = torch.Generator(device="cuda").manual_seed(n)
+    h = torch.randn(n, 64, device="cuda", generator=gen).to(BF16)
+    w = torch.randn(300, 64, device="cuda", generator=gen).to(BF16)
+    labels = torch.randint(0, 300, (n,), device="cuda", generator=gen)
+    want = linear_cross_entropy(h, w, labels)
+    bad = labels.clone()
+    bad[1], bad[n - 1] = 300, -7
+    assert linear_cross_entropy(h, w, bad).isnan()  # waits for it
+    with pytest.raises(IndexError, match="label 300 .* outside its vocabulary"):
+        linear_cross_entropy(h, w, labels)
+    assert torch.equal(linear_cross_entropy(h, w, labels), want)
