@@ -38,7 +38,7 @@ def _gradients(parameters):
 
 
 def _kernels(grads):
-    return grads[0].is_cuda and all(g.dtype in _KERNEL_DTYPES for g in grads) and eager()
+    return grads[0].is_cuda and all(g.dtype in _KERNEL_DTYPES for g in grads) and eager(casts=False)
 
 
 def _once(grads):
@@ -76,7 +76,7 @@ def _run(parameters, norm_type, max_norm, scale, both=False):
         parameters = list(parameters)
     # hundreds of small tensors are bound by what the host does for each of them: the usual case
     # is looked over in C++ (291 tensors: 163 us a call without, 28 with it)
-    if parameters and getattr(parameters[0], "is_cuda", False) and eager():
+    if parameters and getattr(parameters[0], "is_cuda", False) and eager(casts=False):
         out = _ext.load(required=True).param_grad_norm(parameters, code, max_norm, scale, both)
         if out is not None:
             return out
