@@ -5,6 +5,7 @@
 #include <torch/extension.h>
 
 #include <algorithm>
+#include <tuple>
 
 #include "clip_ops.h"
 
@@ -16,11 +17,17 @@ namespace {
 void ok(cudaError_t e, const char* what) { TORCH_CHECK(e == cudaSuccess, what, ": ", cudaGetErrorString(e)); }
 
 // The gradients as ranges of memory; a tensor that does not fill a range of its own is copied,
-// and written back by the caller.  A gradient that stands in the list twice counts once.
+// and written back by the caller, so whatever such tensors share is scaled once.  A gradient that
+// stands in the list twice, whatever tensor it is a view by, counts once.
 struct Gradients {
   std::vector<oab::ClipEntry> entries;
   std::vector<Tensor> copies;                       // keeps them alive
   std::vector<std::pair<Tensor, Tensor>> scattered;  // gradient, its copy
+
+  static bool same(const oab::ClipEntry& a, const oab::ClipEntry& b) { return a.p == b.p && a.n == b.n && a.dtype == b.dtype; }
+  static bool before(const oab::ClipEntry* a, const oab::ClipEntry* b) {
+    return std::tie(a->p, a->n, a->dtype) < std::tie(b->p, b->n, b->dtype);
+  }
 
   Gradients(const std::vector<Tensor>& grads, bool write) {
     entries.reserve(grads.size());
@@ -33,7 +40,8 @@ struct Gradients {
       Tensor x = g;
       if (!g.is_non_overlapping_and_dense()) {
         bool seen = false;
-        for (const auto& [a, b] : scattered) seen = seen || a.is_same(g);
+        for (const auto& [a, b] : scattered)
+          seen = seen || (a.data_ptr() == g.data_ptr() && a.scalar_type() == t && a.sizes() == g.sizes() && a.strides() == g.strides());
         if (seen) continue;
         if (write) {
           const auto z = g.strides();
@@ -50,14 +58,14 @@ struct Gradients {
     order.reserve(entries.size());
     bool sorted = true;
     for (const auto& e : entries) {
-      sorted = sorted && (order.empty() || order.back()->p < e.p);
+      sorted = sorted && (order.empty() || before(order.back(), &e));
       order.push_back(&e);
     }
-    if (!sorted) std::sort(order.begin(), order.end(), [](auto* a, auto* b) { return a->p < b->p; });
+    if (!sorted) std::sort(order.begin(), order.end(), before);
     bool twice = false;
     for (size_t i = 1; i < order.size(); ++i) {
       const auto &a = *order[i - 1], &b = *order[i];
-      if (a.p == b.p && a.n == b.n && a.dtype == b.dtype) twice = true;
+      if (same(a, b)) twice = true;
       else
         TORCH_CHECK_VALUE(static_cast<char*>(a.p) + a.n * (a.dtype == oab::kClipF32 ? 4 : 2) <= b.p,
                           "two gradients share a part of their memory");
@@ -65,7 +73,7 @@ struct Gradients {
     if (twice) {
       std::vector<oab::ClipEntry> once;
       for (size_t i = 0; i < order.size(); ++i)
-        if (i == 0 || order[i]->p != order[i - 1]->p) once.push_back(*order[i]);
+        if (i == 0 || !same(*order[i], *order[i - 1])) once.push_back(*order[i]);
       entries.swap(once);
     }
   }

@@ -41,9 +41,14 @@ def _kernels(grads):
     return grads[0].is_cuda and all(g.dtype in _KERNEL_DTYPES for g in grads) and eager(casts=False)
 
 
+def _dense(g):
+    return torch.ops.aten.is_non_overlapping_and_dense(g)
+
+
 def _once(grads):
-    """Every gradient once, however often it is listed."""
-    return list({(g.data_ptr(), g.dtype, g.shape, g.stride()): g for g in grads if g.numel()}.values())
+    """Every gradient once, however often it is listed and whatever tensor it is a view by."""
+    return list({(g.data_ptr(), g.dtype) + ((g.numel(),) if _dense(g) else (g.shape, g.stride())): g
+                 for g in grads if g.numel()}.values())
 
 
 def _plain(grads, norm_type, max_norm, scale):

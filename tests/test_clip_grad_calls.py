@@ -53,3 +53,31 @@ def test_kernels_run_under_autocast(dtype):
     assert under == launches and all(launches)
     for a, b in zip(got, want):
         assert a.dtype == b.dtype and torch.equal(a, b)
+
+
+def _close(got, want):
+    assert abs(got.item() - want) <= 2.0 ** -23 * want
+
+
+def _check_scaled(tensors, before, coef):
+    for t, b in zip(tensors, before):
+        # the coefficient takes four roundings to fp32, the product one, the result one to bf16
+        assert ((t.double() - coef * b).abs() <= coef * b.abs() * (2.0 ** -8 + 6 * 2.0 ** -24)).all()
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("norm", [2.0, 1.0, math.inf])
+def test_one_gradient_by_several_views(device, norm):
+    """Counts once and is scaled once, with and without gaps, listed one behind the other or not."""
+    base = _random(32, 64, device=device)
+    flat = _random(40 * 30, device=device, seed=1)
+    other = _param(_random(77, device=device, seed=2))
+    views = [base[:, ::2], flat.view(40, 30), base[:, ::2], flat.view(40, 30).T, flat, base[:, ::2]]
+    params = [_param(v) for v in views] + [other]
+    each = [base[:, ::2], flat, other.grad]
+    want = torch.linalg.vector_norm(torch.cat([x.double().reshape(-1) for x in each]), norm).item()
+    before, gaps = [x.double() for x in each], base[:, 1::2].clone()
+    _close(grad_norm(params, norm), want)
+    _close(clip_grad_norm_(params, 0.5 * want, norm), want)
+    _check_scaled(each, before, 0.5)
+    assert torch.equal(base[:, 1::2], gaps)
