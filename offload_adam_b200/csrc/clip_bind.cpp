@@ -66,8 +66,8 @@ struct Gradients {
     for (size_t i = 1; i < order.size(); ++i) {
       const auto &a = *order[i - 1], &b = *order[i];
       if (same(a, b)) twice = true;
-      else
-        TORCH_CHECK_VALUE(static_cast<char*>(a.p) + a.n * (a.dtype == oab::kClipF32 ? 4 : 2) <= b.p,
+      else  // a norm may read both; scaled in place, what they share would be multiplied twice
+        TORCH_CHECK_VALUE(!write || static_cast<char*>(a.p) + a.n * (a.dtype == oab::kClipF32 ? 4 : 2) <= b.p,
                           "two gradients share a part of their memory");
     }
     if (twice) {

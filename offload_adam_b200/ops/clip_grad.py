@@ -51,17 +51,38 @@ def _once(grads):
                  for g in grads if g.numel()}.values())
 
 
+def _check_sharing(grads):
+    """What cannot be scaled in place."""
+    end = 0
+    for g in sorted(filter(_dense, grads), key=lambda g: g.data_ptr()):
+        if g.data_ptr() < end:
+            raise ValueError("two gradients share a part of their memory")
+        end = g.data_ptr() + g.numel() * g.element_size()
+    for g in grads:
+        if any(z == 0 and n > 1 for z, n in zip(g.stride(), g.shape)):
+            raise ValueError("a gradient whose elements share memory cannot be clipped in place")
+
+
 def _plain(grads, norm_type, max_norm, scale):
     """``{coefficient, norm}`` in the operations of PyTorch, summed in fp64."""
     grads = _once(grads)
+    if scale:
+        _check_sharing(grads)
     each = [torch.linalg.vector_norm(g, norm_type, dtype=torch.float64) for g in grads]
     total = torch.linalg.vector_norm(torch.stack(each), norm_type).float() if each else torch.zeros(())
     # a division of two tensors rounds once; a number over a tensor is its reciprocal times the number
     out = torch.stack([(torch.full_like(total, max_norm) / (total + 1e-6)).clamp(max=1.0), total])
     if scale:
-        for g in grads:
+        def scaled(g):
             wide = torch.promote_types(g.dtype, torch.float32)
-            g.copy_(g.to(wide) * out[0].to(wide))
+            return g.to(wide) * out[0].to(wide)
+
+        # those with gaps may share memory with others: all of them before anything is written
+        gaps = [(g, scaled(g)) for g in grads if not _dense(g)]
+        for g in filter(_dense, grads):
+            g.copy_(scaled(g))
+        for g, x in gaps:
+            g.copy_(x)
     return out
 
 

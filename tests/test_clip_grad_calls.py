@@ -81,3 +81,36 @@ def test_one_gradient_by_several_views(device, norm):
     _close(clip_grad_norm_(params, 0.5 * want, norm), want)
     _check_scaled(each, before, 0.5)
     assert torch.equal(base[:, 1::2], gaps)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_gradients_that_share_a_part(device):
+    """A norm reads each of them; scaled in place they are refused, as they stand, unless they have gaps:
+    then what they share is scaled once."""
+    flat = _random(64, device=device)
+    keep = flat.clone()
+    for views in ((flat[:40], flat[24:]), (flat[:40], flat[:41]), (flat[:9], flat[:5], flat[:9])):
+        params = [_param(v) for v in views]
+        once = list({v.numel(): v for v in views}.values()) if len(views) == 3 else views
+        want = math.sqrt(sum(v.double().square().sum().item() for v in once))
+        _close(grad_norm(params), want)
+        for kw in ({}, dict(error_if_nonfinite=True)):
+            with pytest.raises(ValueError, match="share a part"):
+                clip_grad_norm_(params, 0.1, **kw)
+    assert torch.equal(flat, keep)
+    base = _random(32, 64, device=device, seed=3)
+    before = base.double()
+    views = [base[:, :40], base[:, 8:50], base[::2, 5:9], base[:, 50:]]
+    want = math.sqrt(sum(v.double().square().sum().item() for v in views))
+    _close(clip_grad_norm_([_param(v) for v in views], 0.25 * want), want)
+    _check_scaled([base], [before], 0.25)
+    rows = _random(63, device=device, seed=4)
+    before = rows.double()
+    want = rows.double().as_strided((32, 32), (1, 1)).norm().item()
+    _close(clip_grad_norm_([_param(rows.as_strided((32, 32), (1, 1)))], 0.5 * want), want)
+    _check_scaled([rows], [before], 0.5)
+    one = torch.ones(1, device=device, dtype=BF16)
+    with pytest.raises(ValueError, match="share memory"):
+        clip_grad_norm_([_param(one.expand(40))], 0.1)
+    _close(grad_norm([_param(one.expand(40))]), math.sqrt(40))
+    assert one == 1
