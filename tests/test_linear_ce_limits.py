@@ -314,3 +314,40 @@ def test_two_labels_outside_the_vocabulary_raise_once(n):
     with pytest.raises(IndexError, match="label 300 .* outside its vocabulary"):
         linear_cross_entropy(h, w, labels)
     assert torch.equal(linear_cross_entropy(h, w, labels), want)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("reduction", ["mean", "sum", "none"])
+@pytest.mark.parametrize("ignored", [400, -1, -(1 << 62), 1 << 62, 7])
+@pytest.mark.parametrize("n", [5, 70])
+def test_any_label_may_be_the_ignored_one(n, ignored, reduction, device):
+    """Losses and gradients are those with -100 in its place, whatever stands in the ignored rows."""
+    gen = torch.Generator().manual_seed(n)
+    h = torch.randn(n, 64, generator=gen).to(BF16).to(device)
+    w = (torch.randn(300, 64, generator=gen) / 8).to(BF16).to(device).requires_grad_(True)
+    labels = torch.randint(8, 300, (n,), generator=gen).to(device)
+    out = torch.arange(n, device=device) % 3 == 1
+    h[out] = math.nan
+    h.requires_grad_(True)
+    results = []
+    for index in (-100, ignored):
+        loss = linear_cross_entropy(h, w, torch.where(out, index, labels), reduction=reduction, ignore_index=index)
+        gh, gw = torch.autograd.grad(loss.sum(), (h, w))
+        assert loss.isfinite().all() and gw.isfinite().all() and gh.isfinite().all()
+        assert (gh[out] == 0).all() and (reduction != "none" or (loss[out] == 0).all())
+        results.append((loss, gh, gw))
+    for a, b in zip(*results):
+        assert torch.equal(a, b)
+
+
+@gpu
+@pytest.mark.parametrize("n", [5, 100])
+def test_losses_of_a_masked_row_to_the_last_bits(n):
+    """Every word at the lowest value: each logit is one exact product, the label's is the largest, so
+    that log 600 is rounded to fp32 alone."""
+    h = torch.zeros(n, 64, device="cuda", dtype=BF16)
+    h[:, 0] = 1.0
+    w = torch.zeros(600, 64, device="cuda", dtype=BF16)
+    w[:, 0] = torch.finfo(BF16).min
+    loss = linear_cross_entropy(h, w, torch.arange(n, device="cuda"), reduction="none")
+    assert ((loss.double() - math.log(600)).abs() <= 2.0 ** -23 * math.log(600)).all()
