@@ -1638,7 +1638,7 @@ cudaError_t launch_lce_forward(const LceArgs& a, int reduction, float* part, flo
                        sums);
 }
 
-int64_t lce_default_piece(int64_t rows, int64_t hidden, int64_t vocab) {
+int64_t lce_default_piece(int64_t rows, int64_t vocab) {
   const int64_t words = (int64_t(256) << 20) / (2 * lce_padded(rows)) / kTile * kTile;
   const int64_t all = tiles_of(vocab) * kTile;
   const int64_t most = words < all ? words : all;

@@ -74,7 +74,7 @@ inline int64_t lce_piece_pitch(int64_t vocab, int64_t piece) { return ((vocab < 
 // gh goes straight out: its sums are whole after one launch.
 inline bool lce_direct(int64_t vocab, int64_t piece, int splits) { return vocab <= piece && splits == 1; }
 // Words at a time, and splits, when the caller leaves them to the package.
-int64_t lce_default_piece(int64_t rows, int64_t hidden, int64_t vocab);
+int64_t lce_default_piece(int64_t rows, int64_t vocab);
 int lce_splits(int64_t rows, int64_t hidden, int64_t vocab, int64_t piece);
 cudaError_t launch_lce_backward(const LceArgs& a, const LceGrad& g, cudaStream_t st);
 

@@ -121,7 +121,7 @@ struct LinearCE : torch::autograd::Function<LinearCE> {
     const int64_t rows = labels.size(0), hidden = w.size(1), vocab = w.size(0);
     int64_t piece = ctx->saved_data["piece"].toInt();
     piece = std::min({piece, vocab, oab::kLceMaxPiece});
-    piece = piece > 0 ? (piece + oab::kLceTile - 1) / oab::kLceTile * oab::kLceTile : oab::lce_default_piece(rows, hidden, vocab);
+    piece = piece > 0 ? (piece + oab::kLceTile - 1) / oab::kLceTile * oab::kLceTile : oab::lce_default_piece(rows, vocab);
     oab::LceGrad x;
     x.reduction = (int)reduction;
     x.g = gc.data_ptr<float>();
@@ -193,5 +193,4 @@ void bind_linear_ce(py::module_& m) {
   m.def("linear_ce", &linear_ce, py::arg("h"), py::arg("w"), py::arg("labels"), py::arg("reduction"), py::arg("ignore"), py::arg("piece"),
         py::arg("required") = true);
   m.def("linear_ce_wait_limit", &oab::lce_wait_limit, py::arg("nanoseconds"));
-  m.def("linear_ce_piece", &oab::lce_default_piece, py::arg("rows"), py::arg("hidden"), py::arg("vocab"));
 }
