@@ -14,17 +14,16 @@
 //     d_ij = q_i g_i (exp(z_ij - m_i) / s_i - [j = label_i]),    over the other words, as above
 // so the label's entry, which most of a row's gradient hangs on, is -1 exactly in bf16; q_i g_i is
 // applied to the fp32 sums of dh, and to the rows of h that go into dW (bf16, rounded once more).
-// m and log s stay two numbers: their sum would lose the latter beside logits of 1e9, or of a mask's
+// m and log s stay two numbers: their sum would lose the latter beside logits of 1e6, or of a mask's
 // lowest value, and each word of such a row would have the whole of it.
-// tcgen05 cuts off what it adds to an accumulator, towards zero each time: logits of 4096 terms came
-// out 1e-5 too small, the losses of unsure rows 2.5e-5 off.  So the statistics take their logits in
-// chains of 32 additions (512 terms; 256 for few rows) that the epilogue adds up, and the logits that
-// backward forms again in chains of 8192 terms (a logit of 32 is 1e-3 off at most; of 2^18 terms in one
-// chain it was 0.05).  Sums of terms of one
-// sign lose about 1e-7 of their value with each addition of 16 terms (dW of ones over 2^20 rows: 0.7 %,
-// over 2^22: 2.3 %), so an accumulator takes kLceSumTerms of them at most, 4e-4: dW of more rows is
-// summed in fp32 in memory, a launch for every kLceSumTerms rows, and dh of more words in splits (in
-// chains for few rows).
+// tcgen05 cuts off what it adds to an accumulator, towards zero each time: sums of terms of one sign
+// lose 0.4e-7 to 1e-7 of their value with each addition of 16 terms.  Logits of 4096 terms came out 1e-5
+// too small, the losses of unsure rows 2.5e-5 off, so the statistics take their logits in chains of 32
+// additions (512 terms; 256 for few rows) that the epilogue adds up.  The logits that backward forms
+// again come in chains of 8192 terms (of 2^18 terms in one chain, a logit of 32 was 0.05 off).  dW over
+// 2^20 rows was 0.7 % too small, over 2^22 2.3 %, so an accumulator of the gradients takes kLceSumTerms
+// of them, 4e-4 at most: dW of more rows is summed in fp32 in memory, a launch for every kLceSumTerms
+// rows, and dh of more words in splits (in chains for few rows).
 //
 // Forward: one product whose epilogue keeps, per row and 128 words, the maximum and the sum of
 // exponentials (8 bytes for 256 bytes of bf16 logits), and a small kernel that joins them (of a few
@@ -35,8 +34,8 @@
 //
 // What bounds it: the products, at the rate of the library's (4096 rows, hidden 4096, 128256 words on
 // a B200: forward 3.1 ms, 1.37 PFLOP/s, a bf16 product of the library's with nothing behind it 3.1;
-// all 12.7 ms, four products).  Small heads are bound by the exponentials (16 a cycle and SM), few
-// rows by reading W (6.6 TB/s), the smallest calls by the host.
+// all 12.5 to 13.8 ms, four products, as the chip's power allows).  Small heads are bound by the
+// exponentials (16 a cycle and SM), few rows by reading W (6.6 TB/s), the smallest calls by the host.
 //
 // All three products are one pipeline: a CTA pair computes a 256 x 256 tile with tcgen05 (each CTA
 // 128 rows, half of B each), TMA fills six stages of 64 inner values, two accumulators in tensor
@@ -227,8 +226,8 @@ struct Plan {
 // tile, and every other tile of its pair.  A warp is a chain of latencies (the accumulator is
 // done, its load, a fence, the way out), so there are eight for each accumulator, and the accumulator
 // is given back (`release`) with the last load from it, before anything is computed from that.
-// Of the statistics likewise; and of both, unless the sums come in several chains: then all sixteen take
-// 64 columns of every tile.  (4096 rows of 128, 32000 words: 55 us by halves, 78 all together.)
+// Of the statistics likewise.  Where the sums of these or of the logits' gradient come in several chains,
+// all sixteen take 64 columns of every tile.  (4096 rows of 128, 32000 words: 55 us by halves, 78 all together.)
 
 struct RowValues {  // of the packed row that a thread has in a tile
   int label;
@@ -775,6 +774,11 @@ __device__ __forceinline__ double finish_row(const JoinArgs& j, int64_t at, cons
 // (for dh: the hidden columns) are the 128 rows of a tile, one CTA's, and the packed rows its N
 // columns: lanes of tensor memory are words, columns are rows.  A stage is 18 or 24 KB, 16 of
 // them W, so that 12 or 9 stages keep more of W on its way.
+// kLceFewRows is as far as the accumulators go.  The loss alone, and with gradients, us (in brackets as
+// tiles of a pair): 128256 words of 4096, 17 rows 174, 718 (203, 812), 32 rows 195, 723 (235, 874), 64 rows
+// 226, 768 (224, 898).  A small head is bound by the epilogue, which takes the rows one behind the
+// other, and loses by it: 32000 words of 1024, 17 rows 32, 107 (34, 117), 32 rows 41, 117 (34, 118), 64
+// rows 54 to 59, 126 to 135 (29 to 38, 104 to 129).
 constexpr int kFewThreads = 64 + 128;
 // The statistics' last block joins their sums itself, which saves a launch, where its four warps need
 // two turns of 512 partials at most (32000 words of 1024, the loss alone, 8 rows: 28.6 us with the
@@ -1054,8 +1058,8 @@ lce_few_kernel(const __grid_constant__ GemmParams p, float* acc, const JoinArgs 
 // whole, 528 bytes apart (free of bank conflicts), and each lane copies one.  A CTA takes
 // consecutive tiles along the rows of dW: d of its words stays in shared memory and is read once, the
 // rows of h come out of L2 again and again.  32 rows, hidden 8192, 128256 words (h 1 MB, d 16 MB, dW
-// 2.1 GB): 1370 us for loss and gradients, about 375 of them here; with the rows of h kept and d read
-// again, or in the pair kernel, 1460.
+// 2.1 GB), on one GPU in turn: 1370 us for loss and gradients, about 375 of them here; with the rows of h
+// kept and d read again, or in the pair kernel, 1460.
 constexpr int kFewDwStages = 2, kFewDwRow = 528, kFewDwStaging = 32 * kFewDwRow, kFewDwWarps = 8, kFewDwThreads = 64 + 32 * kFewDwWarps;
 constexpr int kFewDwSmem = kFewDwStages * 2 * kHalfBytes + kHalfBytes + kFewDwWarps * kFewDwStaging + 1024;
 __global__ void __launch_bounds__(kFewDwThreads, 1)
@@ -1295,7 +1299,10 @@ lce_pack_kernel(const PackArgs a, const int* __restrict__ index, const int* __re
 
 // Both in one launch for up to kScanPackRows rows: every block looks through all labels (32 KB at
 // most, from L2) for the eight rows that it packs.  One row: 7 us, as two launches 13.
-constexpr int kScanPackRows = 4096, kScanPackBlockRows = 512;  // the latter: a block a row
+// Up to kScanPackBlockRows a row has a block, beyond a warp.  The loss of 256 words of 4096, us, with a
+// block and with a warp: 32 rows 33 and 37, 512 rows 33.4 and 36.6, 768 rows 37.6 and 36.7, 1024 rows 40.0
+// and 36.8.
+constexpr int kScanPackRows = 4096, kScanPackBlockRows = 512;
 template <int THREADS>
 __global__ void __launch_bounds__(kPackThreads)
 lce_scan_pack_kernel(const PackArgs a, const int64_t* __restrict__ labels, int rows, int64_t vocab, int64_t ignore, int* index,
@@ -1488,8 +1495,9 @@ bool encode(CUtensorMap* map, const void* base, int64_t inner, int64_t lines_all
             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-// Launches a kernel that begins with grid_wait: its blocks come up while the last ones of the kernel
-// before it in the stream, one of this file, still run.
+// Launches a kernel that touches no global memory before its grid_wait: its blocks come up while the last
+// ones of the kernel before it in the stream still run, where that one lets them, as those of this file do.
+// The first launch of a backward pass follows whatever ran last.
 template <class... Args, class... Given>
 cudaError_t launch_behind(void (*kernel)(Args...), dim3 grid, int threads, int smem, cudaStream_t st, const Given&... given) {
   cudaLaunchConfig_t c{};

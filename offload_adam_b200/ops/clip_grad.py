@@ -2,7 +2,7 @@
 
 The reference clips inside its offloaded optimizers only (reference:
 src/offload_adam/offload_adam.py:555-561: stack, vector_norm, clamp) and multiplies every
-gradient in a pass of its own.  Here any list of gradients takes one launch for the norm
+gradient in a pass of its own.  Here any 1300 gradients take one launch for the norm
 and one to scale them (``csrc/clip_ops.cu``), and ``Adam`` folds the coefficient into its step.
 """
 
@@ -121,9 +121,9 @@ def grad_norm(parameters, norm_type=2.0):
     """Norm of all gradients of ``parameters`` (a tensor or an iterable) as if they were one
     vector: an fp32 scalar on their device, without a synchronisation.
 
-    ``norm_type`` is 1, 2 or infinity.  Parameters without a gradient are passed over, a
-    gradient that is listed twice counts once; with no gradient at all the norm is 0.
-    The sum is kept in fp64 and has the same bits in every run.
+    ``norm_type`` is 1, 2 or infinity; the gradients are plain dense tensors on one device.  Parameters
+    without a gradient are passed over, a gradient that is listed twice, by whatever view, counts once;
+    with no gradient at all the norm is 0.  The sum is kept in fp64 and has the same bits in every run.
     """
     out = _run(parameters, norm_type, 0.0, False)
     return torch.zeros(()) if out is None else out
@@ -133,9 +133,12 @@ def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=Fals
     """Scales all gradients of ``parameters`` in place so that their norm (see
     :func:`grad_norm`) is at most ``max_norm``; returns the norm before.
 
-    The call of ``torch.nn.utils.clip_grad_norm_``: every gradient is multiplied by
+    Called as ``torch.nn.utils.clip_grad_norm_``: every gradient is multiplied by
     ``min(1, max_norm / (norm + 1e-6))``, in fp32, and rounded once; a coefficient of 1 touches
-    nothing.  ``error_if_nonfinite=True`` waits for the norm and raises, with the gradients as they
+    nothing.  Unlike there, the norm is of order 1, 2 or infinity, all gradients are on one device, tensor
+    subclasses (``DTensor``) are refused, a gradient that is listed twice counts and is scaled once, and
+    gradients that share a part of their memory are refused unless they have gaps (what those share is scaled
+    once).  ``error_if_nonfinite=True`` waits for the norm and raises, with the gradients as they
     were, when it is infinite or NaN.  ``foreach`` is accepted and has no effect.
     """
     max_norm = check_max_norm(max_norm)
