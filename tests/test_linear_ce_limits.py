@@ -357,3 +357,59 @@ def test_losses_of_a_masked_row_to_the_last_bits(n):
     w[:, 0] = torch.finfo(BF16).min
     loss = linear_cross_entropy(h, w, torch.arange(n, device="cuda"), reduction="none")
     assert ((loss.double() - math.log(600)).abs() <= 2.0 ** -23 * math.log(600)).all()
+
+
+@gpu
+@pytest.mark.parametrize("n,hidden,vocab,piece", [(66000, 72, 700, 256), (100, 8264, 300, None), (40, 8264, 1300, 512), (300, 520, 5000, 1024)])
+def test_long_sums_captured_and_replayed(n, hidden, vocab, piece):
+    """Loss and gradients in a graph, replayed on other inputs and another number of rows that count; what
+    ignored rows hold reaches nothing."""
+    gen = torch.Generator(device="cuda").manual_seed(n)
+
+    def inputs():
+        h = torch.randn(n, hidden, device="cuda", generator=gen).to(BF16)
+        w = (torch.randn(vocab, hidden, device="cuda", generator=gen) / math.sqrt(hidden)).to(BF16)
+        labels = torch.randint(0, vocab, (n,), device="cuda", generator=gen)
+        out = torch.rand(n, device="cuda", generator=gen) < 0.5 * torch.rand((), device="cuda", generator=gen)
+        labels[out], h[out] = -100, math.nan
+        return h, w, labels
+
+    def step(x, y, labels):
+        loss = linear_cross_entropy(x, y, labels, piece=piece)
+        return (loss.detach(),) + torch.autograd.grad(loss, (x, y))
+
+    h, w, labels = inputs()
+    x, y = h.requires_grad_(True), w.requires_grad_(True)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.stream(side):
+        step(x, y, labels)
+        with torch.cuda.graph(graph, stream=side):
+            outs = step(x, y, labels)
+    torch.cuda.current_stream().wait_stream(side)
+    for _ in range(3):
+        a, b, c = inputs()
+        want = step(a.requires_grad_(True), b.requires_grad_(True), c)
+        assert want[0].isfinite() and want[1].isfinite().all() and want[2].isfinite().all()
+        with torch.no_grad():
+            x.copy_(a)
+            y.copy_(b)
+            labels.copy_(c)
+        graph.replay()
+        torch.cuda.synchronize()
+        for got, ref in zip(outs, want):
+            assert torch.equal(got, ref)
+
+
+@gpu
+@pytest.mark.parametrize("n", [3, 100])
+def test_in_inference_mode(n):
+    gen = torch.Generator(device="cuda").manual_seed(n)
+    h = torch.randn(n, 64, device="cuda", generator=gen).to(BF16)
+    w = torch.randn(300, 64, device="cuda", generator=gen).to(BF16)
+    labels = torch.randint(0, 300, (n,), device="cuda", generator=gen)
+    for reduction in ("mean", "none"):
+        want = linear_cross_entropy(h, w, labels, reduction=reduction)
+        with torch.inference_mode():
+            assert torch.equal(linear_cross_entropy(h, w, labels, reduction=reduction), want)
